@@ -1,0 +1,212 @@
+// k_rope_append.cu — rotate the new rows' queries and keys and append keys and values to a
+// paged cache, in one launch (sm_100a; include/z2b_ops.h).
+//
+// Pair (a, b) of a head at position s turns by s * w_i:  a' = m (a cos - b sin),
+// b' = m (b cos + a sin). The table holds w_i as a 64-bit fraction of a turn, so s * step
+// wraps modulo one turn and the product is exact: no position is too far for f32 angles
+// (an f32 product s * w is off by 0.06 rad at one million).
+//
+// Bound: bytes (every element is read and written once) for prompts, launch and load
+// latency for decode rows. One warp takes one row: its lanes hold `VEC` pairs each, several
+// heads side by side, and walk the heads with the same pairs, so a lane computes its
+// sines once per row (they cost about as many instructions as rotating a head). Few rows
+// spread a row's heads over several warps instead (blockIdx.y), until the device is full.
+#include "launch.cuh"
+#include "ops.cuh"
+#include "ops.h"
+
+namespace z2b {
+namespace {
+
+struct RopeP {
+    z2b_rope rope;
+    const void *q, *k, *v;
+    void *q_out, *kc, *vc;
+    long long q_row, q_head, o_row, o_head, k_row, k_head, v_row, v_head;
+    long long page_stride, row_stride, head_stride, table_stride;
+    const int *row_off, *seq_len, *table, *pos;
+    uint32_t* err;
+    int n_rows, n_seq, nh, nkv, hd, page_len, n_pages, max_pages, prefix_len;
+};
+
+// VEC consecutive elements as f32, by 16-byte accesses when VEC is 8.
+template <typename T, int VEC> __device__ __forceinline__ void load_vec(const T* p, float (&x)[VEC]) {
+    if constexpr (VEC == 8 && sizeof(T) == 4) {
+        const float4 a = *(const float4*)p, b = *(const float4*)(p + 4);
+        x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+    } else if constexpr (VEC == 8) {
+        const uint4 u = *(const uint4*)p;
+        const T* e = reinterpret_cast<const T*>(&u);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = to_f32(e[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) x[i] = to_f32(p[i]);
+    }
+}
+
+template <typename T, int VEC> __device__ __forceinline__ void store_vec(T* p, const float (&x)[VEC]) {
+    if constexpr (VEC == 8 && sizeof(T) == 4) {
+        *(float4*)p = make_float4(x[0], x[1], x[2], x[3]);
+        *(float4*)(p + 4) = make_float4(x[4], x[5], x[6], x[7]);
+    } else if constexpr (VEC == 8) {
+        uint4 u;
+        T* e = reinterpret_cast<T*>(&u);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) e[i] = from_f32<T>(x[i]);
+        *(uint4*)p = u;
+    } else {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) p[i] = from_f32<T>(x[i]);
+    }
+}
+
+constexpr int ROWS_PER_BLOCK = 4;
+
+// TI: type of q, k, v; TC: of the cache. A unit is VEC pairs of one head: two runs of VEC
+// elements (at a0 and b0) in every layout. VEC 1 takes any alignment and dims.
+template <typename TI, typename TC, int VEC>
+__global__ void __launch_bounds__(32 * ROWS_PER_BLOCK) rope_append_ops_kernel(const __grid_constant__ RopeP p) {
+    const int lane = threadIdx.x & 31, t = blockIdx.x * ROWS_PER_BLOCK + (threadIdx.x >> 5);
+    pdl_wait();
+    pdl_release();
+    if (t >= p.n_rows || t >= p.row_off[p.n_seq]) return;       // padding stays as it is
+    const int b = warp_find_seq(p.row_off, p.n_seq, t);
+    if (b < 0) return;
+    const int lo = p.row_off[b], n = p.row_off[b + 1] - lo;
+    const int len = p.seq_len[b];
+    const long long r = (long long)len - n + (t - lo);          // cache row
+    if (t - lo >= n || r < 0 || r >= (long long)p.max_pages * p.page_len) {
+        if (lane == 0 && p.err) atomicOr(p.err, Z2B_OPS_BAD_INDEX);
+        return;
+    }
+    const long long at = p.pos ? (long long)p.pos[t] : (long long)p.prefix_len + r;
+    int page = 0;
+    bool store = p.k != nullptr;
+    if (store) {
+        page = p.table[(long long)b * p.table_stride + r / p.page_len];
+        if (page < 0 || page >= p.n_pages) {
+            store = false;
+            if (lane == 0 && p.err) atomicOr(p.err, Z2B_OPS_BAD_PAGE);
+        }
+    }
+    const long long crow = (long long)page * p.page_stride + (r % p.page_len) * p.row_stride;
+
+    const int rot = p.rope.rot_dim, half = rot >> 1;
+    const int ur = half / VEC;                                   // rotated units of a head
+    const int units = ur + (p.hd - rot + 2 * VEC - 1) / (2 * VEC);
+    const int side = max(1, 32 / units);                         // heads side by side in a warp
+    const int heads = p.nh + (store ? 2 * p.nkv : 0);
+    const TI *q = (const TI*)p.q, *k = (const TI*)p.k, *v = (const TI*)p.v;
+    for (int u0 = 0; u0 < units; u0 += 32) {
+        const int u = units > 32 ? u0 + lane : lane % units;
+        const int h0 = units > 32 ? 0 : lane / units;
+        if (u >= units || h0 >= side) continue;
+        const bool turns = u < ur;
+        int a0, b0;
+        float cs[VEC], sn[VEC];
+        if (turns) {
+            if (p.rope.layout == Z2B_ROPE_HALF) { a0 = u * VEC; b0 = half + u * VEC; }
+            else { a0 = 2 * u * VEC; b0 = a0 + VEC; }
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+                // signed top half of the wrapped phase: half-turns in [-1, 1)
+                const int top = (int)(((unsigned long long)at * p.rope.step[u * VEC + i]) >> 32);
+                float s, c;
+                sincospif((float)top * 4.6566128730773926e-10f, &s, &c);     // 2^-31
+                cs[i] = c * p.rope.mag;
+                sn[i] = s * p.rope.mag;
+            }
+        } else {
+            a0 = rot + 2 * (u - ur) * VEC;
+            b0 = a0 + VEC;
+        }
+        const bool has_b = VEC > 1 || turns || b0 < p.hd;
+#pragma unroll 2
+        for (int h = h0 + blockIdx.y * side; h < heads; h += gridDim.y * side) {
+            const int kind = h < p.nh ? 0 : h < p.nh + p.nkv ? 1 : 2;       // q, k, v
+            const TI* src = kind == 0 ? q + (long long)t * p.q_row + h * p.q_head
+                          : kind == 1 ? k + (long long)t * p.k_row + (h - p.nh) * p.k_head
+                                      : v + (long long)t * p.v_row + (h - p.nh - p.nkv) * p.v_head;
+            float x[VEC], y[VEC];
+            load_vec<TI, VEC>(src + a0, x);
+            if (has_b) load_vec<TI, VEC>(src + b0, y);
+            if (turns && kind < 2) {
+                if (p.rope.layout == Z2B_ROPE_HALF || VEC == 1) {
+#pragma unroll
+                    for (int i = 0; i < VEC; ++i) {
+                        const float e = x[i], o = y[i];
+                        x[i] = e * cs[i] - o * sn[i];
+                        y[i] = o * cs[i] + e * sn[i];
+                    }
+                } else if constexpr (VEC > 1) {
+                    // the 2 VEC elements are consecutive: pair i is (2i, 2i + 1)
+#pragma unroll
+                    for (int i = 0; i < VEC / 2; ++i) {
+                        const float e = x[2 * i], o = x[2 * i + 1], f = y[2 * i], g = y[2 * i + 1];
+                        x[2 * i] = e * cs[i] - o * sn[i];
+                        x[2 * i + 1] = o * cs[i] + e * sn[i];
+                        y[2 * i] = f * cs[i + VEC / 2] - g * sn[i + VEC / 2];
+                        y[2 * i + 1] = g * cs[i + VEC / 2] + f * sn[i + VEC / 2];
+                    }
+                }
+            }
+            if (kind == 0) {
+                TI* dst = (TI*)p.q_out + (long long)t * p.o_row + h * p.o_head;
+                store_vec<TI, VEC>(dst + a0, x);
+                if (has_b) store_vec<TI, VEC>(dst + b0, y);
+            } else {
+                TC* dst = (TC*)(kind == 1 ? p.kc : p.vc) + crow + (h - p.nh - (kind == 2 ? p.nkv : 0)) * p.head_stride;
+                store_vec<TC, VEC>(dst + a0, x);
+                if (has_b) store_vec<TC, VEC>(dst + b0, y);
+            }
+        }
+    }
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+template <typename TI, typename TC> cudaError_t go(const RopeP& p, bool vec, dim3 grid, cudaStream_t s) {
+    return vec ? launch_pdl(rope_append_ops_kernel<TI, TC, 8>, grid, dim3(32 * ROWS_PER_BLOCK), 0, s, p)
+               : launch_pdl(rope_append_ops_kernel<TI, TC, 1>, grid, dim3(32 * ROWS_PER_BLOCK), 0, s, p);
+}
+
+}  // namespace
+
+cudaError_t launch_rope_append(const z2b_rope_append_args& a, cudaStream_t s) {
+    RopeP p{};
+    const z2b_paged_kv& c = *a.kv;
+    if (a.rope) p.rope = *a.rope;
+    p.q = a.q; p.k = a.k; p.v = a.v; p.q_out = a.q_out; p.kc = c.k; p.vc = c.v;
+    p.q_row = a.q_row; p.q_head = a.q_head; p.o_row = a.o_row; p.o_head = a.o_head;
+    p.k_row = a.k_row; p.k_head = a.k_head; p.v_row = a.v_row; p.v_head = a.v_head;
+    p.page_stride = c.page_stride; p.row_stride = c.row_stride; p.head_stride = c.head_stride;
+    p.table_stride = a.table_stride;
+    p.row_off = a.row_off; p.seq_len = a.seq_len; p.table = a.page_table; p.pos = a.pos; p.err = a.err;
+    p.n_rows = a.n_rows; p.n_seq = a.n_seq; p.nh = a.n_head; p.nkv = c.n_head_kv; p.hd = c.head_dim;
+    p.page_len = c.page_len; p.n_pages = c.n_pages; p.max_pages = a.max_pages; p.prefix_len = a.prefix_len;
+
+    // 16-byte accesses when every run of 8 elements is aligned for both types
+    const long long eight = p.q_row | p.q_head | p.o_row | p.o_head | p.k_row | p.k_head | p.v_row | p.v_head |
+                            p.page_stride | p.row_stride | p.head_stride;
+    const bool vec = p.rope.rot_dim % 16 == 0 && (p.hd - p.rope.rot_dim) % 16 == 0 && eight % 8 == 0 &&
+                     aligned16(p.q) && aligned16(p.k) && aligned16(p.v) && aligned16(p.q_out) && aligned16(p.kc) &&
+                     aligned16(p.vc);
+    const int VEC = vec ? 8 : 1;
+    const int units = (p.rope.rot_dim / 2) / VEC + (p.hd - p.rope.rot_dim + 2 * VEC - 1) / (2 * VEC);
+    const int side = units >= 32 ? 1 : 32 / units;
+    const int heads = p.nh + (p.k ? 2 * p.nkv : 0);
+    const int iters = (heads + side - 1) / side;
+    // a row's heads over `split` warps while that still finds idle schedulers (148 SMs x 8 warps)
+    int split = 1;
+    while (split < iters && (long long)p.n_rows * split < 148 * 8) ++split;
+    const dim3 grid((p.n_rows + ROWS_PER_BLOCK - 1) / ROWS_PER_BLOCK, split);
+    if (a.type == Z2B_TYPE_F32)
+        return c.type == Z2B_TYPE_F16 ? go<float, __half>(p, vec, grid, s) : go<float, __nv_bfloat16>(p, vec, grid, s);
+    if (a.type == Z2B_TYPE_F16)
+        return c.type == Z2B_TYPE_F16 ? go<__half, __half>(p, vec, grid, s) : go<__half, __nv_bfloat16>(p, vec, grid, s);
+    return c.type == Z2B_TYPE_F16 ? go<__nv_bfloat16, __half>(p, vec, grid, s)
+                                  : go<__nv_bfloat16, __nv_bfloat16>(p, vec, grid, s);
+}
+
+}  // namespace z2b
