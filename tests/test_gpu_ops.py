@@ -214,6 +214,13 @@ ATTNS = [
     ([1], [5000], 64, 2, 1, 128, F16, 0, False, 0),                      # one long stream over many CTAs
     ([20] * 4, [20, 33, 90, 64], 16, 2, 1, 128, BF16, 500, False, 0),
     ([9, 17], [64, 128], 40, 12, 2, 16, F16, 0, False, 0),
+    # prefixes of many rows (256-row tiles): borders of tiles and units, tiles half empty, wide groups
+    ([1] * 20, [2] * 20, 256, 16, 4, 128, F16, 128, False, 0),           # 80 rows a key head, one unit
+    ([1] * 33, [1] * 33, 64, 16, 2, 64, BF16, 129, False, 5),            # 264 rows: eight in the second tile
+    ([5] * 13, [70] * 13, 16, 6, 2, 64, F16, 257, True, 0),              # 195 rows, pages of 16
+    ([1] * 100, [3] * 100, 8, 6, 1, 128, BF16, 1000, False, 0),          # 600 rows, pages of 8
+    ([3, 0, 90], [3, 9, 95], 48, 4, 1, 128, F16, 127, False, 9),         # a prompt chunk over the prefix
+    ([1] * 65, [1] * 65, 32, 1, 1, 64, BF16, 3000, False, 0),            # one head; 65 rows
 ]
 
 

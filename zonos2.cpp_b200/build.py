@@ -29,7 +29,7 @@ HOST_COMMON = ["gguf.cpp", "quant.cpp"]
 Z2B_HOST = ["repack.cpp", "model.cpp", "runtime.cpp", "capi.cpp", "dac.cpp", "capi_dac.cpp", "prompt.cpp",
             "capi_ops.cpp"]
 Z2B_CUDA = ["k_gemv.cu", "k_gemm.cu", "k_attn.cu", "k_router.cu", "k_misc.cu", "k_test.cu", "k_dac.cu",
-            "k_rope_append.cu", "k_prefix_attn.cu", "k_verify.cu"]
+            "k_rope_append.cu", "k_prefix_attn.cu", "k_prefix_tc.cu", "k_verify.cu"]
 
 
 def _headers():

@@ -17,103 +17,17 @@
 // advances one of the two, so slots never collide and their number is bounded by
 // segments + CTAs. Nothing is accumulated by atomics: the same call gives the same bits.
 #include "launch.cuh"
-#include "ops.cuh"
 #include "ops.h"
-#include "tc05.cuh"
+#include "prefix_attn.cuh"
 
 #include <atomic>
 
 namespace z2b {
 namespace {
 
-constexpr int KT = 64;                 // keys per unit
 constexpr int COMPUTE_WARPS = 4;
 constexpr int THREADS = 32 * (COMPUTE_WARPS + 1);
 constexpr int MAX_SMEM = 200 * 1024;   // dynamic shared memory a launch may ask for
-constexpr int MIN_UNITS = 2;           // units per CTA at least, before more CTAs are used
-
-struct AttnP {
-    const void* q;
-    long long q_row, q_head, table_stride;
-    const int *row_off, *seq_len, *table, *prefix_pages;
-    uint32_t* err;
-    int n_rows, n_seq, nkv, G, page_len, n_pages, max_pages, prefix_len;
-    int box_rows;                      // rows of one TMA box: a power of two that divides page_len, at most KT
-    float scale2;                      // scale * log2(e)
-    int pf_row_tiles;                  // row tiles of the prefix in this launch (0: none)
-    int own;                           // 1: the streams' own segments are in this launch
-    int stages, max_slots;
-    int after_prefix;                  // 1: the launch before is the prefix's, which this one runs beside
-    float* part_o;                     // [max_slots][MT][HD]
-    float2* part_ml;                   // [max_slots][MT] (m in log2 units, l)
-    int* plan;                         // [2][n_seq + 1] unit and segment offsets of the streams, written for the join
-};
-
-__device__ __forceinline__ int cdiv(int a, int b) { return (a + b - 1) / b; }
-
-// One stream's extent, with offsets and lengths that are out of range cut to nothing.
-struct SeqInfo { int lo, n, len, nt, qt; bool bad; };
-template <int MT> __device__ __forceinline__ SeqInfo seq_info(const AttnP& p, int b) {
-    SeqInfo s;
-    const int lo = p.row_off[b], hi = p.row_off[b + 1], len = p.seq_len[b];
-    const long long cap = (long long)p.max_pages * p.page_len;
-    s.bad = lo < 0 || hi < lo || hi > p.n_rows || len < 0 || len > cap;
-    s.lo = lo;
-    s.n = s.bad ? 0 : hi - lo;
-    s.len = s.bad ? 0 : len;
-    s.nt = s.n ? cdiv(s.len, KT) : 0;
-    s.qt = cdiv(s.n * p.G, MT);
-    return s;
-}
-
-// Which CTA of `ctas` holds unit u of a line of W: the i with W i / ctas <= u < W (i + 1) / ctas.
-__device__ __forceinline__ int unit_owner(long long u, long long W, int ctas) {
-    return (int)(((u + 1) * ctas - 1) / W);
-}
-__device__ __forceinline__ int line_ctas(long long W, int grid) {
-    return (int)max(1ll, min((long long)grid, W / MIN_UNITS));
-}
-
-template <typename T> __device__ __forceinline__ void mma_t(float* d, const uint32_t* a, uint32_t b0, uint32_t b1);
-template <> __device__ __forceinline__ void mma_t<__half>(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
-    mma16816(d, a[0], a[1], a[2], a[3], b0, b1);
-}
-template <> __device__ __forceinline__ void mma_t<__nv_bfloat16>(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 "
-        "{%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float hi);
-template <> __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
-    const __half2 h = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&h);
-}
-template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&h);
-}
-
-__device__ __forceinline__ void ldsm4(uint32_t a, uint32_t (&r)[4]) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
-}
-__device__ __forceinline__ void ldsm4t(uint32_t a, uint32_t (&r)[4]) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
-}
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, int w, uint64_t* bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
-        :: "r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar)) : "memory");
-}
-__device__ __forceinline__ void compute_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
 
 // Shared-memory tile of 64 rows of one key head: rows of RB bytes (at most 128: head_dim 128
 // is two halves), 16-byte chunks XOR-swizzled as the TMA box writes them.
@@ -468,7 +382,7 @@ __global__ void __launch_bounds__(THREADS) prefix_attn_kernel(const __grid_const
 struct PartSet {                        // partial results of one launch
     const float* o;
     const float2* ml;
-    int mt, grid, max_slots;
+    int mt, kt, grid, max_slots;       // rows of a partial, keys of a unit
 };
 struct JoinP {
     AttnP a;
@@ -535,12 +449,12 @@ __global__ void __launch_bounds__(256) prefix_attn_join_kernel(const __grid_cons
             }
         }
     };
-    const int pf_nt = cdiv(a.prefix_len, KT), pf_units = a.pf_row_tiles * a.nkv * pf_nt;
+    const int pf_units = a.pf_row_tiles * a.nkv * cdiv(a.prefix_len, KT);
     const int* units = a.plan;
     const long long W = (long long)pf_units + units[a.n_seq];
     {
         const PartSet& ps = p.pf.o ? p.pf : p.own;
-        const int r = t * a.G + g, seg = (r / ps.mt) * a.nkv + h;
+        const int r = t * a.G + g, seg = (r / ps.mt) * a.nkv + h, pf_nt = cdiv(a.prefix_len, ps.kt);
         const long long Wp = p.pf.o ? (long long)cdiv(a.n_rows * a.G, ps.mt) * a.nkv * pf_nt : W;
         add(ps, Wp, (long long)seg * pf_nt, pf_nt, seg, r % ps.mt);
     }
@@ -567,7 +481,8 @@ struct HostPlan {
     int G, wm, mt;                      // own rows per segment
     int grid, own_slots, pf_rt;         // pf_rt > 0: prefix row tiles inside the own launch
     bool pf_apart;                      // the prefix has a launch of its own
-    int pf_mt, pf_tiles, pf_grid, pf_slots;
+    bool pf_tc;                         // ... on the tcgen05 kernel
+    int pf_mt, pf_kt, pf_tiles, pf_grid, pf_slots;
     size_t off_own_ml, off_own_o, off_pf_ml, off_pf_o, bytes;
 };
 
@@ -588,9 +503,12 @@ HostPlan host_plan(const z2b_prefix_attn_args& a) {
         if (rt <= 2) h.pf_rt = (int)rt;
         else {
             h.pf_apart = true;
-            h.pf_mt = 64;
+            // more rows than one warp-level tile holds: 256-row tiles on tcgen05 (one CTA per SM)
+            h.pf_tc = hd >= 64 && R > 64 && a.scale != 0.0f;
+            h.pf_mt = h.pf_tc ? TC_ROWS : 64;
+            h.pf_kt = h.pf_tc ? TC_KEYS : KT;
             h.pf_tiles = (int)((R + h.pf_mt - 1) / h.pf_mt);
-            h.pf_grid = 148 * 2;
+            h.pf_grid = h.pf_tc ? 148 : 148 * 2;
             h.pf_slots = h.pf_tiles * nkv + h.pf_grid;
         }
     }
@@ -658,7 +576,9 @@ cudaError_t go_all(const z2b_prefix_attn_args& a, const HostPlan& h, cudaStream_
         f.max_slots = h.pf_slots;
         f.part_ml = (float2*)(ws + h.off_pf_ml);
         f.part_o = (float*)(ws + h.off_pf_o);
-        if ((e = go_attn<T, HD, 4>(f, km, vm, h.pf_grid, s)) != cudaSuccess) return e;
+        if constexpr (HD >= 64) e = h.pf_tc ? launch_prefix_tc<T, HD>(f, km, vm, h.pf_grid, s) : go_attn<T, HD, 4>(f, km, vm, h.pf_grid, s);
+        else e = go_attn<T, HD, 4>(f, km, vm, h.pf_grid, s);
+        if (e != cudaSuccess) return e;
     }
     p.own = 1;
     p.pf_row_tiles = h.pf_rt;
@@ -671,8 +591,8 @@ cudaError_t go_all(const z2b_prefix_attn_args& a, const HostPlan& h, cudaStream_
     if (e != cudaSuccess) return e;
     JoinP j{};
     j.a = p;
-    j.own = PartSet{p.part_o, p.part_ml, h.mt, h.grid, h.own_slots};
-    if (h.pf_apart) j.pf = PartSet{(float*)(ws + h.off_pf_o), (float2*)(ws + h.off_pf_ml), h.pf_mt, h.pf_grid, h.pf_slots};
+    j.own = PartSet{p.part_o, p.part_ml, h.mt, KT, h.grid, h.own_slots};
+    if (h.pf_apart) j.pf = PartSet{(float*)(ws + h.off_pf_o), (float2*)(ws + h.off_pf_ml), h.pf_mt, h.pf_kt, h.pf_grid, h.pf_slots};
     j.out = a.out; j.o_row = a.o_row; j.o_head = a.o_head; j.lse = a.lse;
     const dim3 grid((unsigned)(((long long)a.n_rows * a.n_head + 7) / 8));
     if (h.wm == 1) return launch_pdl(prefix_attn_join_kernel<T, HD, 16>, grid, dim3(256), 0, s, j);
