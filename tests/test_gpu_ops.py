@@ -489,3 +489,24 @@ def test_python_refusals():
             f()
     none = ops.prefix_attention(s.kv, q[:0], _i32([0, 0]), s.d_lens, s.d_table)
     assert none.shape == (0, 4, 64)
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.2, 1.0], ids=str)
+def test_prefix_attention_scales(scale):
+    """A scale of zero (all keys alike) and a negative one, few rows and many."""
+    for B in (2, 30):
+        s = Streams([1] * B, [3] * B, 16, 2, 64, F16, prefix=140, seed=14)
+        q = torch.randn((B, 8, 64), generator=_gen(15)).to(F16).to(DEV)
+        out, lse = ops.prefix_attention(s.kv, q, s.d_off, s.d_lens, s.d_table, s.d_shared, 140, scale=scale, lse=True, err=s.err)
+        ops.check(s.err)
+        _check_attention(s, q, out, lse, scale=scale)
+
+
+def test_prefix_attention_many_streams():
+    """More streams than one block holds records for at full width."""
+    B = 1500
+    s = Streams([1 if b % 3 else 0 for b in range(B)], [1 + b % 70 for b in range(B)], 16, 1, 64, F16, prefix=20, seed=16)
+    q = torch.randn((s.rows, 2, 64), generator=_gen(17)).to(F16).to(DEV)
+    out, lse = ops.prefix_attention(s.kv, q, s.d_off, s.d_lens, s.d_table, s.d_shared, 20, lse=True, err=s.err)
+    ops.check(s.err)
+    _check_attention(s, q, out, lse)

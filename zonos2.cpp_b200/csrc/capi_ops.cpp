@@ -135,7 +135,7 @@ static const char* check_attn(const z2b_prefix_attn_args& a, int* rc) {
     if (a.n_seq > OPS_MAX_SEQ) return "prefix_attention: more than 4096 streams";
     // unit and slot numbers are 32-bit
     const long long G = a.n_head / c.n_head_kv, tiles = ((long long)a.n_rows * G + 15) / 16;
-    const long long own = ((long long)a.max_pages * c.page_len + 63) / 64, pf = ((long long)a.prefix_len + 63) / 64;
+    const long long own = ((long long)a.max_pages * c.page_len + 31) / 32, pf = ((long long)a.prefix_len + 31) / 32;
     if (tiles * c.n_head_kv > (1 << 24) || (long long)a.n_seq * c.n_head_kv > (1 << 24) || own > (1 << 24) ||
         (tiles + a.n_seq) * c.n_head_kv * own > 0x7fffffffll || (tiles + 1) * c.n_head_kv * pf > 0x7fffffffll)
         return "prefix_attention: too many rows, streams or pages for one call";

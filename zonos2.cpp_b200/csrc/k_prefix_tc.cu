@@ -118,7 +118,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) prefix_tc_kernel(const __grid_c
     const int live_rows = max(0, min(p.n_rows, p.row_off[p.n_seq])) * p.G;
     const int nt = cdiv(p.prefix_len, TC_KEYS);
     const long long W = (long long)p.pf_row_tiles * p.nkv * nt;
-    const int ctas = line_ctas(W, gridDim.x);
+    const int ctas = line_workers(W, gridDim.x);
     int u0 = 0, u1 = 0;
     if ((int)blockIdx.x < ctas) {
         u0 = (int)(W * blockIdx.x / ctas);
@@ -133,8 +133,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) prefix_tc_kernel(const __grid_c
         int it = 0;
         bool ok = true;
         for (int u = u0; u < u1 && ok;) {
-            const int seg = u / nt, end = min(u1, (seg + 1) * nt), h = seg % p.nkv;
-            if (live_tiles(seg / p.nkv, live_rows) == 0) { u = end; continue; }
+            const int seg = u / nt, end = min(u1, (seg + 1) * nt), h = seg / p.pf_row_tiles;
+            if (live_tiles(seg % p.pf_row_tiles, live_rows) == 0) { u = end; continue; }
             for (; u < end && ok; ++u) {
                 const int key0 = (u - seg * nt) * TC_KEYS;
 #pragma unroll 1
@@ -192,7 +192,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) prefix_tc_kernel(const __grid_c
             };
             for (int u = u0; u < u1 && ok;) {
                 const int seg = u / nt, end = min(u1, (seg + 1) * nt), n = end - u;
-                const int nl = live_tiles(seg / p.nkv, live_rows);
+                const int nl = live_tiles(seg % p.pf_row_tiles, live_rows);
                 u = end;
                 if (nl == 0) continue;
                 wait(&kv_full[2 * c % stages], 2 * c / stages);
@@ -244,13 +244,14 @@ __global__ void __launch_bounds__(TC_THREADS, 1) prefix_tc_kernel(const __grid_c
         const uint32_t ts = tm + lanes + S_COL + t * 128, to = tm + lanes + O_COL + t * HD;
         uint8_t* qt = smem + t * TILE;
         const bool flip = p.scale2 < 0.0f;                       // the maximum of s * scale is taken on s: negate Q instead
-        const float sc = fabsf(p.scale2);
+        const bool flat = p.scale2 == 0.0f;                      // all scores equal: zero Q, so that masked keys stay apart
+        const float sc = flat ? 1.0f : fabsf(p.scale2);
         const bool q16 = ((reinterpret_cast<uintptr_t>(p.q) | (uintptr_t)(p.q_row * 2) | (uintptr_t)(p.q_head * 2)) & 15) == 0;
         int c = 0, ct = 0;
         bool ok = true;
         for (int u = u0; u < u1 && ok;) {
             const int seg = u / nt, end = min(u1, (seg + 1) * nt), n = end - u, key_first = (u - seg * nt) * TC_KEYS;
-            const int j = seg / p.nkv, h = seg % p.nkv, nl = live_tiles(j, live_rows);
+            const int j = seg % p.pf_row_tiles, h = seg / p.pf_row_tiles, nl = live_tiles(j, live_rows);
             u = end;
             if (t >= nl) { c += nl ? n : 0; continue; }
             // Q_t: this thread's row, swizzled by 16-byte chunks
@@ -261,8 +262,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) prefix_tc_kernel(const __grid_c
 #pragma unroll
                 for (int k = 0; k < HD / 8; ++k) {
                     uint4 v = make_uint4(0, 0, 0, 0);
-                    if (live && q16) v = *(const uint4*)(src + k * 8);
-                    else if (live) {
+                    if (live && !flat && q16) v = *(const uint4*)(src + k * 8);
+                    else if (live && !flat) {
                         const uint32_t* w = (const uint32_t*)(src + k * 8);
                         v = make_uint4(w[0], w[1], w[2], w[3]);
                     }

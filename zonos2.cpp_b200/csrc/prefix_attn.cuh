@@ -11,9 +11,9 @@
 
 namespace z2b {
 
-constexpr int KT = 64;                 // keys of a unit on the warp-level kernel
+constexpr int KU = 32;                 // keys of a unit on the warp-level kernel
 constexpr int TC_ROWS = 256, TC_KEYS = 128;    // rows of a segment and keys of a unit on tcgen05
-constexpr int MIN_UNITS = 2;           // units per CTA at least, before more CTAs are used
+constexpr int MIN_UNITS = 2;           // units per worker at least, before more workers are used
 
 struct AttnP {
     const void* q;
@@ -21,14 +21,13 @@ struct AttnP {
     const int *row_off, *seq_len, *table, *prefix_pages;
     uint32_t* err;
     int n_rows, n_seq, nkv, G, page_len, n_pages, max_pages, prefix_len;
-    int box_rows;                      // rows of one TMA box: a power of two that divides page_len, at most KT
+    int box_rows;                      // rows of one TMA box: a power of two that divides page_len, at most a unit's keys
     float scale2;                      // scale * log2(e)
     int pf_row_tiles;                  // row tiles of the prefix in this launch (0: none)
-    int own;                           // 1: the streams' own segments are in this launch
-    int stages, max_slots;
+    int max_slots;
     int after_prefix;                  // 1: the launch before is the prefix's, which this one runs beside
-    float* part_o;                     // [max_slots][MT][HD]
-    float2* part_ml;                   // [max_slots][MT] (m in log2 units, l)
+    float* part_o;                     // [max_slots][rows of a segment][head_dim]
+    float2* part_ml;                   // [max_slots][rows of a segment] (m in log2 units, l)
     int* plan;                         // [2][n_seq + 1] unit and segment offsets of the streams, written for the join
 };
 
@@ -44,17 +43,17 @@ template <int MT> __device__ __forceinline__ SeqInfo seq_info(const AttnP& p, in
     s.lo = lo;
     s.n = s.bad ? 0 : hi - lo;
     s.len = s.bad ? 0 : len;
-    s.nt = s.n ? cdiv(s.len, KT) : 0;
+    s.nt = s.n ? cdiv(s.len, KU) : 0;
     s.qt = cdiv(s.n * p.G, MT);
     return s;
 }
 
-// Which CTA of `ctas` holds unit u of a line of W: the i with W i / ctas <= u < W (i + 1) / ctas.
-__device__ __forceinline__ int unit_owner(long long u, long long W, int ctas) {
-    return (int)(((u + 1) * ctas - 1) / W);
+// Which of `workers` holds unit u of a line of W: the i with W i / workers <= u < W (i + 1) / workers.
+__device__ __forceinline__ int unit_owner(long long u, long long W, int workers) {
+    return (int)(((u + 1) * workers - 1) / W);
 }
-__device__ __forceinline__ int line_ctas(long long W, int grid) {
-    return (int)max(1ll, min((long long)grid, W / MIN_UNITS));
+__device__ __forceinline__ int line_workers(long long W, int most) {
+    return (int)max(1ll, min((long long)most, W / MIN_UNITS));
 }
 
 template <typename T> __device__ __forceinline__ void mma_t(float* d, const uint32_t* a, uint32_t b0, uint32_t b1);
@@ -96,10 +95,9 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map
         "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
         :: "r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar)) : "memory");
 }
-__device__ __forceinline__ void compute_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
 
 // The prefix on tcgen05 (k_prefix_tc.cu): segments of TC_ROWS rows, units of TC_KEYS keys.
-// head_dim 64 or 128, scale not zero.
+// head_dim 64 or 128.
 template <typename T, int HD>
 cudaError_t launch_prefix_tc(const AttnP& p, const CUtensorMap& km, const CUtensorMap& vm, int grid, cudaStream_t s);
 
