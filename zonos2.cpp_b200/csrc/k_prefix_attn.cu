@@ -19,7 +19,7 @@
 //
 // A worker is ONE WARP with a TMA ring of its own, so that no barrier ties warps together and
 // the loads of a warp's next units stay in flight while it finishes a segment or fetches the
-// next one's queries; together the rings of an SM hold 192 KB in flight.
+// next one's queries; together the rings of an SM hold 192 KB.
 #include "launch.cuh"
 #include "ops.h"
 #include "prefix_attn.cuh"
@@ -27,13 +27,17 @@
 namespace z2b {
 namespace {
 
-// Warps of a CTA (one CTA per SM) and ring stages of a warp: 16, 8, 4 and 2 KB stages.
-__host__ __device__ constexpr int max_warps(int hd) { return hd == 128 ? 6 : 8; }
+// Keys of a unit, ring stages of a warp (of 16, 8, 4 and 2 KB), and warps of a CTA (one CTA per
+// SM): as many as registers and shared memory hold.
+__host__ __device__ constexpr int unit_keys(int hd) { return 32; }
 __host__ __device__ constexpr int ring_stages(int hd) { return hd == 128 ? 2 : hd == 64 ? 3 : hd == 32 ? 6 : 8; }
+__host__ __device__ constexpr int max_warps(int hd) { return hd == 128 ? 6 : 8; }
+constexpr int MAX_SMEM = 226 * 1024;   // dynamic shared memory of a launch
 
 // Shared-memory tile of KU rows of one key head: rows of RB bytes (at most 128: head_dim 128
 // is two halves), 16-byte chunks XOR-swizzled as the TMA box writes them.
 template <int HD> struct Tile {
+    static constexpr int KU = unit_keys(HD);
     static constexpr int INNER = HD < 64 ? HD : 64;              // elements of one box row
     static constexpr int HALVES = HD / INNER;
     static constexpr int RB = INNER * 2;
@@ -50,20 +54,23 @@ template <int HD> struct Tile {
 struct Line {
     const int4* rec;                   // [n_seq + 1] first unit, first segment, first row, rows
     const int* len;                    // [n_seq]
-    int pf_nt, pf_units, total_rows;
+    int pf_nt, pf_units, total_rows;   // units of a prefix segment, line positions of all of them
 };
 struct Seg {
-    int h, j, seg, unit0, nt;          // key head, row tile, segment id, first unit, units
+    int h, j, seg, unit0, nt;          // key head, row tile, segment id, position of its first unit, units
     int lo, n, klen, lim_max;          // first row, rows, keys, keys that the tile's last row sees
     const int* pages;
+    bool prefix;
 };
 
-template <int MT> __device__ __forceinline__ Seg find_seg(const AttnP& p, const Line& ln, int u) {
+template <int MT, int KU> __device__ __forceinline__ Seg find_seg(const AttnP& p, const Line& ln, int u) {
     Seg g;
     if (u < ln.pf_units) {
-        g.seg = u / ln.pf_nt;
-        g.unit0 = g.seg * ln.pf_nt;
+        const int size = ln.pf_nt + SEG_COST;
+        g.seg = u / size;
+        g.unit0 = g.seg * size + SEG_COST;
         g.nt = ln.pf_nt;
+        g.prefix = true;
         g.h = g.seg / p.pf_row_tiles;
         g.j = g.seg % p.pf_row_tiles;
         g.lo = 0;
@@ -83,24 +90,27 @@ template <int MT> __device__ __forceinline__ Seg find_seg(const AttnP& p, const 
     g.n = r.w;
     g.klen = ln.len[lo];
     g.nt = cdiv(g.klen, KU);
-    const int qt = cdiv(g.n * p.G, MT), js = (v - r.x) / g.nt;
+    g.prefix = false;
+    const int size = g.nt + SEG_COST, qt = cdiv(g.n * p.G, MT), js = (v - r.x) / size;
     g.seg = p.pf_row_tiles * p.nkv + r.y + js;
-    g.unit0 = ln.pf_units + r.x + js * g.nt;
+    g.unit0 = ln.pf_units + r.x + js * size + SEG_COST;
     g.h = js / qt;
     g.j = js % qt;
-    const int last = min(g.n - 1, (g.j * MT + MT - 1) / p.G);
+    const int last = min(g.n - 1, div_g(p, g.j * MT + MT - 1));
     g.lim_max = min(g.klen, g.klen - g.n + last + 1);
     g.pages = p.table + (long long)lo * p.table_stride;
     return g;
 }
 
-// M16 blocks of 16 rows per segment: 2 when a stream has more than 16 rows of a key head, so
-// that its keys are read once for all of them.
-template <typename T, int HD, int M16>
+// A segment has MT = 8 NB rows. The products are taken transposed, keys and dims on the tensor
+// core's 16-row side and the rows on its 8-column side, since decode has few rows:
+//   S^T[16 keys][8 rows] = K Q^T ,  O^T[16 dims][8 rows] += V^T P^T .
+// P^T comes out of S^T's accumulator layout by one 8 x 8 transpose per tile.
+template <typename T, int HD, int NB>
 __global__ void __launch_bounds__(32 * max_warps(HD), 1) prefix_attn_kernel(const __grid_constant__ AttnP p,
                                                                            const __grid_constant__ CUtensorMap kmap,
                                                                            const __grid_constant__ CUtensorMap vmap) {
-    constexpr int MT = 16 * M16, KS = HD / 16, NT = KU / 8, DT = HD / 8;
+    constexpr int MT = 8 * NB, KU = unit_keys(HD), KS = HD / 16, KM = KU / 16, DT = HD / 16;
     constexpr int STAGE = 2 * Tile<HD>::BYTES, NS = ring_stages(HD);
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
@@ -108,7 +118,8 @@ __global__ void __launch_bounds__(32 * max_warps(HD), 1) prefix_attn_kernel(cons
     __shared__ int s_scan[2][max_warps(HD)];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nw = blockDim.x >> 5;
     uint8_t* ring = smem + (size_t)warp * NS * STAGE;
-    int4* s_rec = (int4*)(smem + (size_t)nw * NS * STAGE);
+    uint8_t* s_q = smem + (size_t)nw * NS * STAGE + (size_t)warp * MT * HD * 2;
+    int4* s_rec = (int4*)(smem + (size_t)nw * (NS * STAGE + MT * HD * 2));
     int* s_len = (int*)(s_rec + p.n_seq + 1);
     uint64_t* full = s_full[warp];
 
@@ -124,11 +135,11 @@ __global__ void __launch_bounds__(32 * max_warps(HD), 1) prefix_attn_kernel(cons
         const int b0 = min(p.n_seq, (int)threadIdx.x * per), b1 = min(p.n_seq, b0 + per);
         int su = 0, sg = 0;
         for (int b = b0; b < b1; ++b) {
-            const SeqInfo s = seq_info<MT>(p, b);
+            const SeqInfo s = seq_info<MT, KU>(p, b);
             if (s.bad && blockIdx.x == 0 && p.err) atomicOr(p.err, Z2B_OPS_BAD_INDEX);
             s_rec[b] = make_int4(su, sg, s.lo, s.n);
             s_len[b] = s.len;
-            su += s.qt * p.nkv * s.nt;
+            su += s.nt ? s.qt * p.nkv * (s.nt + SEG_COST) : 0;
             sg += s.qt * p.nkv;
         }
         int iu = su, ig = sg;
@@ -156,7 +167,7 @@ __global__ void __launch_bounds__(32 * max_warps(HD), 1) prefix_attn_kernel(cons
     ln.len = s_len;
     ln.total_rows = max(0, min(p.n_rows, p.row_off[p.n_seq]));
     ln.pf_nt = cdiv(p.prefix_len, KU);
-    ln.pf_units = p.pf_row_tiles * p.nkv * ln.pf_nt;
+    ln.pf_units = p.pf_row_tiles * p.nkv * (ln.pf_nt + SEG_COST);
     __syncthreads();
     const long long W = (long long)ln.pf_units + s_rec[p.n_seq].x;
     const int workers = line_workers(W, gridDim.x * nw);
@@ -167,35 +178,51 @@ __global__ void __launch_bounds__(32 * max_warps(HD), 1) prefix_attn_kernel(cons
         u1 = (int)(W * (me + 1) / workers);
     }
 
-    // ---- the copies, NS units ahead of the products: one TMA box per lane
-    const int nb = KU / p.box_rows, jobs = 2 * nb * Tile<HD>::HALVES;   // at most 16
-    const int rb = lane % nb, half = lane / nb % Tile<HD>::HALVES, isv = lane / nb / Tile<HD>::HALVES;
-    const uint32_t box_dst = smem_u32(ring) + isv * Tile<HD>::BYTES + half * (KU * Tile<HD>::RB) + rb * p.box_rows * Tile<HD>::RB;
+    // ---- the copies, NS units ahead of the products: a box of K and one of V per run of rows
+    // that stays within a page; lane i looks up run i's page
+    const int nb = KU / p.box_rows;                              // at most 4
     Seg gi;                            // segment of the next unit to copy
     gi.unit0 = -1;
     gi.nt = 0;
-    int ui = u, issued = 0, page = 0;
+    int ui = u, issued = 0, page = 0, pidx = 0, prow = 0;        // this lane's box: page id, its index, row in it
     auto look_up = [&] {               // move ui to the next unit that some row sees; this lane's page of it
-        for (; ui < u1; ui = gi.unit0 + gi.nt) {                 // keys only rise: behind an unseen unit all are
-            if (ui >= gi.unit0 + gi.nt) gi = find_seg<MT>(p, ln, ui);
+        prow += KU;
+        while (prow >= p.page_len) { prow -= p.page_len; ++pidx; }
+        while (ui < u1) {
+            if (ui >= gi.unit0 + gi.nt) {
+                gi = find_seg<MT, KU>(p, ln, ui);
+                ui = max(ui, gi.unit0);
+                const int key = (ui - gi.unit0) * KU + lane * p.box_rows;
+                pidx = key / p.page_len;
+                prow = key % p.page_len;
+            }
             if ((ui - gi.unit0) * KU < gi.lim_max) break;
+            ui = gi.unit0 + gi.nt;                               // keys only rise: behind an unseen unit all are
         }
         if (ui >= u1) return;
-        const int key = (ui - gi.unit0) * KU + rb * p.box_rows;
         page = p.n_pages;                                        // out of the view: the box fills with zeros
-        if (lane < jobs && key < gi.klen) page = gi.pages[key / p.page_len];
+        if (lane < nb && (ui - gi.unit0) * KU + lane * p.box_rows < gi.klen) {
+            page = gi.pages[pidx];
+            if (page < 0 || page >= p.n_pages) {
+                page = p.n_pages;
+                if (p.err) atomicOr(p.err, Z2B_OPS_BAD_PAGE);
+            }
+        }
     };
     auto copy = [&] {
         if (ui >= u1) return;
-        const int st = issued % NS, key = (ui - gi.unit0) * KU + rb * p.box_rows;
-        if (page < 0 || page > p.n_pages || (page == p.n_pages && lane < jobs && key < gi.klen)) {
-            page = p.n_pages;
-            if (p.err) atomicOr(p.err, Z2B_OPS_BAD_PAGE);
-        }
+        const int st = issued % NS;
+        const uint32_t dst = smem_u32(ring) + st * STAGE;
         if (lane == 0) mbar_expect_tx(&full[st], STAGE);
-        __syncwarp();
-        if (lane < jobs)
-            tma_load_4d(box_dst + st * STAGE, isv ? &vmap : &kmap, half * 64, gi.h, key % p.page_len, page, &full[st]);
+        for (int i = 0; i < nb; ++i) {
+            const int pg = __shfl_sync(0xffffffffu, page, i), pr = __shfl_sync(0xffffffffu, prow, i);
+            if (lane == 0)
+                for (int half = 0; half < Tile<HD>::HALVES; half += p.box_halves) {
+                    const uint32_t d = dst + half * (KU * Tile<HD>::RB) + i * p.box_rows * Tile<HD>::RB;
+                    tma_load_page(d, &kmap, pr, half, gi.h, pg, &full[st]);
+                    tma_load_page(d + Tile<HD>::BYTES, &vmap, pr, half, gi.h, pg, &full[st]);
+                }
+        }
         ++issued;
         ++ui;
         look_up();
@@ -203,36 +230,82 @@ __global__ void __launch_bounds__(32 * max_warps(HD), 1) prefix_attn_kernel(cons
     look_up();
     for (int i = 0; i < NS; ++i) copy();
 
+    // ---- the queries of the next segment, on their way while this one is worked on
+    const bool q16 = ((reinterpret_cast<uintptr_t>(p.q) | (uintptr_t)(p.q_row * 2) | (uintptr_t)(p.q_head * 2)) & 15) == 0;
+    auto fetch_q = [&](const Seg& g) {
+        for (int i = lane; i < MT * (HD / 8); i += 32) {
+            const int row = i / (HD / 8), c = i % (HD / 8), rr = g.j * MT + row, t = div_g(p, rr);
+            const bool live = t < g.n;
+            const T* src = (const T*)p.q + (live ? (long long)(g.lo + t) * p.q_row + (long long)(g.h * p.G + rr - t * p.G) * p.q_head + c * 8 : 0);
+            uint8_t* dst = s_q + row * (HD * 2) + ((c ^ (row & (HD / 8 - 1) & 7)) << 4);
+            if (q16) cp_async16(dst, src, live);
+            else
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" :: "r"(smem_u32(dst) + 4 * e), "l"(src + (live ? 2 * e : 0)), "r"(live ? 4 : 0) : "memory");
+        }
+        cp_async_commit();
+    };
+    const bool flat = p.scale2 == 0.0f;                          // all scores equal: zero queries, so that masked keys stay apart
+    const float sc = flat ? 1.0f : fabsf(p.scale2);              // the maximum is taken before the scale: a negative one
+    const uint32_t q_and = flat ? 0u : 0xffffffffu, q_xor = p.scale2 < 0.0f ? 0x80008000u : 0u;     // negates the queries
+    // byte offsets of this lane's 16-byte chunks in a K and a V tile, for four steps of 32 bytes:
+    // K as rows (A of S^T), V transposed on the way (A of O^T)
+    constexpr int OFFS = HD >= 64 ? 4 : HD / 16;
+    uint32_t koff[OFFS], voff[OFFS];
+#pragma unroll
+    for (int k = 0; k < OFFS; ++k) {
+        koff[k] = Tile<HD>::chunk(lane & 15, 2 * k + (lane >> 4));
+        voff[k] = Tile<HD>::BYTES + Tile<HD>::chunk(((lane >> 4) << 3) + (lane & 7), 2 * k + ((lane >> 3) & 1));
+    }
+    const int key_l = lane >> 2, row_l = (lane & 3) * 2;         // this lane's key and first row in an accumulator tile
+
     int it = 0;
     bool dead = false;                                           // a wait ran out
-    while (u < u1 && !dead) {
-        const Seg g = find_seg<MT>(p, ln, u);
+    Seg g;
+    if (u < u1) {
+        g = find_seg<MT, KU>(p, ln, u);
+        u = max(u, g.unit0);
+        if (u < u1) fetch_q(g);
+    }
+    while (u < u1) {
         const int end = min(u1, g.unit0 + g.nt);
-        // this lane's rows: two of each block of 16
-        int lim[M16][2], lim_min = 0x7fffffff;
-        uint32_t qa[M16][KS][4];
+        cp_async_wait_0();
+        __syncwarp();
+        uint32_t qb[NB][KS][2];                                  // Q^T as B operand
 #pragma unroll
-        for (int mb = 0; mb < M16; ++mb)
+        for (int nb_ = 0; nb_ < NB; ++nb_)
+#pragma unroll
+            for (int k = 0; k < KS; k += 2) {
+                const int row = nb_ * 8 + (lane & 7), c = 2 * k + (lane >> 3);
+                uint32_t r[4];
+                ldsm4(smem_u32(s_q) + row * (HD * 2) + (((KS > 1 ? c : c & 1) ^ (row & (HD / 8 - 1) & 7)) << 4), r);
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (k + e / 2 < KS) qb[nb_][k + e / 2][e & 1] = (r[e] & q_and) ^ q_xor;
+            }
+        __syncwarp();
+        Seg gn;
+        if (end < u1) {
+            gn = find_seg<MT, KU>(p, ln, end);
+            if (gn.unit0 < u1) fetch_q(gn);
+        }
+        int lim[NB][2], lim_min = 0x7fffffff;                    // keys that this lane's rows see
+#pragma unroll
+        for (int nb_ = 0; nb_ < NB; ++nb_)
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
-                const int rr = g.j * MT + mb * 16 + (lane >> 2) + 8 * x, i = rr / p.G;
-                const bool live = i < g.n;
-                lim[mb][x] = !live ? 0 : u < ln.pf_units ? g.klen : min(g.klen, g.klen - g.n + i + 1);
-                lim_min = min(lim_min, lim[mb][x]);
-                const T* qp = (const T*)p.q + (long long)(g.lo + i) * p.q_row + (long long)(g.h * p.G + rr % p.G) * p.q_head + (lane & 3) * 2;
-#pragma unroll
-                for (int k = 0; k < KS; ++k) {
-                    qa[mb][k][x] = live ? *(const uint32_t*)(qp + k * 16) : 0u;
-                    qa[mb][k][x + 2] = live ? *(const uint32_t*)(qp + k * 16 + 8) : 0u;
-                }
+                const int i = div_g(p, g.j * MT + nb_ * 8 + row_l + x);
+                lim[nb_][x] = i >= g.n ? 0 : g.prefix ? g.klen : min(g.klen, g.klen - g.n + i + 1);
+                if (i < g.n) lim_min = min(lim_min, lim[nb_][x]);        // rows that do not exist are never stored
             }
-        float o[M16][DT][4], m[M16][2], l[M16][2];
+        float o[NB][DT][4], m[NB][2], l[NB][2];
 #pragma unroll
-        for (int mb = 0; mb < M16; ++mb) {
-            m[mb][0] = m[mb][1] = -INFINITY;
-            l[mb][0] = l[mb][1] = 0.0f;
+        for (int nb_ = 0; nb_ < NB; ++nb_) {
+            m[nb_][0] = m[nb_][1] = -INFINITY;
+            l[nb_][0] = l[nb_][1] = 0.0f;
 #pragma unroll
-            for (int d = 0; d < DT; ++d) o[mb][d][0] = o[mb][d][1] = o[mb][d][2] = o[mb][d][3] = 0.0f;
+            for (int d = 0; d < DT; ++d) o[nb_][d][0] = o[nb_][d][1] = o[nb_][d][2] = o[nb_][d][3] = 0.0f;
         }
 
         for (; u < end; ++u) {
@@ -243,7 +316,7 @@ __global__ void __launch_bounds__(32 * max_warps(HD), 1) prefix_attn_kernel(cons
             if (dead) break;
             ++it;
             uint8_t* kt = ring + (size_t)st * STAGE;
-            const uint32_t ks = smem_u32(kt), vs = ks + Tile<HD>::BYTES;
+            const uint32_t ks = smem_u32(kt);
             const bool tail = key0 + KU > g.klen;
             if (tail) {
                 // rows behind the last key may hold anything: zero times that is not zero
@@ -252,76 +325,101 @@ __global__ void __launch_bounds__(32 * max_warps(HD), 1) prefix_attn_kernel(cons
                         *(uint4*)(kt + Tile<HD>::BYTES + Tile<HD>::chunk(i / (HD / 8), i % (HD / 8))) = make_uint4(0, 0, 0, 0);
                 __syncwarp();
             }
-            float s[M16][NT][4];
+            float s[NB][KM][4];
 #pragma unroll
-            for (int mb = 0; mb < M16; ++mb)
+            for (int nb_ = 0; nb_ < NB; ++nb_)
 #pragma unroll
-                for (int n = 0; n < NT; ++n) s[mb][n][0] = s[mb][n][1] = s[mb][n][2] = s[mb][n][3] = 0.0f;
+                for (int n = 0; n < KM; ++n) s[nb_][n][0] = s[nb_][n][1] = s[nb_][n][2] = s[nb_][n][3] = 0.0f;
 #pragma unroll
             for (int k = 0; k < KS; ++k)
 #pragma unroll
-                for (int n = 0; n < NT; n += 2) {
+                for (int n = 0; n < KM; ++n) {
                     uint32_t r[4];
-                    ldsm4(ks + Tile<HD>::chunk(n * 8 + ((lane >> 4) << 3) + (lane & 7), 2 * k + ((lane >> 3) & 1)), r);
+                    ldsm4(ks + koff[k % OFFS] + (k / OFFS) * (KU * Tile<HD>::RB) + n * 16 * Tile<HD>::RB, r);
 #pragma unroll
-                    for (int mb = 0; mb < M16; ++mb) {
-                        mma_t<T>(s[mb][n], qa[mb][k], r[0], r[1]);
-                        mma_t<T>(s[mb][n + 1], qa[mb][k], r[2], r[3]);
-                    }
+                    for (int nb_ = 0; nb_ < NB; ++nb_) mma_t<T>(s[nb_][n], r, qb[nb_][k][0], qb[nb_][k][1]);
                 }
-            const bool cut = key0 + KU > lim_min;
+            if (__any_sync(0xffffffffu, key0 + KU > lim_min)) {  // some row does not see all of the unit
 #pragma unroll
-            for (int mb = 0; mb < M16; ++mb) {
-                float mx[2] = {m[mb][0], m[mb][1]}, f[2], base[2];
+                for (int nb_ = 0; nb_ < NB; ++nb_)
 #pragma unroll
-                for (int n = 0; n < NT; ++n)
+                    for (int n = 0; n < KM; ++n)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        s[mb][n][e] *= p.scale2;
-                        if (cut && key0 + n * 8 + (lane & 3) * 2 + (e & 1) >= lim[mb][e >> 1]) s[mb][n][e] = -INFINITY;
-                        mx[e >> 1] = fmaxf(mx[e >> 1], s[mb][n][e]);
-                    }
+                        for (int e = 0; e < 4; ++e)
+                            if (key0 + n * 16 + key_l + (e >> 1) * 8 >= lim[nb_][e & 1]) s[nb_][n][e] = -INFINITY;
+            }
+            float top[NB][2];
+            bool raise = false;
+#pragma unroll
+            for (int nb_ = 0; nb_ < NB; ++nb_)
 #pragma unroll
                 for (int x = 0; x < 2; ++x) {
-                    mx[x] = fmaxf(mx[x], __shfl_xor_sync(0xffffffffu, mx[x], 1));
-                    mx[x] = fmaxf(mx[x], __shfl_xor_sync(0xffffffffu, mx[x], 2));
-                    base[x] = mx[x] == -INFINITY ? 0.0f : mx[x];         // a row that has seen no key yet
-                    f[x] = ex2(m[mb][x] - base[x]);
-                    m[mb][x] = mx[x];
-                    l[mb][x] *= f[x];
+                    float mx = fmaxf(s[nb_][0][x], s[nb_][0][2 + x]);
+#pragma unroll
+                    for (int n = 1; n < KM; ++n) mx = fmaxf(mx, fmaxf(s[nb_][n][x], s[nb_][n][2 + x]));
+                    top[nb_][x] = mx;
                 }
+            // maxima over the lanes that share the rows
 #pragma unroll
-                for (int d = 0; d < DT; ++d) { o[mb][d][0] *= f[0]; o[mb][d][1] *= f[0]; o[mb][d][2] *= f[1]; o[mb][d][3] *= f[1]; }
+            for (int w = 4; w < 32; w <<= 1)
 #pragma unroll
-                for (int n = 0; n < NT; ++n)
+                for (int nb_ = 0; nb_ < NB; ++nb_)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        s[mb][n][e] = ex2(s[mb][n][e] - base[e >> 1]);
-                        l[mb][e >> 1] += s[mb][n][e];
+                    for (int x = 0; x < 2; ++x) top[nb_][x] = fmaxf(top[nb_][x], __shfl_xor_sync(0xffffffffu, top[nb_][x], w));
+#pragma unroll
+            for (int nb_ = 0; nb_ < NB; ++nb_)
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    top[nb_][x] *= sc;
+                    raise |= top[nb_][x] > m[nb_][x] + LAG;
+                }
+            // a maximum is raised only when it would lag by more than 2^8: sums and O are f32 and the
+            // probabilities stay below that, so nothing overflows, and rescaling becomes rare
+            if (__any_sync(0xffffffffu, raise)) {
+#pragma unroll
+                for (int nb_ = 0; nb_ < NB; ++nb_) {
+                    float f[2];
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        f[x] = 1.0f;
+                        if (top[nb_][x] > m[nb_][x] + LAG) {
+                            f[x] = ex2(m[nb_][x] - top[nb_][x]);
+                            m[nb_][x] = top[nb_][x];
+                        }
+                        l[nb_][x] *= f[x];
                     }
+#pragma unroll
+                    for (int d = 0; d < DT; ++d) { o[nb_][d][0] *= f[0]; o[nb_][d][1] *= f[1]; o[nb_][d][2] *= f[0]; o[nb_][d][3] *= f[1]; }
+                }
+            }
+            uint32_t pb[NB][KM][2];                              // P^T as B operand
+#pragma unroll
+            for (int nb_ = 0; nb_ < NB; ++nb_) {
+                // a row that has seen no key yet has a maximum of -infinity, and no probability
+                const float b0 = m[nb_][0] == -INFINITY ? 0.0f : -m[nb_][0], b1 = m[nb_][1] == -INFINITY ? 0.0f : -m[nb_][1];
+#pragma unroll
+                for (int n = 0; n < KM; ++n) {
+                    float* x = s[nb_][n];
+                    x[0] = ex2(fmaf(x[0], sc, b0));
+                    x[1] = ex2(fmaf(x[1], sc, b1));
+                    x[2] = ex2(fmaf(x[2], sc, b0));
+                    x[3] = ex2(fmaf(x[3], sc, b1));
+                    l[nb_][0] += x[0] + x[2];
+                    l[nb_][1] += x[1] + x[3];
+                    // rounded (to nearest) to the cache's type: the tensor core's operand
+                    pb[nb_][n][0] = movm(pack2<T>(x[0], x[1]));
+                    pb[nb_][n][1] = movm(pack2<T>(x[2], x[3]));
+                }
             }
 #pragma unroll
-            for (int k = 0; k < KU / 16; ++k) {
-                // the probabilities rounded (to nearest) to the cache's type: the tensor core's operand
-                uint32_t pa[M16][4];
+            for (int n = 0; n < KM; ++n)
 #pragma unroll
-                for (int mb = 0; mb < M16; ++mb) {
-                    pa[mb][0] = pack2<T>(s[mb][2 * k][0], s[mb][2 * k][1]);
-                    pa[mb][1] = pack2<T>(s[mb][2 * k][2], s[mb][2 * k][3]);
-                    pa[mb][2] = pack2<T>(s[mb][2 * k + 1][0], s[mb][2 * k + 1][1]);
-                    pa[mb][3] = pack2<T>(s[mb][2 * k + 1][2], s[mb][2 * k + 1][3]);
-                }
-#pragma unroll
-                for (int d = 0; d < DT; d += 2) {
+                for (int d = 0; d < DT; ++d) {
                     uint32_t r[4];
-                    ldsm4t(vs + Tile<HD>::chunk(k * 16 + (lane & 15), d + (lane >> 4)), r);
+                    ldsm4t(ks + voff[d % OFFS] + (d / OFFS) * (KU * Tile<HD>::RB) + n * 16 * Tile<HD>::RB, r);
 #pragma unroll
-                    for (int mb = 0; mb < M16; ++mb) {
-                        mma_t<T>(o[mb][d], pa[mb], r[0], r[1]);
-                        mma_t<T>(o[mb][d + 1], pa[mb], r[2], r[3]);
-                    }
+                    for (int nb_ = 0; nb_ < NB; ++nb_) mma_t<T>(o[nb_][d], r, pb[nb_][n][0], pb[nb_][n][1]);
                 }
-            }
             if (tail) fence_proxy_async();                       // this stage's zeros before the next copy into it
             __syncwarp();
             copy();
@@ -336,20 +434,25 @@ __global__ void __launch_bounds__(32 * max_warps(HD), 1) prefix_attn_kernel(cons
         float* po = p.part_o + (size_t)slot * MT * HD;
         float2* pm = p.part_ml + (size_t)slot * MT;
 #pragma unroll
-        for (int mb = 0; mb < M16; ++mb)
+        for (int nb_ = 0; nb_ < NB; ++nb_)
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
-                float sum = l[mb][x];
-                sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-                sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-                const int row = mb * 16 + (lane >> 2) + 8 * x;
+                float sum = l[nb_][x];
+#pragma unroll
+                for (int w = 4; w < 32; w <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
+                const int row = nb_ * 8 + row_l + x;
                 if (row >= rows) continue;
 #pragma unroll
-                for (int d = 0; d < DT; ++d)
-                    *(float2*)(po + (size_t)row * HD + d * 8 + (lane & 3) * 2) = make_float2(o[mb][d][2 * x], o[mb][d][2 * x + 1]);
-                if ((lane & 3) == 0) pm[row] = make_float2(m[mb][x], sum);
+                for (int d = 0; d < DT; ++d) {
+                    po[(size_t)row * HD + d * 16 + key_l] = o[nb_][d][x];
+                    po[(size_t)row * HD + d * 16 + 8 + key_l] = o[nb_][d][2 + x];
+                }
+                if (key_l == 0) pm[row] = make_float2(m[nb_][x], sum);
             }
+        if (end < u1) u = max(end, gn.unit0);
+        g = gn;
     }
+    cp_async_wait_0();
     // after a wait that ran out, the copies in flight still land in this CTA's memory
     if (dead)
         for (int k = it; k < issued; ++k) mbar_wait(&full[k % NS], (k / NS) & 1, nullptr, 1u << 16);
@@ -377,7 +480,7 @@ struct JoinP {
 // dims, four loads in flight. Bound: the chain of dependent loads (offsets, statistics, outputs).
 template <typename T, int HD, int MT>
 __global__ void __launch_bounds__(256) prefix_attn_join_kernel(const __grid_constant__ JoinP p) {
-    constexpr int DPL = HD >= 32 ? HD / 32 : 1;
+    constexpr int DPL = HD >= 32 ? HD / 32 : 1, KU = unit_keys(HD);
     const AttnP& a = p.a;
     const int lane = threadIdx.x & 31, nh = a.nkv * a.G;
     const int w = blockIdx.x * 8 + (threadIdx.x >> 5), t = w / nh, head = w % nh;
@@ -389,17 +492,18 @@ __global__ void __launch_bounds__(256) prefix_attn_join_kernel(const __grid_cons
     const int b = warp_find_seq(a.row_off, a.n_seq, t);
     if (t >= total || b < 0) return;                             // padding stays as it is
     const int unit_b = a.plan[b], seg_b = a.plan[a.n_seq + 1 + b];
-    const SeqInfo s = seq_info<MT>(a, b);
+    const SeqInfo s = seq_info<MT, KU>(a, b);
     const int i = t - s.lo;
     if (s.bad || i >= s.n) return;
 
     // the workers that hold this row's segment of the prefix, and of the stream's own rows
-    const int pf_units = a.pf_row_tiles * a.nkv * cdiv(a.prefix_len, KU);
+    const int pf_units = a.pf_row_tiles * a.nkv * (cdiv(a.prefix_len, KU) + SEG_COST);
     const long long W = (long long)pf_units + own_units;
     int n0 = 0, n1 = 0, slot0 = 0, slot1 = 0, row0 = 0, row1 = 0;
     if (a.prefix_len > 0) {
         const int nt = cdiv(a.prefix_len, p.pf.keys), r = t * a.G + g, seg = h * p.pf.row_tiles + r / p.pf.mt;
-        const long long Wp = p.pf_apart ? (long long)p.pf.row_tiles * a.nkv * nt : W, first = (long long)seg * nt;
+        const int cost = p.pf_apart ? TC_SEG_COST : SEG_COST, size = nt + cost;
+        const long long Wp = p.pf_apart ? (long long)p.pf.row_tiles * a.nkv * size : W, first = (long long)seg * size + cost;
         const int workers = line_workers(Wp, p.pf.workers), c0 = unit_owner(first, Wp, workers);
         n0 = unit_owner(first + nt - 1, Wp, workers) - c0 + 1;
         slot0 = seg + c0;
@@ -408,7 +512,7 @@ __global__ void __launch_bounds__(256) prefix_attn_join_kernel(const __grid_cons
     }
     if (s.nt > 0) {
         const int r = i * a.G + g, js = h * s.qt + r / MT;
-        const long long first = (long long)pf_units + unit_b + (long long)js * s.nt;
+        const long long first = (long long)pf_units + unit_b + (long long)js * (s.nt + SEG_COST) + SEG_COST;
         const int workers = line_workers(W, p.own.workers), c0 = unit_owner(first, W, workers);
         n1 = unit_owner(first + s.nt - 1, W, workers) - c0 + 1;
         slot1 = a.pf_row_tiles * a.nkv + seg_b + js + c0;
@@ -478,11 +582,16 @@ __global__ void __launch_bounds__(256) prefix_attn_join_kernel(const __grid_cons
 
 // ---- host -----------------------------------------------------------------------------------
 struct HostPlan {
-    int G, m16, warps;                  // blocks of 16 rows in an own segment, warps of a CTA
+    int G, nb, warps;                   // blocks of 8 rows in an own segment, warps of a CTA
     PartSet own, pf;                    // pointers unset
     bool pf_tc;                         // the prefix has a launch of its own, on tcgen05
     size_t off_own_ml, off_own_o, off_pf_ml, off_pf_o, bytes;
 };
+
+// Rings, queries and the line's streams (20 bytes each; OPS_MAX_SEQ of them leave room for four warps).
+size_t attn_smem(int hd, int nb, int warps, int n_seq) {
+    return 1024 + (size_t)warps * (ring_stages(hd) * 2 * unit_keys(hd) * hd * 2 + 8 * nb * hd * 2) + (size_t)(n_seq + 1) * 20;
+}
 
 size_t up(size_t x) { return (x + 255) & ~(size_t)255; }
 
@@ -490,15 +599,17 @@ HostPlan host_plan(const z2b_prefix_attn_args& a) {
     HostPlan h{};
     const int nkv = a.kv->n_head_kv, hd = a.kv->head_dim;
     h.G = a.n_head / nkv;
-    // rows of one stream and key head, on average; head_dim 128 keeps 16 (32 rows do not fit the
-    // registers), a second row tile then finds its keys in L2
-    h.m16 = hd > 64 || (long long)((a.n_rows + a.n_seq - 1) / a.n_seq) * h.G <= 16 ? 1 : 2;
-    h.warps = a.n_seq > 1024 ? 4 : max_warps(hd);                // room for the line's streams beside the rings
+    // rows of one stream and key head, on average: the smallest tile that holds them. head_dim 128
+    // keeps 16 (32 rows do not fit the registers); a second row tile then finds its keys in L2
+    const long long rows = (long long)((a.n_rows + a.n_seq - 1) / a.n_seq) * h.G;
+    h.nb = rows <= 8 ? 1 : rows <= 16 || hd > 64 ? 2 : 4;
+    h.warps = max_warps(hd);                                     // fewer where the line's streams need the room
+    while (attn_smem(hd, h.nb, h.warps, a.n_seq) > MAX_SMEM) --h.warps;
     const long long R = (long long)a.n_rows * h.G;
-    const int mt = 16 * h.m16;
+    const int mt = 8 * h.nb;
     h.pf_tc = a.prefix_len > 0 && hd >= 64 && R > 64;
     const int pf_tiles = a.prefix_len > 0 && !h.pf_tc ? (int)((R + mt - 1) / mt) : 0;
-    h.own = PartSet{nullptr, nullptr, mt, KU, 148 * h.warps, 0, pf_tiles};
+    h.own = PartSet{nullptr, nullptr, mt, unit_keys(hd), 148 * h.warps, 0, pf_tiles};
     const long long segs = ((R + mt - 1) / mt + a.n_seq + pf_tiles) * nkv;
     h.own.max_slots = (int)(segs + h.own.workers);
     h.pf = h.own;
@@ -515,33 +626,19 @@ HostPlan host_plan(const z2b_prefix_attn_args& a) {
     return h;
 }
 
-bool make_map(CUtensorMap* m, const void* base, const z2b_paged_kv& c, int box_rows, int inner) {
-    auto enc = tensor_map_encoder();
-    if (!enc) return false;
-    const cuuint64_t dims[4] = {(cuuint64_t)c.head_dim, (cuuint64_t)c.n_head_kv, (cuuint64_t)c.page_len, (cuuint64_t)c.n_pages};
-    const cuuint64_t strides[3] = {(cuuint64_t)c.head_stride * 2, (cuuint64_t)c.row_stride * 2, (cuuint64_t)c.page_stride * 2};
-    const cuuint32_t box[4] = {(cuuint32_t)inner, 1, (cuuint32_t)box_rows, 1}, one[4] = {1, 1, 1, 1};
-    const CUtensorMapSwizzle sw = inner == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : inner == 32 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B;
-    return enc(m, c.type == Z2B_TYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
-               const_cast<void*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, sw,
-               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
-template <typename T, int HD, int M16>
+template <typename T, int HD, int NB>
 cudaError_t go_attn(const AttnP& p, const CUtensorMap& km, const CUtensorMap& vm, int warps, cudaStream_t s) {
-    constexpr int STAGE = 2 * Tile<HD>::BYTES;
-    constexpr int most = 224 * 1024;
-    const size_t smem = 1024 + (size_t)warps * ring_stages(HD) * STAGE + (size_t)(p.n_seq + 1) * 20;
     static std::atomic<uint64_t> opted{0};                       // devices whose shared-memory opt-in is done
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
     if (dev >= 64 || !(opted.load(std::memory_order_relaxed) >> dev & 1)) {
-        e = cudaFuncSetAttribute(prefix_attn_kernel<T, HD, M16>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+        e = cudaFuncSetAttribute(prefix_attn_kernel<T, HD, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, MAX_SMEM);
         if (e != cudaSuccess) return e;
         if (dev < 64) opted.fetch_or(1ull << dev, std::memory_order_relaxed);
     }
-    return launch_pdl(prefix_attn_kernel<T, HD, M16>, dim3(148), dim3(32 * warps), smem, s, p, km, vm);
+    return launch_pdl(prefix_attn_kernel<T, HD, NB>, dim3(148), dim3(32 * warps),
+                      attn_smem(HD, NB, warps, p.n_seq), s, p, km, vm);
 }
 
 template <typename T, int HD>
@@ -552,7 +649,7 @@ cudaError_t go_all(const z2b_prefix_attn_args& a, HostPlan h, cudaStream_t s) {
     p.row_off = a.row_off; p.seq_len = a.seq_len; p.table = a.page_table; p.prefix_pages = a.prefix_pages; p.err = a.err;
     p.n_rows = a.n_rows; p.n_seq = a.n_seq; p.nkv = c.n_head_kv; p.G = h.G; p.page_len = c.page_len; p.n_pages = c.n_pages;
     p.max_pages = a.max_pages; p.prefix_len = a.prefix_len;
-    const int page_pow2 = c.page_len & -c.page_len;
+    p.g_mul = (uint32_t)((0x100000000ull + h.G - 1) / h.G);
     p.scale2 = a.scale * 1.4426950408889634f;
     uint8_t* ws = (uint8_t*)a.workspace;
     p.plan = (int*)ws;
@@ -561,31 +658,34 @@ cudaError_t go_all(const z2b_prefix_attn_args& a, HostPlan h, cudaStream_t s) {
     if constexpr (HD >= 64) {
         if (h.pf_tc) {
             AttnP f = p;
-            f.box_rows = page_pow2 > TC_KEYS ? TC_KEYS : page_pow2;
+            cut_boxes(f, TC_KEYS, HD);
             f.pf_row_tiles = h.pf.row_tiles;
             f.max_slots = h.pf.max_slots;
             h.pf.ml = f.part_ml = (float2*)(ws + h.off_pf_ml);
             h.pf.o = f.part_o = (float*)(ws + h.off_pf_o);
-            if (!make_map(&km, c.k, c, f.box_rows, 64) || !make_map(&vm, c.v, c, f.box_rows, 64)) return cudaErrorNotSupported;
+            if (!make_page_map(&km, c.k, c, f) || !make_page_map(&vm, c.v, c, f)) return cudaErrorNotSupported;
             if ((e = launch_prefix_tc<T, HD>(f, km, vm, h.pf.workers, s)) != cudaSuccess) return e;
         }
     }
-    p.box_rows = page_pow2 > KU ? KU : page_pow2;
-    if (!make_map(&km, c.k, c, p.box_rows, Tile<HD>::INNER) || !make_map(&vm, c.v, c, p.box_rows, Tile<HD>::INNER))
+    cut_boxes(p, unit_keys(HD), HD);
+    if (!make_page_map(&km, c.k, c, p) || !make_page_map(&vm, c.v, c, p))
         return cudaErrorNotSupported;
     p.pf_row_tiles = h.own.row_tiles;
     p.after_prefix = h.pf_tc;
     p.max_slots = h.own.max_slots;
     h.own.ml = p.part_ml = (float2*)(ws + h.off_own_ml);
     h.own.o = p.part_o = (float*)(ws + h.off_own_o);
-    if constexpr (HD > 64) e = go_attn<T, HD, 1>(p, km, vm, h.warps, s);
-    else e = h.m16 == 1 ? go_attn<T, HD, 1>(p, km, vm, h.warps, s) : go_attn<T, HD, 2>(p, km, vm, h.warps, s);
+    e = h.nb == 1 ? go_attn<T, HD, 1>(p, km, vm, h.warps, s) : cudaSuccess;
+    if (h.nb == 2) e = go_attn<T, HD, 2>(p, km, vm, h.warps, s);
+    if constexpr (HD <= 64)
+        if (h.nb == 4) e = go_attn<T, HD, 4>(p, km, vm, h.warps, s);
     if (e != cudaSuccess) return e;
     const JoinP j{p, h.pf_tc ? h.pf : h.own, h.own, h.pf_tc, a.out, a.lse, a.o_row, a.o_head};
     const dim3 grid((unsigned)(((long long)a.n_rows * a.n_head + 7) / 8));
     if constexpr (HD <= 64)
-        if (h.m16 == 2) return launch_pdl(prefix_attn_join_kernel<T, HD, 32>, grid, dim3(256), 0, s, j);
-    return launch_pdl(prefix_attn_join_kernel<T, HD, 16>, grid, dim3(256), 0, s, j);
+        if (h.nb == 4) return launch_pdl(prefix_attn_join_kernel<T, HD, 32>, grid, dim3(256), 0, s, j);
+    return h.nb == 1 ? launch_pdl(prefix_attn_join_kernel<T, HD, 8>, grid, dim3(256), 0, s, j)
+                     : launch_pdl(prefix_attn_join_kernel<T, HD, 16>, grid, dim3(256), 0, s, j);
 }
 
 template <typename T> cudaError_t go_type(const z2b_prefix_attn_args& a, const HostPlan& h, cudaStream_t s) {

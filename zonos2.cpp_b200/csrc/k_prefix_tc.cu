@@ -25,10 +25,9 @@ namespace z2b {
 namespace {
 
 // Three warpgroups: two of softmax, one of TMA (warp 8) and MMA (warp 9). Launched at 168
-// registers a thread (384 x 168 = 64512); the third keeps 72 so that the softmax
-// rows fit 216: 256 x 216 + 128 x 72 = 64512.
+// registers a thread (384 x 168 = 64512); the third keeps 80 so that the softmax
+// rows fit 208: 256 x 208 + 128 x 80 = 63488.
 constexpr int TC_THREADS = 384;
-constexpr float LAG = 8.0f;            // log2 by which a row's maximum may run ahead of the one in use
 
 __device__ __forceinline__ uint32_t idesc_t(bool bf16, int n, bool b_mn) {
     return (1u << 4) | (bf16 ? (1u << 7) | (1u << 10) : 0u) | (b_mn ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) |
@@ -116,8 +115,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) prefix_tc_kernel(const __grid_c
     pdl_release();
 
     const int live_rows = max(0, min(p.n_rows, p.row_off[p.n_seq])) * p.G;
-    const int nt = cdiv(p.prefix_len, TC_KEYS);
-    const long long W = (long long)p.pf_row_tiles * p.nkv * nt;
+    const int nt = cdiv(p.prefix_len, TC_KEYS), size = nt + TC_SEG_COST;   // line positions of a segment
+    const long long W = (long long)p.pf_row_tiles * p.nkv * size;
     const int ctas = line_workers(W, gridDim.x);
     int u0 = 0, u1 = 0;
     if ((int)blockIdx.x < ctas) {
@@ -126,43 +125,42 @@ __global__ void __launch_bounds__(TC_THREADS, 1) prefix_tc_kernel(const __grid_c
     }
 
     if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
     if (warp == 8) {
-        // ---- TMA producer: the boxes of a tile spread over the lanes
-        const int nb = TC_KEYS / p.box_rows, jobs = nb * HALVES;
+        // ---- TMA producer: lane i looks up run i's page, one lane issues the boxes
+        const int nb = TC_KEYS / p.box_rows;                     // at most 16
         int it = 0;
         bool ok = true;
         for (int u = u0; u < u1 && ok;) {
-            const int seg = u / nt, end = min(u1, (seg + 1) * nt), h = seg / p.pf_row_tiles;
+            const int seg = u / size, end = min(u1, (seg + 1) * size), unit0 = seg * size + TC_SEG_COST, h = seg / p.pf_row_tiles;
             if (live_tiles(seg % p.pf_row_tiles, live_rows) == 0) { u = end; continue; }
-            for (; u < end && ok; ++u) {
-                const int key0 = (u - seg * nt) * TC_KEYS;
+            for (u = max(u, unit0); u < end && ok; ++u) {
+                const int key = (u - unit0) * TC_KEYS + lane * p.box_rows, row = key % p.page_len;
+                int page = p.n_pages;                            // out of the view: zeros
+                if (lane < nb && key < p.prefix_len) {
+                    page = p.prefix_pages[key / p.page_len];
+                    if (page < 0 || page >= p.n_pages) {
+                        page = p.n_pages;
+                        if (p.err) atomicOr(p.err, Z2B_OPS_BAD_PAGE);
+                    }
+                }
 #pragma unroll 1
                 for (int isv = 0; isv < 2 && ok; ++isv) {
                     const int st = it % stages, use = it / stages;
-                    for (int base = 0; base < jobs; base += 32) {
-                        const int i = base + lane, rb = i % nb, half = i / nb, key = key0 + rb * p.box_rows;
-                        int page = p.n_pages;                    // out of the view: zeros
-                        if (i < jobs && key < p.prefix_len) {
-                            page = p.prefix_pages[key / p.page_len];
-                            if (page < 0 || page >= p.n_pages) {
-                                page = p.n_pages;
-                                if (p.err) atomicOr(p.err, Z2B_OPS_BAD_PAGE);
-                            }
-                        }
-                        if (base == 0) {
-                            if (lane == 0) {
-                                ok = use == 0 || wait_ab(&kv_empty[st], (use - 1) & 1, p.err, &s_abort);
-                                if (ok) mbar_expect_tx(&kv_full[st], TILE);
-                            }
-                            ok = __shfl_sync(0xffffffffu, ok, 0);
-                            if (!ok) break;
-                        }
-                        if (i < jobs)
-                            tma_load_4d(smem_u32(ring) + st * TILE + half * 16384 + rb * p.box_rows * 128, isv ? &vmap : &kmap,
-                                        half * 64, h, key % p.page_len, page, &kv_full[st]);
+                    if (lane == 0) {
+                        ok = use == 0 || wait_ab(&kv_empty[st], (use - 1) & 1, p.err, &s_abort);
+                        if (ok) mbar_expect_tx(&kv_full[st], TILE);
                     }
-                    if (ok) ++it;
+                    ok = __shfl_sync(0xffffffffu, ok, 0);
+                    if (!ok) break;
+                    for (int i = 0; i < nb; ++i) {
+                        const int pg = __shfl_sync(0xffffffffu, page, i), pr = __shfl_sync(0xffffffffu, row, i);
+                        if (lane == 0)
+                            for (int half = 0; half < HALVES; half += p.box_halves)
+                                tma_load_page(smem_u32(ring) + st * TILE + half * 16384 + i * p.box_rows * 128, isv ? &vmap : &kmap, pr,
+                                              half, h, pg, &kv_full[st]);
+                    }
+                    ++it;
                 }
             }
         }
@@ -191,10 +189,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1) prefix_tc_kernel(const __grid_c
                 umma_commit(&s_full[t]);
             };
             for (int u = u0; u < u1 && ok;) {
-                const int seg = u / nt, end = min(u1, (seg + 1) * nt), n = end - u;
+                const int seg = u / size, end = min(u1, (seg + 1) * size), n = end - max(u, seg * size + TC_SEG_COST);
                 const int nl = live_tiles(seg % p.pf_row_tiles, live_rows);
                 u = end;
-                if (nl == 0) continue;
+                if (nl == 0 || n <= 0) continue;
                 wait(&kv_full[2 * c % stages], 2 * c / stages);
                 for (int t = 0; t < nl; ++t) {
                     wait(&q_full[t], segs[t]++);
@@ -237,7 +235,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) prefix_tc_kernel(const __grid_c
         __syncwarp();
     }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
         // ---- softmax: thread = row
         const int t = warp >> 2, row = threadIdx.x & 127;
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;       // 32 (warp % 4) lanes, in the address's upper half
@@ -250,9 +248,11 @@ __global__ void __launch_bounds__(TC_THREADS, 1) prefix_tc_kernel(const __grid_c
         int c = 0, ct = 0;
         bool ok = true;
         for (int u = u0; u < u1 && ok;) {
-            const int seg = u / nt, end = min(u1, (seg + 1) * nt), n = end - u, key_first = (u - seg * nt) * TC_KEYS;
+            const int seg = u / size, end = min(u1, (seg + 1) * size), unit0 = seg * size + TC_SEG_COST;
+            const int n = end - max(u, unit0), key_first = (max(u, unit0) - unit0) * TC_KEYS;
             const int j = seg % p.pf_row_tiles, h = seg / p.pf_row_tiles, nl = live_tiles(j, live_rows);
             u = end;
+            if (n <= 0) continue;
             if (t >= nl) { c += nl ? n : 0; continue; }
             // Q_t: this thread's row, swizzled by 16-byte chunks
             const int r = j * TC_ROWS + t * 128 + row;

@@ -11,9 +11,13 @@
 
 namespace z2b {
 
-constexpr int KU = 32;                 // keys of a unit on the warp-level kernel
 constexpr int TC_ROWS = 256, TC_KEYS = 128;    // rows of a segment and keys of a unit on tcgen05
-constexpr int MIN_UNITS = 2;           // units per worker at least, before more workers are used
+constexpr int MIN_UNITS = 2;           // line positions per worker at least, before more workers are used
+// Line positions that a segment takes ahead of its units: what a worker spends on a segment
+// besides its units (queries, the partial result), so that ranges of short segments are not
+// the longest ones.
+constexpr int SEG_COST = 1, TC_SEG_COST = 2;
+constexpr float LAG = 8.0f;            // log2 by which a row's maximum may run ahead of the one in use
 
 struct AttnP {
     const void* q;
@@ -21,7 +25,9 @@ struct AttnP {
     const int *row_off, *seq_len, *table, *prefix_pages;
     uint32_t* err;
     int n_rows, n_seq, nkv, G, page_len, n_pages, max_pages, prefix_len;
-    int box_rows;                      // rows of one TMA box: a power of two that divides page_len, at most a unit's keys
+    uint32_t g_mul;                    // ceil(2^32 / G), for quotients by G of numbers x with x G < 2^32
+    int box_rows, box_halves;          // rows of one TMA box (a power of two that divides page_len, at most a
+                                       // unit's keys), and how many 64-dim halves it holds
     float scale2;                      // scale * log2(e)
     int pf_row_tiles;                  // row tiles of the prefix in this launch (0: none)
     int max_slots;
@@ -31,11 +37,12 @@ struct AttnP {
     int* plan;                         // [2][n_seq + 1] unit and segment offsets of the streams, written for the join
 };
 
+__device__ __forceinline__ int div_g(const AttnP& p, int x) { return p.G == 1 ? x : (int)__umulhi((uint32_t)x, p.g_mul); }
 __device__ __forceinline__ int cdiv(int a, int b) { return (a + b - 1) / b; }
 
 // One stream's extent, with offsets and lengths that are out of range cut to nothing.
 struct SeqInfo { int lo, n, len, nt, qt; bool bad; };
-template <int MT> __device__ __forceinline__ SeqInfo seq_info(const AttnP& p, int b) {
+template <int MT, int KU> __device__ __forceinline__ SeqInfo seq_info(const AttnP& p, int b) {
     SeqInfo s;
     const int lo = p.row_off[b], hi = p.row_off[b + 1], len = p.seq_len[b];
     const long long cap = (long long)p.max_pages * p.page_len;
@@ -48,7 +55,7 @@ template <int MT> __device__ __forceinline__ SeqInfo seq_info(const AttnP& p, in
     return s;
 }
 
-// Which of `workers` holds unit u of a line of W: the i with W i / workers <= u < W (i + 1) / workers.
+// Which of `workers` holds position u of a line of W: the i with W i / workers <= u < W (i + 1) / workers.
 __device__ __forceinline__ int unit_owner(long long u, long long W, int workers) {
     return (int)(((u + 1) * workers - 1) / W);
 }
@@ -56,6 +63,7 @@ __device__ __forceinline__ int line_workers(long long W, int most) {
     return (int)max(1ll, min((long long)most, W / MIN_UNITS));
 }
 
+// D[16][8] += A[16][16] B[16][8], f32 sums.
 template <typename T> __device__ __forceinline__ void mma_t(float* d, const uint32_t* a, uint32_t b0, uint32_t b1);
 template <> __device__ __forceinline__ void mma_t<__half>(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
     mma16816(d, a[0], a[1], a[2], a[3], b0, b1);
@@ -85,15 +93,46 @@ __device__ __forceinline__ void ldsm4t(uint32_t a, uint32_t (&r)[4]) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
 }
+// Transpose of an 8 x 8 tile of 16-bit values held two to a lane.
+__device__ __forceinline__ uint32_t movm(uint32_t a) {
+    uint32_t d;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+    return d;
+}
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, int w, uint64_t* bar) {
+// One box of a page: rows [row, row + box_rows) of key head h, dims from 64 half on. The view is
+// [page][head][half][row][up to 64 dims], so one box can bring both halves of a tile's rows.
+__device__ __forceinline__ void tma_load_page(uint32_t dst, const CUtensorMap* map, int row, int half, int h, int page, uint64_t* bar) {
     asm volatile(
-        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
-        :: "r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar)) : "memory");
+        "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];"
+        :: "r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(row), "r"(half), "r"(h), "r"(page), "r"(smem_u32(bar))
+        : "memory");
+}
+
+// How a tile of `keys` rows is cut into boxes: runs of rows that stay within a page, both halves
+// of head_dim 128 in one box when a run is the whole tile.
+inline void cut_boxes(AttnP& p, int keys, int hd) {
+    const int pow2 = p.page_len & -p.page_len;
+    p.box_rows = pow2 > keys ? keys : pow2;
+    p.box_halves = hd > 64 && p.box_rows == keys ? 2 : 1;
+}
+
+inline bool make_page_map(CUtensorMap* m, const void* base, const z2b_paged_kv& c, const AttnP& p) {
+    auto enc = tensor_map_encoder();
+    if (!enc) return false;
+    const int inner = c.head_dim < 64 ? c.head_dim : 64;
+    const cuuint64_t dims[5] = {(cuuint64_t)inner, (cuuint64_t)c.page_len, (cuuint64_t)(c.head_dim / inner), (cuuint64_t)c.n_head_kv,
+                                (cuuint64_t)c.n_pages};
+    const cuuint64_t strides[4] = {(cuuint64_t)c.row_stride * 2, 128, (cuuint64_t)c.head_stride * 2, (cuuint64_t)c.page_stride * 2};
+    const cuuint32_t box[5] = {(cuuint32_t)inner, (cuuint32_t)p.box_rows, (cuuint32_t)p.box_halves, 1, 1}, one[5] = {1, 1, 1, 1, 1};
+    const CUtensorMapSwizzle sw = inner == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : inner == 32 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B;
+    return enc(m, c.type == Z2B_TYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5,
+               const_cast<void*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, sw,
+               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 // The prefix on tcgen05 (k_prefix_tc.cu): segments of TC_ROWS rows, units of TC_KEYS keys.
