@@ -127,7 +127,10 @@ __global__ void __launch_bounds__(32 * max_warps(HD), 1) prefix_attn_kernel(cons
         for (int i = 0; i < NS; ++i) mbar_init(&full[i], 1);
         fence_mbar_init();
     }
-    if (!p.after_prefix) { pdl_wait(); pdl_release(); }
+    if (threadIdx.x == 0) { prefetch_map(&kmap); prefetch_map(&vmap); }
+    if (!p.after_prefix) pdl_wait();
+    pdl_release();                                               // the join reads its streams' extents meanwhile
+    const int last_off = p.row_off[p.n_seq];
 
     // ---- the line: offsets of every stream's units and segments, by a block scan
     {
@@ -165,17 +168,17 @@ __global__ void __launch_bounds__(32 * max_warps(HD), 1) prefix_attn_kernel(cons
     Line ln;
     ln.rec = s_rec;
     ln.len = s_len;
-    ln.total_rows = max(0, min(p.n_rows, p.row_off[p.n_seq]));
+    ln.total_rows = max(0, min(p.n_rows, last_off));
     ln.pf_nt = cdiv(p.prefix_len, KU);
     ln.pf_units = p.pf_row_tiles * p.nkv * (ln.pf_nt + SEG_COST);
     __syncthreads();
-    const long long W = (long long)ln.pf_units + s_rec[p.n_seq].x;
-    const int workers = line_workers(W, gridDim.x * nw);
+    const int W = ln.pf_units + s_rec[p.n_seq].x;
+    const Cut cut(W, gridDim.x * nw);
     const int me = warp * gridDim.x + blockIdx.x;                // few workers: one per SM first
     int u = 0, u1 = 0;
-    if (me < workers) {
-        u = (int)(W * me / workers);
-        u1 = (int)(W * (me + 1) / workers);
+    if (me < cut.workers) {
+        u = cut.begin(me);
+        u1 = cut.begin(me + 1);
     }
 
     // ---- the copies, NS units ahead of the products: a box of K and one of V per run of rows
@@ -185,6 +188,7 @@ __global__ void __launch_bounds__(32 * max_warps(HD), 1) prefix_attn_kernel(cons
     gi.unit0 = -1;
     gi.nt = 0;
     int ui = u, issued = 0, page = 0, pidx = 0, prow = 0;        // this lane's box: page id, its index, row in it
+    bool wanted = false;
     auto look_up = [&] {               // move ui to the next unit that some row sees; this lane's page of it
         prow += KU;
         while (prow >= p.page_len) { prow -= p.page_len; ++pidx; }
@@ -201,18 +205,20 @@ __global__ void __launch_bounds__(32 * max_warps(HD), 1) prefix_attn_kernel(cons
         }
         if (ui >= u1) return;
         page = p.n_pages;                                        // out of the view: the box fills with zeros
+        wanted = false;
         if (lane < nb && (ui - gi.unit0) * KU + lane * p.box_rows < gi.klen) {
-            page = gi.pages[pidx];
-            if (page < 0 || page >= p.n_pages) {
-                page = p.n_pages;
-                if (p.err) atomicOr(p.err, Z2B_OPS_BAD_PAGE);
-            }
+            page = gi.pages[pidx];                               // on its way until copy() checks it
+            wanted = true;
         }
     };
     auto copy = [&] {
         if (ui >= u1) return;
         const int st = issued % NS;
         const uint32_t dst = smem_u32(ring) + st * STAGE;
+        if (wanted && (page < 0 || page >= p.n_pages)) {
+            page = p.n_pages;
+            if (p.err) atomicOr(p.err, Z2B_OPS_BAD_PAGE);
+        }
         if (lane == 0) mbar_expect_tx(&full[st], STAGE);
         for (int i = 0; i < nb; ++i) {
             const int pg = __shfl_sync(0xffffffffu, page, i), pr = __shfl_sync(0xffffffffu, prow, i);
@@ -457,7 +463,7 @@ __global__ void __launch_bounds__(32 * max_warps(HD), 1) prefix_attn_kernel(cons
     if (dead)
         for (int k = it; k < issued; ++k) mbar_wait(&full[k % NS], (k / NS) & 1, nullptr, 1u << 16);
     // beside a prefix launch: the join that follows waits for this grid, so this grid ends after that one
-    if (p.after_prefix) { pdl_release(); pdl_wait(); }
+    if (p.after_prefix) pdl_wait();
 }
 
 // ---- join ---------------------------------------------------------------------------------
@@ -475,56 +481,81 @@ struct JoinP {
     long long o_row, o_head;
 };
 
-// One warp per (row, head). The partials of both sets are numbered through; lanes take the
+// W warps per (row, head): one, or where there are few rows, whose keys then lie with many
+// workers, a block of eight. The partials of both sets are numbered through; lanes take the
 // statistics of 32 at a time, then the weighted outputs are summed with each lane on its own
-// dims, four loads in flight. Bound: the chain of dependent loads (offsets, statistics, outputs).
-template <typename T, int HD, int MT>
-__global__ void __launch_bounds__(256) prefix_attn_join_kernel(const __grid_constant__ JoinP p) {
+// dims, four loads in flight. Bound: the chain of dependent loads; what depends on the call's
+// inputs alone is read before the wait for the launch ahead.
+template <typename T, int HD, int MT, int W>
+__global__ void __launch_bounds__(256, 4) prefix_attn_join_kernel(const __grid_constant__ JoinP p) {
     constexpr int DPL = HD >= 32 ? HD / 32 : 1, KU = unit_keys(HD);
     const AttnP& a = p.a;
-    const int lane = threadIdx.x & 31, nh = a.nkv * a.G;
-    const int w = blockIdx.x * 8 + (threadIdx.x >> 5), t = w / nh, head = w % nh;
-    const int h = head / a.G, g = head % a.G;
-    pdl_wait();
-    pdl_release();
-    if (t >= a.n_rows) return;
-    const int total = a.row_off[a.n_seq], own_units = a.plan[a.n_seq];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nh = a.nkv * a.G;
+    const int item = W == 1 ? blockIdx.x * 8 + warp : blockIdx.x, t = item / nh, head = item - t * nh;
+    const int h = head / a.G, g = head - h * a.G;
+    if (t >= a.n_rows) { pdl_wait(); return; }
+    // the launches ahead release this one once their own predecessors are done: the call's inputs are there
+    const int total = a.row_off[a.n_seq];
     const int b = warp_find_seq(a.row_off, a.n_seq, t);
-    if (t >= total || b < 0) return;                             // padding stays as it is
-    const int unit_b = a.plan[b], seg_b = a.plan[a.n_seq + 1 + b];
     const SeqInfo s = seq_info<MT, KU>(a, b);
+    int own_units = 0, unit_b = 0, seg_b = 0;
+    const bool scan = a.n_seq <= 256;                            // the line's offsets: few streams are summed here, ahead of the wait
+    if (scan) {
+        for (int c = lane; c < a.n_seq; c += 32) {
+            const SeqInfo x = seq_info<MT, KU>(a, c);
+            const int segs = x.qt * a.nkv, units = x.nt ? segs * (x.nt + SEG_COST) : 0;
+            own_units += units;
+            if (c < b) { unit_b += units; seg_b += segs; }
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            own_units += __shfl_xor_sync(0xffffffffu, own_units, o);
+            unit_b += __shfl_xor_sync(0xffffffffu, unit_b, o);
+            seg_b += __shfl_xor_sync(0xffffffffu, seg_b, o);
+        }
+    } else {
+        pdl_wait();
+        own_units = a.plan[a.n_seq];
+        unit_b = a.plan[b];
+        seg_b = a.plan[a.n_seq + 1 + b];
+    }
     const int i = t - s.lo;
-    if (s.bad || i >= s.n) return;
+    const bool live = t < total && !s.bad && i >= 0 && i < s.n;  // else padding, which stays as it is
 
     // the workers that hold this row's segment of the prefix, and of the stream's own rows
     const int pf_units = a.pf_row_tiles * a.nkv * (cdiv(a.prefix_len, KU) + SEG_COST);
-    const long long W = (long long)pf_units + own_units;
+    const int positions = pf_units + own_units;
+    const Cut cut(positions, p.own.workers);
     int n0 = 0, n1 = 0, slot0 = 0, slot1 = 0, row0 = 0, row1 = 0;
-    if (a.prefix_len > 0) {
-        const int nt = cdiv(a.prefix_len, p.pf.keys), r = t * a.G + g, seg = h * p.pf.row_tiles + r / p.pf.mt;
-        const int cost = p.pf_apart ? TC_SEG_COST : SEG_COST, size = nt + cost;
-        const long long Wp = p.pf_apart ? (long long)p.pf.row_tiles * a.nkv * size : W, first = (long long)seg * size + cost;
-        const int workers = line_workers(Wp, p.pf.workers), c0 = unit_owner(first, Wp, workers);
-        n0 = unit_owner(first + nt - 1, Wp, workers) - c0 + 1;
+    if (live && a.prefix_len > 0) {
+        const int nt = cdiv(a.prefix_len, p.pf.keys), r = t * a.G + g, j = r / p.pf.mt, seg = h * p.pf.row_tiles + j;
+        const int cost = p.pf_apart ? TC_SEG_COST : SEG_COST, first = seg * (nt + cost) + cost;
+        const int Wp = p.pf_apart ? p.pf.row_tiles * a.nkv * (nt + cost) : positions;
+        const Cut cp(Wp, p.pf.workers);
+        const int c0 = cp.owner(first, Wp);
+        n0 = cp.owner(first + nt - 1, Wp) - c0 + 1;
         slot0 = seg + c0;
-        row0 = r % p.pf.mt;
+        row0 = r - j * p.pf.mt;
         if (slot0 + n0 > p.pf.max_slots) n0 = 0;
     }
-    if (s.nt > 0) {
+    if (live && s.nt > 0) {
         const int r = i * a.G + g, js = h * s.qt + r / MT;
-        const long long first = (long long)pf_units + unit_b + (long long)js * (s.nt + SEG_COST) + SEG_COST;
-        const int workers = line_workers(W, p.own.workers), c0 = unit_owner(first, W, workers);
-        n1 = unit_owner(first + s.nt - 1, W, workers) - c0 + 1;
+        const int first = pf_units + unit_b + js * (s.nt + SEG_COST) + SEG_COST;
+        const int c0 = cut.owner(first, positions);
+        n1 = cut.owner(first + s.nt - 1, positions) - c0 + 1;
         slot1 = a.pf_row_tiles * a.nkv + seg_b + js + c0;
         row1 = r % MT;
         if (slot1 + n1 > p.own.max_slots) n1 = 0;                // only for offsets that do not ascend
     }
     const int n = n0 + n1;
+    if (scan) pdl_wait();
+    pdl_release();
+    if (!live) return;
     float M = -INFINITY, L = 0.0f, acc[DPL];
 #pragma unroll
     for (int d = 0; d < DPL; ++d) acc[d] = 0.0f;
-    for (int base = 0; base < n; base += 32) {
-        const int k = base + lane;
+    for (int base = 0; base < n; base += 32 * W) {
+        const int k = base + lane * W + (W > 1 ? warp : 0);      // W > 1: warp w has the partials w, w + W, ...
         float2 ml = make_float2(-INFINITY, 0.0f);
         const float* src = p.own.o;
         if (k < n) {
@@ -533,22 +564,13 @@ __global__ void __launch_bounds__(256) prefix_attn_join_kernel(const __grid_cons
             ml = ps.ml[at];
             src = ps.o + at * HD;
         }
-        const float top = fmaxf(M, warp_max(ml.x));
-        if (top == -INFINITY) continue;
-        const float f = ex2(M - top), wt = ex2(ml.x - top);
-        M = top;
-        L = L * f + warp_sum(ml.y * wt);
-#pragma unroll
-        for (int d = 0; d < DPL; ++d) acc[d] *= f;
-        const int cnt = min(32, n - base);
+        const int cnt = min(32, cdiv(n - base - (W > 1 ? warp : 0), W));
+        float wt = 0.0f;
         for (int k0 = 0; k0 < cnt; k0 += 4) {
-            float v[4][DPL], wk[4];
+            float v[4][DPL];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const int from = min(k0 + e, cnt - 1);
-                const float* sp = (const float*)__shfl_sync(0xffffffffu, (unsigned long long)src, from);
-                wk[e] = __shfl_sync(0xffffffffu, wt, from);
-                if (k0 + e >= cnt) wk[e] = 0.0f;
+                const float* sp = (const float*)__shfl_sync(0xffffffffu, (unsigned long long)src, min(k0 + e, cnt - 1));
                 if (HD >= 32 || lane < HD) {
                     if constexpr (DPL == 4) {
                         const float4 x = *(const float4*)(sp + lane * 4);
@@ -561,10 +583,42 @@ __global__ void __launch_bounds__(256) prefix_attn_join_kernel(const __grid_cons
                     }
                 }
             }
+            if (k0 == 0) {                                       // the weights, with the first outputs on their way
+                const float top = fmaxf(M, warp_max(ml.x));
+                const float to = top == -INFINITY ? 0.0f : top;  // no partial has seen a key
+                const float f = ex2(M - to);
+                wt = ex2(ml.x - to);
+                M = top;
+                L = L * f + warp_sum(ml.y * wt);
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
+                for (int d = 0; d < DPL; ++d) acc[d] *= f;
+            }
 #pragma unroll
-                for (int d = 0; d < DPL; ++d) acc[d] += wk[e] * v[e][d];
+            for (int e = 0; e < 4; ++e) {
+                float wk = __shfl_sync(0xffffffffu, wt, min(k0 + e, cnt - 1));
+                if (k0 + e >= cnt) wk = 0.0f;
+#pragma unroll
+                for (int d = 0; d < DPL; ++d) acc[d] += wk * v[e][d];
+            }
+        }
+    }
+    if constexpr (W > 1) {                                       // the block's warps, in a fixed order
+        __shared__ float s_acc[W][HD + 2];
+        if (lane == 0) { s_acc[warp][HD] = M; s_acc[warp][HD + 1] = L; }
+        if (HD >= 32 || lane < HD)
+#pragma unroll
+            for (int d = 0; d < DPL; ++d) s_acc[warp][lane * DPL + d] = acc[d];
+        __syncthreads();
+        if (warp > 0) return;
+        for (int w = 1; w < W; ++w) {
+            const float top = fmaxf(M, s_acc[w][HD]);
+            if (top == -INFINITY) continue;
+            const float f = ex2(M - top), fw = ex2(s_acc[w][HD] - top);
+            M = top;
+            L = L * f + s_acc[w][HD + 1] * fw;
+            if (HD >= 32 || lane < HD)
+#pragma unroll
+                for (int d = 0; d < DPL; ++d) acc[d] = acc[d] * f + s_acc[w][lane * DPL + d] * fw;
         }
     }
     const float inv = L > 0.0f ? 1.0f / L : 0.0f;
@@ -641,6 +695,14 @@ cudaError_t go_attn(const AttnP& p, const CUtensorMap& km, const CUtensorMap& vm
                       attn_smem(HD, NB, warps, p.n_seq), s, p, km, vm);
 }
 
+template <typename T, int HD, int MT>
+cudaError_t go_join(const JoinP& j, const z2b_prefix_attn_args& a, cudaStream_t s) {
+    const long long items = (long long)a.n_rows * a.n_head;
+    // a block per row and head while those are fewer than two blocks an SM hold in warps
+    if (items <= 148 * 16) return launch_pdl(prefix_attn_join_kernel<T, HD, MT, 8>, dim3((unsigned)items), dim3(256), 0, s, j);
+    return launch_pdl(prefix_attn_join_kernel<T, HD, MT, 1>, dim3((unsigned)((items + 7) / 8)), dim3(256), 0, s, j);
+}
+
 template <typename T, int HD>
 cudaError_t go_all(const z2b_prefix_attn_args& a, HostPlan h, cudaStream_t s) {
     const z2b_paged_kv& c = *a.kv;
@@ -681,11 +743,9 @@ cudaError_t go_all(const z2b_prefix_attn_args& a, HostPlan h, cudaStream_t s) {
         if (h.nb == 4) e = go_attn<T, HD, 4>(p, km, vm, h.warps, s);
     if (e != cudaSuccess) return e;
     const JoinP j{p, h.pf_tc ? h.pf : h.own, h.own, h.pf_tc, a.out, a.lse, a.o_row, a.o_head};
-    const dim3 grid((unsigned)(((long long)a.n_rows * a.n_head + 7) / 8));
     if constexpr (HD <= 64)
-        if (h.nb == 4) return launch_pdl(prefix_attn_join_kernel<T, HD, 32>, grid, dim3(256), 0, s, j);
-    return h.nb == 1 ? launch_pdl(prefix_attn_join_kernel<T, HD, 8>, grid, dim3(256), 0, s, j)
-                     : launch_pdl(prefix_attn_join_kernel<T, HD, 16>, grid, dim3(256), 0, s, j);
+        if (h.nb == 4) return go_join<T, HD, 32>(j, a, s);
+    return h.nb == 1 ? go_join<T, HD, 8>(j, a, s) : go_join<T, HD, 16>(j, a, s);
 }
 
 template <typename T> cudaError_t go_type(const z2b_prefix_attn_args& a, const HostPlan& h, cudaStream_t s) {

@@ -106,6 +106,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) prefix_tc_kernel(const __grid_c
         mbar_init(&fin, 1);
         s_abort = 0;
         fence_mbar_init();
+        prefetch_map(&kmap);
+        prefetch_map(&vmap);
     }
     tc_fence_before();
     __syncthreads();
@@ -116,12 +118,12 @@ __global__ void __launch_bounds__(TC_THREADS, 1) prefix_tc_kernel(const __grid_c
 
     const int live_rows = max(0, min(p.n_rows, p.row_off[p.n_seq])) * p.G;
     const int nt = cdiv(p.prefix_len, TC_KEYS), size = nt + TC_SEG_COST;   // line positions of a segment
-    const long long W = (long long)p.pf_row_tiles * p.nkv * size;
-    const int ctas = line_workers(W, gridDim.x);
+    const int W = p.pf_row_tiles * p.nkv * size;
+    const Cut cut(W, gridDim.x);
     int u0 = 0, u1 = 0;
-    if ((int)blockIdx.x < ctas) {
-        u0 = (int)(W * blockIdx.x / ctas);
-        u1 = (int)(W * (blockIdx.x + 1) / ctas);
+    if ((int)blockIdx.x < cut.workers) {
+        u0 = cut.begin(blockIdx.x);
+        u1 = cut.begin(blockIdx.x + 1);
     }
 
     if (warp >= 8) {

@@ -70,13 +70,14 @@ __global__ void __launch_bounds__(32 * ROWS_PER_BLOCK) rope_append_ops_kernel(co
     const int lane = threadIdx.x & 31, t = blockIdx.x * ROWS_PER_BLOCK + (threadIdx.x >> 5);
     pdl_wait();
     pdl_release();
-    if (t >= p.n_rows || t >= p.row_off[p.n_seq]) return;       // padding stays as it is
+    if (t >= p.n_rows) return;
+    const int total = p.row_off[p.n_seq];
     const int b = warp_find_seq(p.row_off, p.n_seq, t);
-    if (b < 0) return;
     const int lo = p.row_off[b], n = p.row_off[b + 1] - lo;
     const int len = p.seq_len[b];
+    if (t >= total) return;                                      // padding stays as it is
     const long long r = (long long)len - n + (t - lo);          // cache row
-    if (t - lo >= n || r < 0 || r >= (long long)p.max_pages * p.page_len) {
+    if (t < lo || t - lo >= n || r < 0 || r >= (long long)p.max_pages * p.page_len) {
         if (lane == 0 && p.err) atomicOr(p.err, Z2B_OPS_BAD_INDEX);
         return;
     }

@@ -9,11 +9,11 @@ namespace z2b {
 
 // The stream that owns packed row t: the last b with row_off[b] <= t, by a 32-way search
 // (each round one coalesced-enough load per lane: one round to 32 streams, two to 1024,
-// three to OPS_MAX_SEQ). Called by a whole warp; -1 when row_off[0] > t.
+// three to OPS_MAX_SEQ). Called by a whole warp; rows ahead of row_off[0] come out as
+// stream 0's, so the caller compares t with the stream's first row.
 __device__ __forceinline__ int warp_find_seq(const int* __restrict__ row_off, int n_seq, int t) {
     const int lane = threadIdx.x & 31;
     int lo = 0, n = n_seq;
-    if (row_off[0] > t) return -1;
     while (n > 1) {
         const int step = (n + 31) >> 5;
         const int i = lane * step;

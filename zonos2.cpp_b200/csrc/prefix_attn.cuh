@@ -55,15 +55,26 @@ template <int MT, int KU> __device__ __forceinline__ SeqInfo seq_info(const Attn
     return s;
 }
 
-// Which of `workers` holds position u of a line of W: the i with W i / workers <= u < W (i + 1) / workers.
-__device__ __forceinline__ int unit_owner(long long u, long long W, int workers) {
-    return (int)(((u + 1) * workers - 1) / W);
-}
-__device__ __forceinline__ int line_workers(long long W, int most) {
-    return (int)max(1ll, min((long long)most, W / MIN_UNITS));
-}
+// A line of W positions cut into equal ranges: worker i's begins at floor(W i / workers). W is
+// below 2^31 and i * workers below 2^31, so 32-bit arithmetic is exact: W i / workers =
+// i (W / workers) + i (W % workers) / workers.
+struct Cut {
+    int workers, each, rest;
+    __device__ __forceinline__ Cut(int W, int most) {
+        workers = max(1, min(most, W / MIN_UNITS));
+        each = W / workers;
+        rest = W - each * workers;
+    }
+    __device__ __forceinline__ int begin(int i) const { return i * each + (int)((unsigned)(i * rest) / (unsigned)workers); }
+    // The worker that holds position u: an f32 guess, off by one at most, put right exactly.
+    __device__ __forceinline__ int owner(int u, int W) const {
+        int i = min(workers - 1, (int)((float)u * (float)workers / (float)W));
+        while (begin(i) > u) --i;
+        while (begin(i + 1) <= u) ++i;
+        return i;
+    }
+};
 
-// D[16][8] += A[16][16] B[16][8], f32 sums.
 template <typename T> __device__ __forceinline__ void mma_t(float* d, const uint32_t* a, uint32_t b0, uint32_t b1);
 template <> __device__ __forceinline__ void mma_t<__half>(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
     mma16816(d, a[0], a[1], a[2], a[3], b0, b1);
@@ -98,6 +109,9 @@ __device__ __forceinline__ uint32_t movm(uint32_t a) {
     uint32_t d;
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
     return d;
+}
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* m) {
+    asm volatile("prefetch.tensormap [%0];" :: "l"(reinterpret_cast<uint64_t>(m)) : "memory");
 }
 __device__ __forceinline__ float ex2(float x) {
     float y;
