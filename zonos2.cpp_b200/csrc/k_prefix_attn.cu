@@ -220,15 +220,17 @@ __global__ void __launch_bounds__(32 * max_warps(HD), 1) prefix_attn_kernel(cons
             if (p.err) atomicOr(p.err, Z2B_OPS_BAD_PAGE);
         }
         if (lane == 0) mbar_expect_tx(&full[st], STAGE);
+        __syncwarp();
         for (int i = 0; i < nb; ++i) {
             const int pg = __shfl_sync(0xffffffffu, page, i), pr = __shfl_sync(0xffffffffu, prow, i);
-            if (lane == 0)
+            if (elect_one())
                 for (int half = 0; half < Tile<HD>::HALVES; half += p.box_halves) {
                     const uint32_t d = dst + half * (KU * Tile<HD>::RB) + i * p.box_rows * Tile<HD>::RB;
                     tma_load_page(d, &kmap, pr, half, gi.h, pg, &full[st]);
                     tma_load_page(d + Tile<HD>::BYTES, &vmap, pr, half, gi.h, pg, &full[st]);
                 }
         }
+        __syncwarp();
         ++issued;
         ++ui;
         look_up();

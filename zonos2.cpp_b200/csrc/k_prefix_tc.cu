@@ -149,19 +149,18 @@ __global__ void __launch_bounds__(TC_THREADS, 1) prefix_tc_kernel(const __grid_c
 #pragma unroll 1
                 for (int isv = 0; isv < 2 && ok; ++isv) {
                     const int st = it % stages, use = it / stages;
-                    if (lane == 0) {
-                        ok = use == 0 || wait_ab(&kv_empty[st], (use - 1) & 1, p.err, &s_abort);
-                        if (ok) mbar_expect_tx(&kv_full[st], TILE);
-                    }
-                    ok = __shfl_sync(0xffffffffu, ok, 0);
+                    ok = __all_sync(0xffffffffu, use == 0 || wait_ab(&kv_empty[st], (use - 1) & 1, p.err, &s_abort));
                     if (!ok) break;
+                    if (lane == 0) mbar_expect_tx(&kv_full[st], TILE);
+                    __syncwarp();
                     for (int i = 0; i < nb; ++i) {
                         const int pg = __shfl_sync(0xffffffffu, page, i), pr = __shfl_sync(0xffffffffu, row, i);
-                        if (lane == 0)
+                        if (elect_one())
                             for (int half = 0; half < HALVES; half += p.box_halves)
                                 tma_load_page(smem_u32(ring) + st * TILE + half * 16384 + i * p.box_rows * 128, isv ? &vmap : &kmap, pr,
                                               half, h, pg, &kv_full[st]);
                     }
+                    __syncwarp();
                     ++it;
                 }
             }
@@ -171,70 +170,72 @@ __global__ void __launch_bounds__(TC_THREADS, 1) prefix_tc_kernel(const __grid_c
             for (int k = max(0, it - stages); k < it; ++k) mbar_wait(&kv_full[k % stages], (k / stages) & 1, nullptr, 1u << 16);
         __syncwarp();
     } else if (warp == 9) {
-        // ---- MMA issuer
-        if (lane == 0) {
-            const uint32_t id_s = idesc_t(BF, TC_KEYS, false), id_o = idesc_t(BF, HD, true);
-            const uint32_t qs = smem_u32(smem), rs = smem_u32(ring);
-            int c = 0;                                           // units done
-            int segs[2] = {0, 0}, ct[2] = {0, 0};                // segments and units done of each row tile
-            bool ok = true;
-            auto wait = [&](uint64_t* bar, int phase) {
-                if (ok) ok = wait_ab(bar, phase & 1, p.err, &s_abort);
-                return ok;
-            };
-            auto scores = [&](int t, int idx) {                  // S_t = Q_t K^T
-                const uint32_t a = qs + t * TILE, b = rs + (idx % stages) * TILE;
+        // ---- MMA issuer: the warp walks together, one thread issues
+        const uint32_t id_s = idesc_t(BF, TC_KEYS, false), id_o = idesc_t(BF, HD, true);
+        const uint64_t qd = umma_desc_sw128(smem_u32(smem)), kd = umma_desc_sw128(smem_u32(ring)), vd = desc_v(smem_u32(ring));
+        int c = 0;                                               // units done
+        int segs[2] = {0, 0}, ct[2] = {0, 0};                    // segments and units done of each row tile
+        bool ok = true;
+        auto wait = [&](uint64_t* bar, int phase) {
+            if (ok) ok = __all_sync(0xffffffffu, wait_ab(bar, phase & 1, p.err, &s_abort));
+            return ok;
+        };
+        auto scores = [&](int t, int idx, bool last) {           // S_t = Q_t K^T; `last`: K's stage is free after it
+            const uint64_t a = qd + (uint64_t)(t * (TILE >> 4)), b = kd + (uint64_t)((idx % stages) * (TILE >> 4));
+            if (elect_one()) {
 #pragma unroll
-                for (int k = 0; k < HD / 16; ++k)
-                    umma_f16(tm + S_COL + t * 128, umma_desc_sw128(a + (k >> 2) * 16384 + (k & 3) * 32),
-                             umma_desc_sw128(b + (k >> 2) * 16384 + (k & 3) * 32), id_s, k > 0);
+                for (int k = 0; k < HD / 16; ++k)                // 32 bytes a step, 16 KB a half
+                    umma_f16(tm + S_COL + t * 128, a + ((k >> 2) * 1024 + (k & 3) * 2), b + ((k >> 2) * 1024 + (k & 3) * 2), id_s, k > 0);
                 umma_commit(&s_full[t]);
-            };
-            for (int u = u0; u < u1 && ok;) {
-                const int seg = u / size, end = min(u1, (seg + 1) * size), n = end - max(u, seg * size + TC_SEG_COST);
-                const int nl = live_tiles(seg % p.pf_row_tiles, live_rows);
-                u = end;
-                if (nl == 0 || n <= 0) continue;
-                wait(&kv_full[2 * c % stages], 2 * c / stages);
-                for (int t = 0; t < nl; ++t) {
-                    wait(&q_full[t], segs[t]++);
+                if (last) umma_commit(&kv_empty[idx % stages]);
+            }
+            __syncwarp();
+        };
+        for (int u = u0; u < u1 && ok;) {
+            const int seg = u / size, end = min(u1, (seg + 1) * size), n = end - max(u, seg * size + TC_SEG_COST);
+            const int nl = live_tiles(seg % p.pf_row_tiles, live_rows);
+            u = end;
+            if (nl == 0 || n <= 0) continue;
+            wait(&kv_full[2 * c % stages], 2 * c / stages);
+            for (int t = 0; t < nl; ++t) {
+                wait(&q_full[t], segs[t]++);
+                if (!ok) break;
+                tc_fence_after();
+                scores(t, 2 * c, t == nl - 1);
+            }
+            if (!ok) break;
+            for (int j = 0; j < n && ok; ++j, ++c) {
+                const int vi = 2 * c + 1, ki = 2 * c + 2;
+                for (int t = 0; t < nl && ok; ++t) {
+                    wait(&p_full[t], ct[t]);
+                    if (t == 0) wait(&kv_full[vi % stages], vi / stages);
                     if (!ok) break;
                     tc_fence_after();
-                    scores(t, 2 * c);
-                }
-                if (!ok) break;
-                umma_commit(&kv_empty[2 * c % stages]);
-                for (int j = 0; j < n && ok; ++j, ++c) {
-                    const int vi = 2 * c + 1, ki = 2 * c + 2;
-                    for (int t = 0; t < nl && ok; ++t) {
-                        wait(&p_full[t], ct[t]);
-                        if (t == 0) wait(&kv_full[vi % stages], vi / stages);
-                        if (!ok) break;
-                        tc_fence_after();
-                        const uint32_t b = rs + (vi % stages) * TILE;
+                    const uint64_t b = vd + (uint64_t)((vi % stages) * (TILE >> 4));
+                    if (elect_one()) {
 #pragma unroll
-                        for (int k = 0; k < TC_KEYS / 16; ++k)   // O_t += P_t V
-                            umma_ts(tm + O_COL + t * HD, tm + S_COL + t * 128 + k * 8, desc_v(b + k * 2048), id_o, j > 0 || k > 0);
+                        for (int k = 0; k < TC_KEYS / 16; ++k)   // O_t += P_t V, 2 KB a step of 16 keys
+                            umma_ts(tm + O_COL + t * HD, tm + S_COL + t * 128 + k * 8, b + k * 128, id_o, j > 0 || k > 0);
                         umma_commit(&pv_done[t]);
                         if (t == nl - 1) umma_commit(&kv_empty[vi % stages]);
-                        if (j + 1 < n) {
-                            // the next scores overwrite P_t: they wait for the product that reads it
-                            if (t == 0) wait(&kv_full[ki % stages], ki / stages);
-                            wait(&pv_done[t], ct[t]);
-                            if (!ok) break;
-                            tc_fence_after();
-                            scores(t, ki);
-                            if (t == nl - 1) umma_commit(&kv_empty[ki % stages]);
-                        }
-                        ++ct[t];
                     }
+                    __syncwarp();
+                    if (j + 1 < n) {
+                        // the next scores overwrite P_t: they wait for the product that reads it
+                        if (t == 0) wait(&kv_full[ki % stages], ki / stages);
+                        wait(&pv_done[t], ct[t]);
+                        if (!ok) break;
+                        tc_fence_after();
+                        scores(t, ki, t == nl - 1);
+                    }
+                    ++ct[t];
                 }
             }
-            // every product issued completes before the block gives its memory back
-            umma_commit(&fin);
-            (void)mbar_wait(&fin, 0, nullptr, 1u << 16);
         }
+        // every product issued completes before the block gives its memory back
+        if (elect_one()) umma_commit(&fin);
         __syncwarp();
+        (void)mbar_wait(&fin, 0, nullptr, 1u << 16);
     }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");

@@ -110,6 +110,15 @@ __device__ __forceinline__ uint32_t movm(uint32_t a) {
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
     return d;
 }
+// True in one thread of a whole converged warp, the same one at every call. Under this
+// predicate the compiler issues a copy or a product once; under a plain lane test it must
+// allow for several lanes and loops over them, moving every operand again (measured: some
+// 120 cycles a product).
+__device__ __forceinline__ bool elect_one() {
+    uint32_t one;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(one));
+    return one != 0;
+}
 __device__ __forceinline__ void prefetch_map(const CUtensorMap* m) {
     asm volatile("prefetch.tensormap [%0];" :: "l"(reinterpret_cast<uint64_t>(m)) : "memory");
 }
