@@ -530,7 +530,7 @@ __global__ void __launch_bounds__(256, 4) prefix_attn_join_kernel(const __grid_c
     const Cut cut(positions, p.own.workers);
     int n0 = 0, n1 = 0, slot0 = 0, slot1 = 0, row0 = 0, row1 = 0;
     if (live && a.prefix_len > 0) {
-        const int nt = cdiv(a.prefix_len, p.pf.keys), r = t * a.G + g, j = r / p.pf.mt, seg = h * p.pf.row_tiles + j;
+        const int nt = cdiv(a.prefix_len, p.pf.keys), r = t * a.G + g, j = r / p.pf.mt, seg = p.pf_apart ? j * a.nkv + h : h * p.pf.row_tiles + j;
         const int cost = p.pf_apart ? TC_SEG_COST : SEG_COST, first = seg * (nt + cost) + cost;
         const int Wp = p.pf_apart ? p.pf.row_tiles * a.nkv * (nt + cost) : positions;
         const Cut cp(Wp, p.pf.workers);
@@ -674,7 +674,10 @@ HostPlan host_plan(const z2b_prefix_attn_args& a) {
     h.off_own_o = n; n += up((size_t)h.own.max_slots * mt * hd * 4);
     if (h.pf_tc) {
         const int tiles = (int)((R + TC_ROWS - 1) / TC_ROWS);
-        h.pf = PartSet{nullptr, nullptr, TC_ROWS, TC_KEYS, 148, tiles * nkv + 148, tiles};
+        // a multiple of the row tiles, where that leaves few SMs idle: the row tiles are cut alike then,
+        // so the CTAs that read the same keys do so at the same time and all but one find them in L2
+        const int ctas = tiles <= 148 && 148 % tiles * 20 <= 148 ? 148 - 148 % tiles : 148;
+        h.pf = PartSet{nullptr, nullptr, TC_ROWS, TC_KEYS, ctas, tiles * nkv + ctas, tiles};
         h.off_pf_ml = n; n += up((size_t)h.pf.max_slots * TC_ROWS * 8);
         h.off_pf_o = n; n += up((size_t)h.pf.max_slots * TC_ROWS * hd * 4);
     }

@@ -4,11 +4,12 @@
 // A segment is 256 rows (query heads of one key head, over the streams) of one key head, a
 // unit 128 keys. One CTA per SM walks its range of the line (prefix_attn.cuh):
 //   warp 8   TMA: K and V tiles of 128 keys through a ring, boxes by page, 128-byte swizzle;
-//   warp 9   one lane issues S_t = Q_t K^T (both operands in shared memory) and
-//            O_t += P_t V (P_t from TMEM, V as it lies in the cache: N-major);
+//   warp 9   one thread issues S_t = Q_t K^T (both operands in shared memory) and O_t += P_t V
+//            (P_t from TMEM, V as it lies in the cache: N-major);
 //   warps 0-3 and 4-7: softmax of row tile t = 0, 1. A thread holds one row: no shuffles. It
 //            reads S_t from TMEM, takes the running maximum, and writes P_t, rounded to the
-//            cache's type, over S_t.
+//            cache's type, over S_t. The first half of P_t is handed over while the second is
+//            taken.
 // TMEM (512 columns): S_0, S_1 of 128 each, O_0, O_1 of head_dim each. While one tile's
 // probabilities are taken the tensor core works on the other's products.
 //
@@ -16,8 +17,15 @@
 // stays below 2^8, so nothing overflows or loses bits, and the rescale (O through registers)
 // becomes rare. l sums the unrounded probabilities.
 //
-// Bound: per unit 2 x (2 x 128^2 x head_dim) MACs take 2048 cycles at head_dim 128, and the
-// 2 x 128^2 exponentials take the same at 16 per cycle and SM.
+// Bound: per unit the products of both tiles take 2048 cycles at head_dim 128, and the
+// 2 x 128^2 exponentials the same at 16 per cycle and SM; under the load the SMs run at about
+// 1.5 GHz. 1024 rows of each of 8 key heads over 32768 keys (137 GFLOP) take 125 us, 1.1
+// PFLOP/s, 67% of measured cuBLAS bf16. Tried on that case and slower: two blocks of 64 scores
+// a tile in place of one of 128, so that scores never wait for the product that frees them
+// (+14 us: 64 keys are fed at 3/4 rate, 6 KB of operands per 32 cycles from shared memory);
+// reading the scores twice to spare registers (+10 us); a quarter of the exponentials by a
+// polynomial on the multiply-add pipe (+8 us); issuing whichever tile's product is ready
+// instead of in turn (+20 us: the polling warp takes issue slots).
 #include "launch.cuh"
 #include "prefix_attn.cuh"
 
@@ -25,8 +33,8 @@ namespace z2b {
 namespace {
 
 // Three warpgroups: two of softmax, one of TMA (warp 8) and MMA (warp 9). Launched at 168
-// registers a thread (384 x 168 = 64512); the third keeps 80 so that the softmax
-// rows fit 208: 256 x 208 + 128 x 80 = 63488.
+// registers a thread (384 x 168 = 64512); the third keeps 80 so that the softmax rows' 128
+// scores fit 208: 256 x 208 + 128 x 80 = 63488.
 constexpr int TC_THREADS = 384;
 
 __device__ __forceinline__ uint32_t idesc_t(bool bf16, int n, bool b_mn) {
@@ -71,6 +79,29 @@ __device__ __forceinline__ void tmem_st16(uint32_t a, const uint32_t* r) {
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// Pairs of f32 for the two-wide multiply-adds.
+__device__ __forceinline__ uint64_t f2(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void un2(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
 // Row tiles (of 128) of segment row tile j that hold live rows.
 __device__ __forceinline__ int live_tiles(int j, int live_rows) {
     return max(0, min(2, cdiv(live_rows - j * TC_ROWS, 128)));
@@ -90,7 +121,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) prefix_tc_kernel(const __grid_c
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     uint8_t* ring = smem + 2 * TILE;
-    __shared__ __align__(8) uint64_t kv_full[stages], kv_empty[stages], q_full[2], s_full[2], p_full[2], pv_done[2], fin;
+    __shared__ __align__(8) uint64_t kv_full[stages], kv_empty[stages], q_full[2], s_full[2], p_full[2][2], pv_done[2], fin;
     __shared__ uint32_t tmem_base;
     __shared__ volatile int s_abort;
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
@@ -102,7 +133,13 @@ __global__ void __launch_bounds__(TC_THREADS, 1) prefix_tc_kernel(const __grid_c
     }
     if (threadIdx.x == 0) {
         for (int i = 0; i < stages; ++i) { mbar_init(&kv_full[i], 1); mbar_init(&kv_empty[i], 1); }
-        for (int t = 0; t < 2; ++t) { mbar_init(&q_full[t], 4); mbar_init(&s_full[t], 1); mbar_init(&p_full[t], 4); mbar_init(&pv_done[t], 1); }
+        for (int t = 0; t < 2; ++t) {
+            mbar_init(&q_full[t], 4);
+            mbar_init(&s_full[t], 1);
+            mbar_init(&p_full[t][0], 4);
+            mbar_init(&p_full[t][1], 4);
+            mbar_init(&pv_done[t], 1);
+        }
         mbar_init(&fin, 1);
         s_abort = 0;
         fence_mbar_init();
@@ -134,8 +171,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) prefix_tc_kernel(const __grid_c
         int it = 0;
         bool ok = true;
         for (int u = u0; u < u1 && ok;) {
-            const int seg = u / size, end = min(u1, (seg + 1) * size), unit0 = seg * size + TC_SEG_COST, h = seg / p.pf_row_tiles;
-            if (live_tiles(seg % p.pf_row_tiles, live_rows) == 0) { u = end; continue; }
+            const int seg = u / size, end = min(u1, (seg + 1) * size), unit0 = seg * size + TC_SEG_COST, h = seg % p.nkv;
+            if (live_tiles(seg / p.nkv, live_rows) == 0) { u = end; continue; }
             for (u = max(u, unit0); u < end && ok; ++u) {
                 const int key = (u - unit0) * TC_KEYS + lane * p.box_rows, row = key % p.page_len;
                 int page = p.n_pages;                            // out of the view: zeros
@@ -181,11 +218,11 @@ __global__ void __launch_bounds__(TC_THREADS, 1) prefix_tc_kernel(const __grid_c
             return ok;
         };
         auto scores = [&](int t, int idx, bool last) {           // S_t = Q_t K^T; `last`: K's stage is free after it
-            const uint64_t a = qd + (uint64_t)(t * (TILE >> 4)), b = kd + (uint64_t)((idx % stages) * (TILE >> 4));
+            const uint64_t da = qd + (uint64_t)(t * (TILE >> 4)), db = kd + (uint64_t)((idx % stages) * (TILE >> 4));
             if (elect_one()) {
 #pragma unroll
                 for (int k = 0; k < HD / 16; ++k)                // 32 bytes a step, 16 KB a half
-                    umma_f16(tm + S_COL + t * 128, a + ((k >> 2) * 1024 + (k & 3) * 2), b + ((k >> 2) * 1024 + (k & 3) * 2), id_s, k > 0);
+                    umma_f16(tm + S_COL + t * 128, da + ((k >> 2) * 1024 + (k & 3) * 2), db + ((k >> 2) * 1024 + (k & 3) * 2), id_s, k > 0);
                 umma_commit(&s_full[t]);
                 if (last) umma_commit(&kv_empty[idx % stages]);
             }
@@ -193,7 +230,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) prefix_tc_kernel(const __grid_c
         };
         for (int u = u0; u < u1 && ok;) {
             const int seg = u / size, end = min(u1, (seg + 1) * size), n = end - max(u, seg * size + TC_SEG_COST);
-            const int nl = live_tiles(seg % p.pf_row_tiles, live_rows);
+            const int nl = live_tiles(seg / p.nkv, live_rows);
             u = end;
             if (nl == 0 || n <= 0) continue;
             wait(&kv_full[2 * c % stages], 2 * c / stages);
@@ -203,23 +240,27 @@ __global__ void __launch_bounds__(TC_THREADS, 1) prefix_tc_kernel(const __grid_c
                 tc_fence_after();
                 scores(t, 2 * c, t == nl - 1);
             }
-            if (!ok) break;
             for (int j = 0; j < n && ok; ++j, ++c) {
                 const int vi = 2 * c + 1, ki = 2 * c + 2;
                 for (int t = 0; t < nl && ok; ++t) {
-                    wait(&p_full[t], ct[t]);
-                    if (t == 0) wait(&kv_full[vi % stages], vi / stages);
-                    if (!ok) break;
-                    tc_fence_after();
-                    const uint64_t b = vd + (uint64_t)((vi % stages) * (TILE >> 4));
-                    if (elect_one()) {
 #pragma unroll
-                        for (int k = 0; k < TC_KEYS / 16; ++k)   // O_t += P_t V, 2 KB a step of 16 keys
-                            umma_ts(tm + O_COL + t * HD, tm + S_COL + t * 128 + k * 8, b + k * 128, id_o, j > 0 || k > 0);
-                        umma_commit(&pv_done[t]);
-                        if (t == nl - 1) umma_commit(&kv_empty[vi % stages]);
+                    for (int half = 0; half < 2; ++half) {
+                        wait(&p_full[t][half], ct[t]);
+                        if (half == 0 && t == 0) wait(&kv_full[vi % stages], vi / stages);
+                        if (!ok) break;
+                        tc_fence_after();
+                        const uint64_t db = vd + (uint64_t)((vi % stages) * (TILE >> 4) + half * 512);
+                        if (elect_one()) {
+#pragma unroll
+                            for (int k = 0; k < 4; ++k)          // O_t += P_t V, 2 KB a step of 16 keys
+                                umma_ts(tm + O_COL + t * HD, tm + S_COL + t * 128 + half * 32 + k * 8, db + k * 128, id_o, j > 0 || half > 0 || k > 0);
+                            if (half == 1) {
+                                umma_commit(&pv_done[t]);
+                                if (t == nl - 1) umma_commit(&kv_empty[vi % stages]);
+                            }
+                        }
+                        __syncwarp();
                     }
-                    __syncwarp();
                     if (j + 1 < n) {
                         // the next scores overwrite P_t: they wait for the product that reads it
                         if (t == 0) wait(&kv_full[ki % stages], ki / stages);
@@ -253,7 +294,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) prefix_tc_kernel(const __grid_c
         for (int u = u0; u < u1 && ok;) {
             const int seg = u / size, end = min(u1, (seg + 1) * size), unit0 = seg * size + TC_SEG_COST;
             const int n = end - max(u, unit0), key_first = (max(u, unit0) - unit0) * TC_KEYS;
-            const int j = seg % p.pf_row_tiles, h = seg / p.pf_row_tiles, nl = live_tiles(j, live_rows);
+            const int j = seg / p.nkv, h = seg % p.nkv, nl = live_tiles(j, live_rows);
             u = end;
             if (n <= 0) continue;
             if (t >= nl) { c += nl ? n : 0; continue; }
@@ -283,33 +324,32 @@ __global__ void __launch_bounds__(TC_THREADS, 1) prefix_tc_kernel(const __grid_c
                 if (!ok) break;
                 ++ct;
                 tc_fence_after();
+                const int keys = p.prefix_len - key_first - i * TC_KEYS;
+                if (keys < TC_KEYS) {
+                    // V rows behind the last key may hold anything: zero times that is not zero. Each tile
+                    // clears them before its go-ahead, whichever comes first.
+                    const int vi = 2 * c + 1;
+                    ok = __all_sync(0xffffffffu, wait_ab(&kv_full[vi % stages], (vi / stages) & 1, p.err, &s_abort));
+                    if (!ok) break;
+                    if (row >= keys)
+#pragma unroll
+                        for (int k = 0; k < HD / 8; ++k)
+                            *(uint4*)(ring + (vi % stages) * TILE + (k >> 3) * 16384 + row * 128 + ((k & 7) << 4)) = make_uint4(0, 0, 0, 0);
+                    fence_proxy_async();
+                }
                 uint32_t s[TC_KEYS];
 #pragma unroll
                 for (int k = 0; k < TC_KEYS; k += 32) tmem_ld32(ts + k, s + k);
                 tmem_wait_ld();
-                const int keys = p.prefix_len - key_first - i * TC_KEYS;
                 if (keys < TC_KEYS) {
 #pragma unroll
                     for (int k = 0; k < TC_KEYS; ++k)
                         if (k >= keys) s[k] = 0xff800000u;       // -inf
-                    if (t == 0) {
-                        // V rows behind the last key may hold anything: zero times that is not zero.
-                        // Tile 0's go-ahead comes before every product with this V.
-                        const int vi = 2 * c + 1;
-                        ok = __all_sync(0xffffffffu, wait_ab(&kv_full[vi % stages], (vi / stages) & 1, p.err, &s_abort));
-                        if (!ok) break;
-                        if (row >= keys)
-#pragma unroll
-                            for (int k = 0; k < HD / 8; ++k)
-                                *(uint4*)(ring + (vi % stages) * TILE + (k >> 3) * 16384 + row * 128 + ((k & 7) << 4)) = make_uint4(0, 0, 0, 0);
-                        fence_proxy_async();
-                    }
                 }
-                float mx[4];
+                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                for (int k = 0; k < 4; ++k) mx[k] = __uint_as_float(s[k]);
-#pragma unroll
-                for (int k = 4; k < TC_KEYS; ++k) mx[k & 3] = fmaxf(mx[k & 3], __uint_as_float(s[k]));
+                for (int e = 0; e < TC_KEYS; e += 2)
+                    mx[(e >> 1) & 3] = max3(mx[(e >> 1) & 3], __uint_as_float(s[e]), __uint_as_float(s[e + 1]));
                 const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sc;
                 const bool raise = top > m + LAG;
                 if (__any_sync(0xffffffffu, raise)) {
@@ -328,25 +368,31 @@ __global__ void __launch_bounds__(TC_THREADS, 1) prefix_tc_kernel(const __grid_c
                         }
                     }
                 }
-                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                uint64_t sum[2] = {0, 0};
+                const uint64_t sc2 = f2(sc, sc), m2 = f2(-m, -m);
 #pragma unroll
-                for (int k = 0; k < TC_KEYS; k += 32) {
+                for (int k = 0; k < 4; ++k) {
                     uint32_t pk[16];
 #pragma unroll
                     for (int e = 0; e < 32; e += 2) {
-                        const float a = ex2(fmaf(__uint_as_float(s[k + e]), sc, -m));
-                        const float b = ex2(fmaf(__uint_as_float(s[k + e + 1]), sc, -m));
-                        sum[e & 2] += a;
-                        sum[(e & 2) + 1] += b;
-                        pk[e / 2] = pack2<T>(a, b);
+                        float x, y;
+                        un2(fma2(f2(__uint_as_float(s[k * 32 + e]), __uint_as_float(s[k * 32 + e + 1])), sc2, m2), x, y);
+                        x = ex2(x);
+                        y = ex2(y);
+                        sum[(e >> 1) & 1] = add2(sum[(e >> 1) & 1], f2(x, y));
+                        pk[e / 2] = pack2<T>(x, y);
                     }
-                    tmem_st16(ts + k / 2, pk);
+                    tmem_st16(ts + k * 16, pk);
+                    if (k & 1) {
+                        tmem_wait_st();
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&p_full[t][k >> 1]);
+                    }
                 }
-                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-                tmem_wait_st();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&p_full[t]);
+                float x, y;
+                un2(add2(sum[0], sum[1]), x, y);
+                l += x + y;
             }
             if (!ok) break;
             ok = __all_sync(0xffffffffu, wait_ab(&pv_done[t], (ct - 1) & 1, p.err, &s_abort));

@@ -16,7 +16,7 @@ constexpr int MIN_UNITS = 2;           // line positions per worker at least, be
 // Line positions that a segment takes ahead of its units: what a worker spends on a segment
 // besides its units (queries, the partial result), so that ranges of short segments are not
 // the longest ones.
-constexpr int SEG_COST = 1, TC_SEG_COST = 2;
+constexpr int SEG_COST = 1, TC_SEG_COST = 3;
 constexpr float LAG = 8.0f;            // log2 by which a row's maximum may run ahead of the one in use
 
 struct AttnP {
