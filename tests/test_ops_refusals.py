@@ -124,12 +124,17 @@ def test_null_arguments():
     for fn in ("z2b_rope_append", "z2b_prefix_attention", "z2b_verify_drafts"):
         assert getattr(L, fn)(None, None) == ARG
     assert L.z2b_prefix_attention_workspace(None) == 0
-    assert L.z2b_prefix_attention_workspace(ctypes.addressof(_attn(n_head=3))) == 0
+    a = _attn(n_head=3)
+    assert L.z2b_prefix_attention_workspace(ctypes.addressof(a)) == 0
 
 
 def test_workspace_grows_with_the_call():
     L = ops._lib()
-    size = lambda **kw: L.z2b_prefix_attention_workspace(ctypes.addressof(_attn(**kw)))  # noqa: E731
+
+    def size(**kw):
+        a = _attn(**kw)
+        return L.z2b_prefix_attention_workspace(ctypes.addressof(a))
+
     assert 0 < size() <= size(n_rows=64, n_seq=64) <= size(n_rows=4096, n_seq=64)
 
 
@@ -168,3 +173,11 @@ def test_rope_table_against_decimals(kw):
             # pow amplifies a base's rounding by the exponent (at most 1 here; ln(base) < 16 bounds the rest)
             assert abs(decimal.Decimal(int(t.step[i])) - want) <= want * decimal.Decimal(16 * 2.0 ** -53) + 1
     assert t.mag == pytest.approx(0.1 * math.log(16.0) + 1.0 if kw.get("scaling") == "by_parts" else 1.0, rel=2.0 ** -23)
+
+
+def test_packed_arguments_match_the_structures():
+    """The binding packs argument structures by format strings; they are the C layout byte for byte."""
+    for cls, pack in ((ops.RopeAppendArgs, ops._pack_append), (ops.PrefixAttnArgs, ops._pack_attn), (ops.VerifyArgs, ops._pack_verify)):
+        values = [0.5 if f is ctypes.c_float else 3 + 7 * i for i, (_, f) in enumerate(cls._fields_)]
+        packed = pack(*values)
+        assert bytes(cls(*values))[: len(packed)] == packed and ctypes.sizeof(cls) - len(packed) < 8

@@ -15,6 +15,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import struct
 
 import torch
 
@@ -64,6 +65,18 @@ class VerifyArgs(ctypes.Structure):
                [("err", _P)]
 
 
+def _packer(cls):
+    """struct packer of an argument structure: a quarter of the time its constructor takes, which
+    is a good part of a small call."""
+    code = {_I: "i", _L: "q", _P: "P", _F: "f", _Z: "N"}
+    return struct.Struct("@" + "".join(code[f] for _, f in cls._fields_)).pack
+
+
+_pack_append, _pack_attn, _pack_verify = _packer(RopeAppendArgs), _packer(PrefixAttnArgs), _packer(VerifyArgs)
+_F16, _BF16, _F32, _F64, _I32, _U8 = torch.float16, torch.bfloat16, torch.float32, torch.float64, torch.int32, torch.uint8
+_empty_like = torch.empty_like
+# the raw handle of torch's current stream without building a Stream object, where torch has it
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
 _fn = None
 
 
@@ -87,19 +100,11 @@ def _refuse(msg):
     raise Z2BError(1, msg)
 
 
-def _ints(t, shape, device, what):
-    """Address of an int32 array on the device, of that shape and without gaps."""
-    if t.dtype != torch.int32 or t.shape != shape or t.device != device or not t.is_contiguous():
-        _refuse(f"{what}: a contiguous int32 tensor {tuple(shape)} on {device} is wanted")
-    return t.data_ptr()
-
-
-def _err(err, device):
-    return None if err is None else _ints(err, (1,), device, "err")
-
-
-def _stream(device):
-    return torch.cuda.current_stream(device).cuda_stream
+def _ints(t, n, idx, what):
+    """Address of an int32 array of n on device idx, without gaps."""
+    if t.dtype is _I32 and t.get_device() == idx and t.is_contiguous() and t.dim() == 1 and t.numel() == n:
+        return t.data_ptr()
+    _refuse(f"{what}: a contiguous int32 tensor of {n} on device {idx} is wanted")
 
 
 def check(err):
@@ -121,7 +126,8 @@ class Rope:
         if layout not in _LAYOUT or scaling not in _SCALING:
             _refuse("rope: layout is 'interleaved' or 'half', scaling 'none', 'linear', 'ntk' or 'by_parts'")
         self.table = RopeTable()
-        rc = _lib().z2b_rope_init(ctypes.addressof(self.table), int(rot_dim), _LAYOUT[layout], float(base),
+        self._at = ctypes.addressof(self.table)
+        rc = _lib().z2b_rope_init(self._at, int(rot_dim), _LAYOUT[layout], float(base),
                                   _SCALING[scaling], float(factor), int(orig_ctx))
         if rc:
             _raise(rc)
@@ -141,20 +147,28 @@ class PagedKV:
         self.k, self.v, self.device, self.dtype = k, v, k.device, k.dtype
         self.n_pages, self.page_len, self.n_head_kv, self.head_dim = k.shape
         self.view = PagedKVView(k.data_ptr(), v.data_ptr(), _TYPE[k.dtype], *k.shape, *k.stride()[:3])
+        self._idx, self._at, self._scale = k.get_device(), ctypes.addressof(self.view), 1.0 / math.sqrt(self.head_dim)
+        self._bytes = {}                # workspace bytes by sizes
 
 
-def _rows(t, heads, kv, what, dtype=None):
-    if t.dim() != 3 or t.shape[2] != kv.head_dim or (heads is not None and t.shape[1] != heads):
-        _refuse(f"{what}: [rows][{heads or 'heads'}][{kv.head_dim}] is wanted")
-    if t.device != kv.device or t.stride(2) != 1 or (dtype is not None and t.dtype != dtype):
+def _rows(t, n, heads, kv, dtype, what):
+    """Strides and address of rows [n][heads][head_dim] on the cache's device."""
+    s, r = t.shape, t.stride()
+    if len(s) != 3 or s[0] != n or s[1] != heads or s[2] != kv.head_dim:
+        _refuse(f"{what}: [{n}][{heads}][{kv.head_dim}] is wanted")
+    if r[2] != 1 or t.dtype is not dtype or t.get_device() != kv._idx:
         _refuse(f"{what}: wrong device or type, or the dims of a head are not contiguous")
+    return r[0], r[1], t.data_ptr()
 
 
-def _table(page_table, n_seq, kv):
-    if page_table.dim() != 2 or page_table.shape[0] != n_seq or page_table.dtype != torch.int32 or \
-            page_table.device != kv.device or (page_table.shape[1] > 1 and page_table.stride(1) != 1):
-        _refuse("page_table: an int32 tensor [streams][pages] on the cache's device is wanted")
-    return page_table.data_ptr(), page_table.stride(0), page_table.shape[1]
+def _table(t, n_seq, idx):
+    s = t.shape
+    if t.dtype is not _I32 or t.get_device() != idx or len(s) != 2 or s[0] != n_seq:
+        _refuse(f"page_table: an int32 tensor [{n_seq}][pages] on device {idx} is wanted")
+    r = t.stride()
+    if r[1] != 1 and s[1] > 1:
+        _refuse("page_table: the pages of a stream must be contiguous")
+    return t.data_ptr(), r[0], s[1]
 
 
 def rope_append(rope: Rope | None, kv: PagedKV, q, k, v, row_off, seq_len, page_table, prefix_len: int = 0, pos=None,
@@ -166,39 +180,32 @@ def rope_append(rope: Rope | None, kv: PagedKV, q, k, v, row_off, seq_len, page_
     lead = q if q is not None else k
     if lead is None or (k is None) != (v is None):
         _refuse("rope_append: q, or k and v, or all three")
-    dev, n, dt = kv.device, lead.shape[0], lead.dtype
-    if dt not in _TYPE:
+    if lead.dim() != 3:
+        _refuse("rope_append: rows [rows][heads][head_dim] are wanted")
+    idx, dt, n, nh = kv._idx, lead.dtype, lead.shape[0], 0
+    code = _TYPE.get(dt)
+    if code is None:
         _refuse("rope_append: f32, f16 or bf16 rows are wanted")
-    n_seq = seq_len.shape[0]
-    qs = os_ = ks = vs = (0, 0)
-    nh = 0
+    n_seq = seq_len.numel()
+    qr = qh = qp = outr = outh = outp = kr = kh = kp = vr = vh = vp = 0
     if q is not None:
-        _rows(q, None, kv, "q")
         nh = q.shape[1]
+        qr, qh, qp = _rows(q, n, nh, kv, dt, "q")
         if out is None:
-            out = torch.empty(q.shape, dtype=dt, device=dev)
-        else:
-            _rows(out, nh, kv, "out", dt)
-            if out.shape[0] != n:
-                _refuse("out: as many rows as q are wanted")
-        qs, os_ = q.stride(), out.stride()
+            out = _empty_like(q)
+        outr, outh, outp = _rows(out, n, nh, kv, dt, "out")
     elif out is not None:
         _refuse("rope_append: out without q")
     if k is not None:
-        _rows(k, kv.n_head_kv, kv, "k", dt)
-        _rows(v, kv.n_head_kv, kv, "v", dt)
-        if k.shape[0] != n or v.shape[0] != n:
-            _refuse("rope_append: q, k and v must have the same rows")
-        ks, vs = k.stride(), v.stride()
-    tab, tstride, pages = _table(page_table, n_seq, kv)
-    a = RopeAppendArgs(
-        dev.index, _TYPE[dt], n, n_seq, nh, prefix_len, ctypes.addressof(rope.table) if rope is not None else None,
-        ctypes.addressof(kv.view), q.data_ptr() if nh else None, out.data_ptr() if nh else None,
-        k.data_ptr() if k is not None else None, v.data_ptr() if v is not None else None,
-        qs[0], qs[1], os_[0], os_[1], ks[0], ks[1], vs[0], vs[1],
-        _ints(row_off, (n_seq + 1,), dev, "row_off"), _ints(seq_len, (n_seq,), dev, "seq_len"), tab, tstride, pages,
-        None if pos is None else _ints(pos, (n,), dev, "pos"), _err(err, dev))
-    rc = _lib().z2b_rope_append(ctypes.addressof(a), _stream(dev))
+        kr, kh, kp = _rows(k, n, kv.n_head_kv, kv, dt, "k")
+        vr, vh, vp = _rows(v, n, kv.n_head_kv, kv, dt, "v")
+    tab, tstride, pages = _table(page_table, n_seq, idx)
+    rc = _lib().z2b_rope_append(
+        _pack_append(idx, code, n, n_seq, nh, prefix_len, rope._at if rope is not None else 0, kv._at, qp, outp, kp, vp,
+                     qr, qh, outr, outh, kr, kh, vr, vh, _ints(row_off, n_seq + 1, idx, "row_off"),
+                     _ints(seq_len, n_seq, idx, "seq_len"), tab, tstride, pages,
+                     0 if pos is None else _ints(pos, n, idx, "pos"), 0 if err is None else _ints(err, 1, idx, "err")),
+        _raw_stream(idx))
     if rc:
         _raise(rc)
     return out
@@ -210,38 +217,41 @@ def prefix_attention(kv: PagedKV, q, row_off, seq_len, page_table, prefix_pages=
     stream's own rows up to its own (z2b_prefix_attention). q [rows][heads][head_dim] of the cache's
     type; scale defaults to 1 / sqrt(head_dim). Returns out, or (out, lse) when lse is True or an f32
     tensor [rows][heads]. Padding rows of new results are not written."""
-    dev, n_seq = kv.device, seq_len.shape[0]
-    _rows(q, None, kv, "q", kv.dtype)
+    if q.dim() != 3:
+        _refuse("q: rows [rows][heads][head_dim] are wanted")
+    idx, n_seq = kv._idx, seq_len.numel()
     n, nh, _ = q.shape
+    qr, qh, qp = _rows(q, n, nh, kv, kv.dtype, "q")
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    else:
-        _rows(out, nh, kv, "out", q.dtype)
-        if out.shape[0] != n:
-            _refuse("out: as many rows as q are wanted")
+        out = _empty_like(q)
+    outr, outh, outp = _rows(out, n, nh, kv, kv.dtype, "out")
     if lse is True:
-        lse = torch.empty((n, nh), dtype=torch.float32, device=dev)
+        lse = q.new_empty((n, nh), dtype=_F32)
     elif lse is False:
         lse = None
-    if lse is not None and (lse.dtype != torch.float32 or lse.shape != (n, nh) or lse.device != dev or not lse.is_contiguous()):
+    elif lse is not None and (lse.dtype is not _F32 or lse.shape != (n, nh) or lse.get_device() != idx or not lse.is_contiguous()):
         _refuse("lse: a contiguous f32 tensor [rows][heads] on the cache's device is wanted")
-    need = -(-prefix_len // kv.page_len)
-    if prefix_len > 0 and (prefix_pages is None or prefix_pages.dim() != 1 or prefix_pages.shape[0] < need):
-        _refuse("prefix_pages: a page for every page_len rows of the prefix is wanted")
-    tab, tstride, pages = _table(page_table, n_seq, kv)
-    qs, os_ = q.stride(), out.stride()
-    a = PrefixAttnArgs(
-        dev.index, n, n_seq, nh, prefix_len, 1.0 / math.sqrt(kv.head_dim) if scale is None else scale,
-        ctypes.addressof(kv.view), q.data_ptr(), out.data_ptr(), None if lse is None else lse.data_ptr(), qs[0], qs[1],
-        os_[0], os_[1], _ints(row_off, (n_seq + 1,), dev, "row_off"), _ints(seq_len, (n_seq,), dev, "seq_len"), tab,
-        tstride, pages, _ints(prefix_pages, prefix_pages.shape, dev, "prefix_pages") if prefix_len > 0 else None,
-        None, 0, _err(err, dev))
-    L, at = _lib(), ctypes.addressof(a)
-    a.workspace_bytes = L.z2b_prefix_attention_workspace(at)
-    if a.workspace_bytes:
-        ws = torch.empty(a.workspace_bytes, dtype=torch.uint8, device=dev)
-        a.workspace = ws.data_ptr()
-    rc = L.z2b_prefix_attention(at, _stream(dev))
+    shared = 0
+    if prefix_len > 0:
+        if prefix_pages is None or prefix_pages.numel() * kv.page_len < prefix_len:
+            _refuse("prefix_pages: a page for every page_len rows of the prefix is wanted")
+        shared = _ints(prefix_pages, prefix_pages.numel(), idx, "prefix_pages")
+    tab, tstride, pages = _table(page_table, n_seq, idx)
+    if scale is None:
+        scale = kv._scale
+    off, lens, flag = _ints(row_off, n_seq + 1, idx, "row_off"), _ints(seq_len, n_seq, idx, "seq_len"), 0 if err is None else _ints(err, 1, idx, "err")
+    L = _lib()
+    need = kv._bytes.get((n, n_seq, nh, prefix_len, pages))
+    if need is None:
+        need = L.z2b_prefix_attention_workspace(
+            _pack_attn(idx, n, n_seq, nh, prefix_len, scale, kv._at, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, pages, 0, 0, 0, 0))
+        if len(kv._bytes) > 1000:
+            kv._bytes.clear()
+        kv._bytes[(n, n_seq, nh, prefix_len, pages)] = need
+    ws = q.new_empty((need,), dtype=_U8)            # 0: the call below says what is wrong with the sizes
+    rc = L.z2b_prefix_attention(
+        _pack_attn(idx, n, n_seq, nh, prefix_len, scale, kv._at, qp, outp, 0 if lse is None else lse.data_ptr(), qr, qh, outr,
+                   outh, off, lens, tab, tstride, pages, shared, ws.data_ptr(), need, flag), _raw_stream(idx))
     if rc:
         _raise(rc)
     return out if lse is None else (out, lse)
@@ -254,29 +264,30 @@ def verify_drafts(p, q, draft, u_accept, u_draw, n_draft=None, err=None):
     float64 [streams][drafts + 1][codebooks]; n_draft [streams] int32. Returns (tokens int32
     [streams][drafts + 1][codebooks], accepted frames int32 [streams]); tokens behind the frame after
     the accepted ones are -1."""
-    dev = p.device
-    if p.dim() != 4 or not p.is_cuda or p.dtype not in _TYPE or (p.shape[3] > 1 and p.stride(3) != 1):
+    idx, code, dt = p.get_device(), _TYPE.get(p.dtype), p.dtype
+    if p.dim() != 4 or idx < 0 or code is None or p.shape[1] < 1:
         _refuse("p: a CUDA tensor [streams][drafts + 1][codebooks][vocab], f32, f16 or bf16, is wanted")
     B, N1, C, V = p.shape
-    N = N1 - 1
-    if N < 0:
-        _refuse("p: at least one frame is wanted")
-    qs = (0, 0, 0)
+    N, ps, qs, qp = N1 - 1, p.stride(), (0, 0, 0), 0
+    if ps[3] != 1 and V > 1:
+        _refuse("p: the vocabulary must be contiguous")
     if q is not None:
-        if q.shape != (B, N, C, V) or q.dtype != p.dtype or q.device != dev or (V > 1 and q.stride(3) != 1):
-            _refuse("q: [streams][drafts][codebooks][vocab] of p's type is wanted")
-        qs = q.stride()
-    for t, shape, what in ((u_accept, (B, N, C), "u_accept"), (u_draw, (B, N1, C), "u_draw")):
-        if t.dtype != torch.float64 or t.shape != shape or t.device != dev or not t.is_contiguous():
-            _refuse(f"{what}: a contiguous float64 tensor {shape} on {dev} is wanted")
-    ps = p.stride()
-    tokens = torch.empty((B, N1, C), dtype=torch.int32, device=dev)
-    kept = torch.empty((B,), dtype=torch.int32, device=dev)
-    a = VerifyArgs(dev.index, _TYPE[p.dtype], B, N, C, V, p.data_ptr(), q.data_ptr() if q is not None and N else None,
-                   _ints(draft, (B, N, C), dev, "draft"), None if n_draft is None else _ints(n_draft, (B,), dev, "n_draft"),
-                   u_accept.data_ptr(), u_draw.data_ptr(), tokens.data_ptr(), kept.data_ptr(), ps[0], ps[1], ps[2],
-                   qs[0], qs[1], qs[2], _err(err, dev))
-    rc = _lib().z2b_verify_drafts(ctypes.addressof(a), _stream(dev))
+        qs, qp = q.stride(), q.data_ptr()
+        if q.shape != (B, N, C, V) or q.dtype is not dt or q.get_device() != idx or (qs[3] != 1 and V > 1):
+            _refuse(f"q: [{B}][{N}][{C}][{V}] of p's type is wanted, the vocabulary contiguous")
+    if draft.dtype is not _I32 or draft.get_device() != idx or draft.shape != (B, N, C) or not draft.is_contiguous():
+        _refuse(f"draft: a contiguous int32 tensor [{B}][{N}][{C}] is wanted")
+    if u_accept.dtype is not _F64 or u_accept.get_device() != idx or u_accept.shape != (B, N, C) or not u_accept.is_contiguous():
+        _refuse(f"u_accept: a contiguous float64 tensor [{B}][{N}][{C}] is wanted")
+    if u_draw.dtype is not _F64 or u_draw.get_device() != idx or u_draw.shape != (B, N1, C) or not u_draw.is_contiguous():
+        _refuse(f"u_draw: a contiguous float64 tensor [{B}][{N1}][{C}] is wanted")
+    tokens = _empty_like(u_draw, dtype=_I32)
+    kept = draft.new_empty((B,))
+    rc = _lib().z2b_verify_drafts(
+        _pack_verify(idx, code, B, N, C, V, p.data_ptr(), qp, draft.data_ptr(),
+                     0 if n_draft is None else _ints(n_draft, B, idx, "n_draft"), u_accept.data_ptr(), u_draw.data_ptr(),
+                     tokens.data_ptr(), kept.data_ptr(), ps[0], ps[1], ps[2], qs[0], qs[1], qs[2],
+                     0 if err is None else _ints(err, 1, idx, "err")), _raw_stream(idx))
     if rc:
         _raise(rc)
     return tokens, kept
