@@ -8,10 +8,12 @@
 //
 // Bound: latency for frame-sized vocabularies, else the bytes of one row of p and of q per
 // drawn token: the kept tokens cost one gathered value each, and no other row is read. One
-// cluster of CTAs takes one (stream, codebook): every CTA finds the run's end for itself
-// (a handful of gathers), then the row is split over the cluster, each warp summing one
-// contiguous share; the totals are exchanged through distributed shared memory, and the
-// one CTA whose range holds the target walks the one warp's share that does.
+// CTA, or a cluster of them for large vocabularies, takes one (stream, codebook): every CTA
+// finds the run's end for itself (a handful of gathers). Then
+//   small rows: a thread holds up to EACH consecutive entries; one block scan finds the draw;
+//   large rows: the row is split over the cluster, each warp summing one contiguous share with
+//   lanes side by side; the totals are exchanged through distributed shared memory, and the one
+//   CTA whose range holds the target scans the one warp's share that does.
 //
 // The sums are f64 over exact differences of the inputs, so where they are split does not
 // move a draw except within 1e-15 of a border; u * q and the comparison are f64 as well.
@@ -26,8 +28,9 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int WARPS = 8, THREADS = 32 * WARPS;
 constexpr int MAX_CLUSTER = 8;          // CTAs per row: the portable cluster size
+constexpr int EACH = 8;                 // entries of a small row that a thread holds
+constexpr int SMALL_WARPS = 8, LARGE_WARPS = 12;
 
 struct VerifyP {
     z2b_verify_args a;
@@ -51,56 +54,100 @@ __device__ __forceinline__ double warp_sum_f64(double v) {
     return v;
 }
 
-struct DrawShared {
+template <int WARPS> struct DrawShared {
     double warp_tot[WARPS];
-    double cta_tot;                     // read by the cluster's other CTAs
+    double cta[2][MAX_CLUSTER];         // the cluster's totals, each CTA's pushed by itself; one set per draw
     double scan[WARPS];
     int found, last;
 };
 
+// The drawn token of a row of at most 32 WARPS EACH entries, or -1 when the mass is zero
+// everywhere. Called by the whole CTA; all threads get it.
+template <typename T, bool HAS_Q, bool SUB, int WARPS>
+__device__ int draw_small(const T* p, const T* q, int V, int drafted, double r, DrawShared<WARPS>& sh) {
+    const int w = threadIdx.x >> 5, lane = threadIdx.x & 31, each = (V + 32 * WARPS - 1) / (32 * WARPS);
+    const int lo = min(V, (int)threadIdx.x * each);
+    double x[EACH], mine = 0.0;
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) x[i] = i < each && lo + i < V ? left_at<T, HAS_Q, SUB>(p, q, lo + i, drafted) : 0.0;
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) mine += x[i];
+    double inc = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const double y = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += y;
+    }
+    __syncthreads();                                             // sh from an earlier draw
+    if (lane == 31) sh.warp_tot[w] = inc;
+    if (threadIdx.x == 0) { sh.found = 0x7fffffff; sh.last = -1; }
+    __syncthreads();
+    double before = 0.0, total = 0.0;
+#pragma unroll
+    for (int i = 0; i < WARPS; ++i) {
+        if (i == w) before = total;
+        total += sh.warp_tot[i];
+    }
+    if (!(total > 0.0)) return -1;
+    const double target = r * total;
+    before += inc - mine;
+    if (mine > 0.0) {
+        int last = -1, first = 0x7fffffff;
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+            before += x[i];
+            if (x[i] > 0.0) last = lo + i;
+            if (before > target && first == 0x7fffffff) first = lo + i;
+        }
+        if (first != 0x7fffffff) atomicMin(&sh.found, first);
+        else atomicMax(&sh.last, last);                          // rounding may leave the target at the total
+    }
+    __syncthreads();
+    return sh.found != 0x7fffffff ? sh.found : sh.last;
+}
+
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
+
 // The drawn token, or -1 when the mass is zero everywhere. Called by every thread of the
-// cluster; all get the same `total`, only the CTA whose range holds the target a token
-// (the others -2).
-template <typename T, bool HAS_Q, bool SUB>
-__device__ int draw(const T* p, const T* q, int V, int drafted, double r, int rank, int n_cta, DrawShared& sh) {
+// cluster, all of whose CTAs have started; all get the same `total`, only the CTA whose range
+// holds the target a token (the others -2). `set`: 0 for a cluster's first draw, 1 for its second.
+template <typename T, bool HAS_Q, bool SUB, int WARPS>
+__device__ int draw_large(const T* p, const T* q, int V, int drafted, double r, int rank, int n_cta, int set, DrawShared<WARPS>& sh) {
+    constexpr int THREADS = 32 * WARPS;
     const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int shares = n_cta * WARPS;
     const int per = (V + shares - 1) / shares;
     const int share = rank * WARPS + w;
     const int lo = min(V, share * per), hi = min(V, lo + per);
     double s0 = 0.0, s1 = 0.0;
-    int v = lo + lane;
-    for (; v + 7 * 32 < hi; v += 8 * 32) {                       // eight loads of each row in flight
+    for (int v = lo + lane; v < hi; v += 8 * 32) {               // eight loads of each row in flight
         double x[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = left_at<T, HAS_Q, SUB>(p, q, v + j * 32, drafted);
+        for (int j = 0; j < 8; ++j) x[j] = v + j * 32 < hi ? left_at<T, HAS_Q, SUB>(p, q, v + j * 32, drafted) : 0.0;
 #pragma unroll
         for (int j = 0; j < 8; j += 2) { s0 += x[j]; s1 += x[j + 1]; }
     }
-#pragma unroll 4
-    for (; v < hi; v += 32) s0 += left_at<T, HAS_Q, SUB>(p, q, v, drafted);
     const double ws = warp_sum_f64(s0 + s1);
     __syncthreads();                                             // sh from an earlier draw
     if (lane == 0) sh.warp_tot[w] = ws;
     __syncthreads();
-    if (threadIdx.x == 0) {
+    if (threadIdx.x < n_cta) {                                   // thread i hands this CTA's total to CTA i
         double t = 0.0;
         for (int i = 0; i < WARPS; ++i) t += sh.warp_tot[i];
-        sh.cta_tot = t;
-        sh.found = 0x7fffffff;
-        sh.last = -1;
+        if (n_cta > 1) *cg::this_cluster().map_shared_rank(&sh.cta[set][rank], threadIdx.x) = t;
+        else sh.cta[set][0] = t;
+        if (threadIdx.x == 0) { sh.found = 0x7fffffff; sh.last = -1; }
     }
-    cg::cluster_group cl = cg::this_cluster();
-    if (n_cta > 1) cl.sync(); else __syncthreads();
+    if (n_cta > 1) { cluster_arrive(); cluster_wait(); } else __syncthreads();
     double base = 0.0, total = 0.0;
     int owner = -1, tail = -1;                                   // the range that holds the target
     double cta[MAX_CLUSTER];
 #pragma unroll
     for (int i = 0; i < MAX_CLUSTER; ++i) {
-        cta[i] = i >= n_cta ? 0.0 : n_cta > 1 ? *cl.map_shared_rank(&sh.cta_tot, i) : sh.cta_tot;
+        cta[i] = i < n_cta ? sh.cta[set][i] : 0.0;
         total += cta[i];
     }
-    if (n_cta > 1) cl.sync();                                    // no CTA leaves or reuses its total before all read it
     if (!(total > 0.0)) return -1;
     const double target = r * total;
     double run = 0.0;
@@ -126,12 +173,19 @@ __device__ int draw(const T* p, const T* q, int V, int drafted, double r, int ra
     const int slo = min(V, (rank * WARPS + share_w) * per), shi = min(V, slo + per);
     const int each = (shi - slo + THREADS - 1) / THREADS;
     const int tlo = min(shi, slo + (int)threadIdx.x * each), thi = min(shi, tlo + each);
-    double mine = 0.0;
+    double mine = 0.0, x[EACH];
     int last = -1;
-    for (int i = tlo; i < thi; ++i) {
-        const double x = left_at<T, HAS_Q, SUB>(p, q, i, drafted);
-        if (x > 0.0) last = i;
-        mine += x;
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) x[i] = tlo + i < thi ? left_at<T, HAS_Q, SUB>(p, q, tlo + i, drafted) : 0.0;
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+        if (x[i] > 0.0) last = tlo + i;
+        mine += x[i];
+    }
+    for (int i = tlo + EACH; i < thi; ++i) {                     // vocabularies beyond what the threads hold
+        const double y = left_at<T, HAS_Q, SUB>(p, q, i, drafted);
+        if (y > 0.0) last = i;
+        mine += y;
     }
     double inc = mine;
 #pragma unroll
@@ -146,25 +200,33 @@ __device__ int draw(const T* p, const T* q, int V, int drafted, double r, int ra
     before += inc - mine;
     if (last >= 0) atomicMax(&sh.last, last);
     if (!past_w && mine > 0.0 && before + mine > target) {
-        double c = before;
-        for (int i = tlo; i < thi; ++i) {
-            c += left_at<T, HAS_Q, SUB>(p, q, i, drafted);
-            if (c > target) { atomicMin(&sh.found, i); break; }
+        int first = 0x7fffffff;
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+            before += x[i];
+            if (before > target && first == 0x7fffffff) first = tlo + i;
         }
+        for (int i = tlo + EACH; i < thi && first == 0x7fffffff; ++i) {
+            before += left_at<T, HAS_Q, SUB>(p, q, i, drafted);
+            if (before > target) first = i;
+        }
+        atomicMin(&sh.found, first);
     }
     __syncthreads();
     // rounding may leave the target at the very end of the share: its last entry with mass
     return sh.found != 0x7fffffff ? sh.found : sh.last;
 }
 
-template <typename T, bool HAS_Q>
-__global__ void __launch_bounds__(THREADS) verify_kernel(const __grid_constant__ VerifyP P) {
+template <typename T, bool HAS_Q, int WARPS>
+__global__ void __launch_bounds__(32 * WARPS) verify_kernel(const __grid_constant__ VerifyP P) {
+    constexpr int THREADS = 32 * WARPS;
     const z2b_verify_args& a = P.a;
-    __shared__ DrawShared sh;
+    __shared__ DrawShared<WARPS> sh;
     __shared__ int s_end;
     const int n_cta = P.cluster, rank = blockIdx.x % n_cta;
     const int item = blockIdx.x / n_cta, b = item / a.n_codebooks, c = item % a.n_codebooks;
     const int C = a.n_codebooks, N = a.max_draft, V = a.vocab;
+    if (n_cta > 1) cluster_arrive();                             // waited for before the first total is handed over
     pdl_wait();
     pdl_release();
     int n = a.n_draft ? a.n_draft[b] : N;
@@ -177,18 +239,19 @@ __global__ void __launch_bounds__(THREADS) verify_kernel(const __grid_constant__
     const T* q = HAS_Q ? (const T*)a.q + (long long)b * a.q_seq : nullptr;
     auto kept = [&](int f, int cb) {
         const int x = draft[f * C + cb];
+        const double u = a.u_accept[((long long)b * N + f) * C + cb];
+        if (f >= n) return true;                                 // not drafted: decides nothing
         if (x < 0 || x >= V) {
             if (a.err) atomicOr(a.err, Z2B_OPS_BAD_INDEX);
             return false;
         }
-        const double u = a.u_accept[((long long)b * N + f) * C + cb];
         const double pt = (double)to_f32(p[f * a.p_frame + cb * a.p_book + x]);
         const double qt = HAS_Q ? (double)to_f32(q[f * a.q_frame + cb * a.q_book + x]) : 1.0;
         return u * qt < pt;
     };
     if (threadIdx.x == 0) s_end = n;
     __syncthreads();
-    for (int i = threadIdx.x; i < n * C; i += THREADS)
+    for (int i = threadIdx.x; i < N * C; i += THREADS)           // all N: not waiting for n to load the drafts
         if (!kept(i / C, i % C)) atomicMin(&s_end, i / C);
     __syncthreads();
     const int end = s_end;
@@ -200,26 +263,31 @@ __global__ void __launch_bounds__(THREADS) verify_kernel(const __grid_constant__
     }
     // uniform over the cluster from here on
     const int x = end < n ? draft[end * C + c] : -1;
-    if (end < n && kept(end, c)) {
+    const bool keep = end < n && kept(end, c);
+    if (n_cta > 1) cluster_wait();
+    if (keep) {
         if (rank == 0 && threadIdx.x == 0) out[end * C] = x;
         return;
     }
     const double r = a.u_draw[((long long)b * (N + 1) + end) * C + c];
     const T* pr = p + end * a.p_frame + c * a.p_book;
+    const T* qr = HAS_Q && end < n ? q + end * a.q_frame + c * a.q_book : nullptr;
     int tok = -1;
-    if (end < n) {
-        const T* qr = HAS_Q ? q + end * a.q_frame + c * a.q_book : nullptr;
-        tok = draw<T, HAS_Q, true>(pr, qr, V, x, r, rank, n_cta, sh);
+    if constexpr (WARPS == SMALL_WARPS) {
+        if (end < n) tok = draw_small<T, HAS_Q, true, WARPS>(pr, qr, V, x, r, sh);
+        if (tok == -1) tok = draw_small<T, HAS_Q, false, WARPS>(pr, nullptr, V, -1, r, sh);
+    } else {
+        if (end < n) tok = draw_large<T, HAS_Q, true, WARPS>(pr, qr, V, x, r, rank, n_cta, 0, sh);
+        if (tok == -1) tok = draw_large<T, HAS_Q, false, WARPS>(pr, nullptr, V, -1, r, rank, n_cta, 1, sh);
     }
-    if (tok == -1) tok = draw<T, HAS_Q, false>(pr, nullptr, V, -1, r, rank, n_cta, sh);
     // -1: a row without any mass has no token; its first CTA says so
     if (threadIdx.x == 0 && (tok >= 0 || (tok == -1 && rank == 0))) out[end * C] = tok;
 }
 
-template <typename T> cudaError_t go(const VerifyP& P, bool has_q, dim3 grid, cudaStream_t s) {
+template <typename T, int WARPS> cudaError_t go(const VerifyP& P, bool has_q, dim3 grid, cudaStream_t s) {
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = grid;
-    cfg.blockDim = dim3(THREADS);
+    cfg.blockDim = dim3(32 * WARPS);
     cfg.stream = s;
     cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -228,22 +296,25 @@ template <typename T> cudaError_t go(const VerifyP& P, bool has_q, dim3 grid, cu
     at[1].val.clusterDim.x = P.cluster;
     at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
     cfg.attrs = at;
-    cfg.numAttrs = 2;
-    return has_q ? cudaLaunchKernelEx(&cfg, verify_kernel<T, true>, P) : cudaLaunchKernelEx(&cfg, verify_kernel<T, false>, P);
+    cfg.numAttrs = P.cluster > 1 ? 2 : 1;
+    return has_q ? cudaLaunchKernelEx(&cfg, verify_kernel<T, true, WARPS>, P) : cudaLaunchKernelEx(&cfg, verify_kernel<T, false, WARPS>, P);
+}
+
+template <typename T> cudaError_t go_type(VerifyP P, cudaStream_t s) {
+    const z2b_verify_args& a = P.a;
+    const long long items = (long long)a.n_seq * a.n_codebooks;
+    if (a.vocab <= 32 * SMALL_WARPS * EACH) return go<T, SMALL_WARPS>(P, a.q != nullptr, dim3((unsigned)items), s);
+    // CTAs per row: enough that one CTA's share is a few thousand entries, while all clusters
+    // are resident together (four of these CTAs an SM, 148 SMs)
+    while (P.cluster < MAX_CLUSTER && a.vocab / P.cluster > 4096 && items * P.cluster * 2 <= 592) P.cluster *= 2;
+    return go<T, LARGE_WARPS>(P, a.q != nullptr, dim3((unsigned)(items * P.cluster)), s);
 }
 
 }  // namespace
 
 cudaError_t launch_verify(const z2b_verify_args& a, cudaStream_t s) {
-    VerifyP P{a, 1};
-    // CTAs per row: enough that one CTA's share is a few thousand entries, while the
-    // clusters of all rows still fit the device about twice over (148 SMs)
-    const long long items = (long long)a.n_seq * a.n_codebooks;
-    while (P.cluster < MAX_CLUSTER && a.vocab / P.cluster > 2048 && items * P.cluster < 296) P.cluster *= 2;
-    const dim3 grid((unsigned)(items * P.cluster));
-    if (a.type == Z2B_TYPE_F32) return go<float>(P, a.q != nullptr, grid, s);
-    if (a.type == Z2B_TYPE_F16) return go<__half>(P, a.q != nullptr, grid, s);
-    return go<__nv_bfloat16>(P, a.q != nullptr, grid, s);
+    const VerifyP P{a, 1};
+    return a.type == Z2B_TYPE_F32 ? go_type<float>(P, s) : a.type == Z2B_TYPE_F16 ? go_type<__half>(P, s) : go_type<__nv_bfloat16>(P, s);
 }
 
 }  // namespace z2b
