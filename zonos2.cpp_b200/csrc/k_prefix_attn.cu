@@ -483,111 +483,225 @@ struct JoinP {
     long long o_row, o_head;
 };
 
-// W warps per (row, head): one, or where there are few rows, whose keys then lie with many
-// workers, a block of eight. The partials of both sets are numbered through; lanes take the
-// statistics of 32 at a time, then the weighted outputs are summed with each lane on its own
-// dims, four loads in flight. Bound: the chain of dependent loads; what depends on the call's
-// inputs alone is read before the wait for the launch ahead.
-template <typename T, int HD, int MT, int W>
-__global__ void __launch_bounds__(256, 4) prefix_attn_join_kernel(const __grid_constant__ JoinP p) {
-    constexpr int DPL = HD >= 32 ? HD / 32 : 1, KU = unit_keys(HD);
-    const AttnP& a = p.a;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nh = a.nkv * a.G;
-    const int item = W == 1 ? blockIdx.x * 8 + warp : blockIdx.x, t = item / nh, head = item - t * nh;
-    const int h = head / a.G, g = head - h * a.G;
-    if (t >= a.n_rows) { pdl_wait(); return; }
-    // the launches ahead release this one once their own predecessors are done: the call's inputs are there
+// Where the partial results of one head of a row lie: n0 in the prefix's set from slot0 on, n1 in
+// the stream's own, each at its row of a slot.
+struct Parts { int n0, n1, slot0, slot1, row0, row1; };
+
+// One row's stream, and the offsets of its units and segments on the line. What depends on the
+// call's inputs alone is read before the wait for the launch ahead: the launches ahead release
+// this one once their own predecessors are done.
+struct RowInfo { SeqInfo s; int i, own_units, unit_b, seg_b; bool live, scan; };
+template <int MT, int KU> __device__ __forceinline__ RowInfo row_info(const AttnP& a, int t) {
+    const int lane = threadIdx.x & 31;
+    RowInfo x;
     const int total = a.row_off[a.n_seq];
     const int b = warp_find_seq(a.row_off, a.n_seq, t);
-    const SeqInfo s = seq_info<MT, KU>(a, b);
-    int own_units = 0, unit_b = 0, seg_b = 0;
-    const bool scan = a.n_seq <= 256;                            // the line's offsets: few streams are summed here, ahead of the wait
-    if (scan) {
+    x.s = seq_info<MT, KU>(a, b);
+    x.own_units = x.unit_b = x.seg_b = 0;
+    x.scan = a.n_seq <= 256;                                     // few streams are summed here, many read from the plan
+    if (x.scan) {
         for (int c = lane; c < a.n_seq; c += 32) {
-            const SeqInfo x = seq_info<MT, KU>(a, c);
-            const int segs = x.qt * a.nkv, units = x.nt ? segs * (x.nt + SEG_COST) : 0;
-            own_units += units;
-            if (c < b) { unit_b += units; seg_b += segs; }
+            const SeqInfo y = seq_info<MT, KU>(a, c);
+            const int segs = y.qt * a.nkv, units = y.nt ? segs * (y.nt + SEG_COST) : 0;
+            x.own_units += units;
+            if (c < b) { x.unit_b += units; x.seg_b += segs; }
         }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) {
-            own_units += __shfl_xor_sync(0xffffffffu, own_units, o);
-            unit_b += __shfl_xor_sync(0xffffffffu, unit_b, o);
-            seg_b += __shfl_xor_sync(0xffffffffu, seg_b, o);
+            x.own_units += __shfl_xor_sync(0xffffffffu, x.own_units, o);
+            x.unit_b += __shfl_xor_sync(0xffffffffu, x.unit_b, o);
+            x.seg_b += __shfl_xor_sync(0xffffffffu, x.seg_b, o);
         }
     } else {
         pdl_wait();
-        own_units = a.plan[a.n_seq];
-        unit_b = a.plan[b];
-        seg_b = a.plan[a.n_seq + 1 + b];
+        x.own_units = a.plan[a.n_seq];
+        x.unit_b = a.plan[b];
+        x.seg_b = a.plan[a.n_seq + 1 + b];
     }
-    const int i = t - s.lo;
-    const bool live = t < total && !s.bad && i >= 0 && i < s.n;  // else padding, which stays as it is
+    x.i = t - x.s.lo;
+    x.live = t < total && !x.s.bad && x.i >= 0 && x.i < x.s.n;   // else padding, which stays as it is
+    return x;
+}
 
-    // the workers that hold this row's segment of the prefix, and of the stream's own rows
+template <int MT, int KU> __device__ __forceinline__ Parts find_parts(const JoinP& p, const RowInfo& x, int t, int head) {
+    const AttnP& a = p.a;
+    const int h = div_g(a, head), g = head - h * a.G;
     const int pf_units = a.pf_row_tiles * a.nkv * (cdiv(a.prefix_len, KU) + SEG_COST);
-    const int positions = pf_units + own_units;
+    const int positions = pf_units + x.own_units;
     const Cut cut(positions, p.own.workers);
-    int n0 = 0, n1 = 0, slot0 = 0, slot1 = 0, row0 = 0, row1 = 0;
-    if (live && a.prefix_len > 0) {
-        const int nt = cdiv(a.prefix_len, p.pf.keys), r = t * a.G + g, j = r / p.pf.mt, seg = p.pf_apart ? j * a.nkv + h : h * p.pf.row_tiles + j;
+    Parts r{0, 0, 0, 0, 0, 0};
+    if (a.prefix_len > 0) {
+        const int nt = cdiv(a.prefix_len, p.pf.keys), row = t * a.G + g, j = row / p.pf.mt, seg = p.pf_apart ? j * a.nkv + h : h * p.pf.row_tiles + j;
         const int cost = p.pf_apart ? TC_SEG_COST : SEG_COST, first = seg * (nt + cost) + cost;
         const int Wp = p.pf_apart ? p.pf.row_tiles * a.nkv * (nt + cost) : positions;
         const Cut cp(Wp, p.pf.workers);
         const int c0 = cp.owner(first, Wp);
-        n0 = cp.owner(first + nt - 1, Wp) - c0 + 1;
-        slot0 = seg + c0;
-        row0 = r - j * p.pf.mt;
-        if (slot0 + n0 > p.pf.max_slots) n0 = 0;
+        r.n0 = cp.owner(first + nt - 1, Wp) - c0 + 1;
+        r.slot0 = seg + c0;
+        r.row0 = row - j * p.pf.mt;
+        if (r.slot0 + r.n0 > p.pf.max_slots) r.n0 = 0;
     }
-    if (live && s.nt > 0) {
-        const int r = i * a.G + g, js = h * s.qt + r / MT;
-        const int first = pf_units + unit_b + js * (s.nt + SEG_COST) + SEG_COST;
+    if (x.s.nt > 0) {
+        const int row = x.i * a.G + g, js = h * x.s.qt + row / MT;
+        const int first = pf_units + x.unit_b + js * (x.s.nt + SEG_COST) + SEG_COST;
         const int c0 = cut.owner(first, positions);
-        n1 = cut.owner(first + s.nt - 1, positions) - c0 + 1;
-        slot1 = a.pf_row_tiles * a.nkv + seg_b + js + c0;
-        row1 = r % MT;
-        if (slot1 + n1 > p.own.max_slots) n1 = 0;                // only for offsets that do not ascend
+        r.n1 = cut.owner(first + x.s.nt - 1, positions) - c0 + 1;
+        r.slot1 = a.pf_row_tiles * a.nkv + x.seg_b + js + c0;
+        r.row1 = row % MT;
+        if (r.slot1 + r.n1 > p.own.max_slots) r.n1 = 0;          // only for offsets that do not ascend
     }
-    const int n = n0 + n1;
-    if (scan) pdl_wait();
+    return r;
+}
+
+// Statistics and address of partial k of a head.
+template <int HD> __device__ __forceinline__ void part(const JoinP& p, const Parts& r, int k, float2& ml, const float*& src) {
+    ml = make_float2(-INFINITY, 0.0f);
+    src = p.own.o;
+    if (k < r.n0 + r.n1) {
+        const PartSet& ps = k < r.n0 ? p.pf : p.own;
+        const size_t at = k < r.n0 ? (size_t)(r.slot0 + k) * ps.mt + r.row0 : (size_t)(r.slot1 + k - r.n0) * ps.mt + r.row1;
+        ml = ps.ml[at];
+        src = ps.o + at * HD;
+    }
+}
+
+template <int DPL, int HD> __device__ __forceinline__ void load_dims(const float* src, int lane, float (&v)[DPL]) {
+    if constexpr (DPL == 4) {
+        const float4 x = *(const float4*)(src + lane * 4);
+        v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+    } else if constexpr (DPL == 2) {
+        const float2 x = *(const float2*)(src + lane * 2);
+        v[0] = x.x; v[1] = x.y;
+    } else {
+        v[0] = HD >= 32 || lane < HD ? src[lane] : 0.0f;
+    }
+}
+
+template <typename T, int DPL, int HD>
+__device__ __forceinline__ void put_row(const JoinP& p, int t, int head, int lane, float M, float L, const float (&acc)[DPL]) {
+    const float inv = L > 0.0f ? 1.0f / L : 0.0f;
+    if (HD >= 32 || lane < HD) {
+        T* dst = (T*)p.out + (long long)t * p.o_row + (long long)head * p.o_head + lane * DPL;
+        if constexpr (DPL == 1) *dst = from_f32<T>(acc[0] * inv);
+        else {
+#pragma unroll
+            for (int d = 0; d < DPL; d += 2) *(uint32_t*)(dst + d) = pack2<T>(acc[d] * inv, acc[d + 1] * inv);
+        }
+    }
+    // ln(sum) = (M + log2 L) ln 2
+    if (lane == 0 && p.lse) p.lse[(long long)t * (p.a.nkv * p.a.G) + head] = L > 0.0f ? (M + log2f(L)) * 0.6931471805599453f : -INFINITY;
+}
+
+// Many rows: a warp per row and four heads. Lane 8 g + k takes the statistics of partial k of
+// head g (8 at a time), then the outputs are summed with each lane on its own dims, the four
+// heads' loads in flight together and the first ahead of the weights. Bound: the bytes of the
+// partials once resident, the chain of dependent loads (statistics, outputs) before.
+template <typename T, int HD, int MT>
+__global__ void __launch_bounds__(128, 4) prefix_attn_join_kernel(const __grid_constant__ JoinP p) {
+    constexpr int DPL = HD >= 32 ? HD / 32 : 1, KU = unit_keys(HD), GH = 4;
+    const AttnP& a = p.a;
+    const int lane = threadIdx.x & 31, nh = a.nkv * a.G, groups = cdiv(nh, GH);
+    const int item = blockIdx.x * 4 + (threadIdx.x >> 5), t = item / groups, head0 = (item - t * groups) * GH;
+    if (t >= a.n_rows) { pdl_wait(); return; }
+    const RowInfo x = row_info<MT, KU>(a, t);
+    const int g = lane >> 3, k_l = lane & 7;
+    Parts r{0, 0, 0, 0, 0, 0};
+    if (x.live && head0 + g < nh) r = find_parts<MT, KU>(p, x, t, head0 + g);
+    if (x.scan) pdl_wait();
     pdl_release();
-    if (!live) return;
+    if (!x.live) return;
+    const int n = r.n0 + r.n1;
+    int most = n;
+#pragma unroll
+    for (int o = 8; o < 32; o <<= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+    float M = -INFINITY, L = 0.0f, acc[GH][DPL];                 // M, L: of head g
+#pragma unroll
+    for (int h = 0; h < GH; ++h)
+#pragma unroll
+        for (int d = 0; d < DPL; ++d) acc[h][d] = 0.0f;
+    for (int base = 0; base < most; base += 8) {
+        float2 ml;
+        const float* src;
+        part<HD>(p, r, base + k_l, ml, src);
+        const int cnt = min(8, most - base);
+        float wt = 0.0f;
+        for (int k = 0; k < cnt; ++k) {
+            float v[GH][DPL];
+#pragma unroll
+            for (int h = 0; h < GH; ++h) {
+                const float* sp = (const float*)__shfl_sync(0xffffffffu, (unsigned long long)src, h * 8 + k);
+                const bool has = base + k < __shfl_sync(0xffffffffu, n, h * 8);
+#pragma unroll
+                for (int d = 0; d < DPL; ++d) v[h][d] = 0.0f;
+                if (has) load_dims<DPL, HD>(sp, lane, v[h]);
+            }
+            if (k == 0) {
+                float top = ml.x, sum;
+#pragma unroll
+                for (int o = 1; o < 8; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                top = fmaxf(M, top);
+                const float to = top == -INFINITY ? 0.0f : top;  // no partial has seen a key
+                const float f = ex2(M - to);
+                wt = ex2(ml.x - to);
+                sum = ml.y * wt;
+#pragma unroll
+                for (int o = 1; o < 8; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                M = top;
+                L = L * f + sum;
+#pragma unroll
+                for (int h = 0; h < GH; ++h) {
+                    const float fh = __shfl_sync(0xffffffffu, f, h * 8);
+#pragma unroll
+                    for (int d = 0; d < DPL; ++d) acc[h][d] *= fh;
+                }
+            }
+#pragma unroll
+            for (int h = 0; h < GH; ++h) {
+                const float wk = __shfl_sync(0xffffffffu, wt, h * 8 + k);
+#pragma unroll
+                for (int d = 0; d < DPL; ++d) acc[h][d] += wk * v[h][d];
+            }
+        }
+    }
+#pragma unroll
+    for (int h = 0; h < GH; ++h) {
+        const float Mh = __shfl_sync(0xffffffffu, M, h * 8), Lh = __shfl_sync(0xffffffffu, L, h * 8);
+        if (head0 + h < nh) put_row<T, DPL, HD>(p, t, head0 + h, lane, Mh, Lh, acc[h]);
+    }
+}
+
+// Few rows, whose keys then lie with many workers: a block of eight warps per row and head, warp
+// w taking the partials w, w + 8, ...
+template <typename T, int HD, int MT>
+__global__ void __launch_bounds__(256, 4) prefix_attn_join_few_kernel(const __grid_constant__ JoinP p) {
+    constexpr int DPL = HD >= 32 ? HD / 32 : 1, KU = unit_keys(HD), W = 8;
+    const AttnP& a = p.a;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nh = a.nkv * a.G;
+    const int t = blockIdx.x / nh, head = blockIdx.x - t * nh;
+    const RowInfo x = row_info<MT, KU>(a, t);
+    Parts r{0, 0, 0, 0, 0, 0};
+    if (x.live) r = find_parts<MT, KU>(p, x, t, head);
+    if (x.scan) pdl_wait();
+    pdl_release();
+    if (!x.live) return;
+    const int n = r.n0 + r.n1;
     float M = -INFINITY, L = 0.0f, acc[DPL];
 #pragma unroll
     for (int d = 0; d < DPL; ++d) acc[d] = 0.0f;
-    for (int base = 0; base < n; base += 32 * W) {
-        const int k = base + lane * W + (W > 1 ? warp : 0);      // W > 1: warp w has the partials w, w + W, ...
-        float2 ml = make_float2(-INFINITY, 0.0f);
-        const float* src = p.own.o;
-        if (k < n) {
-            const PartSet& ps = k < n0 ? p.pf : p.own;
-            const size_t at = k < n0 ? (size_t)(slot0 + k) * ps.mt + row0 : (size_t)(slot1 + k - n0) * ps.mt + row1;
-            ml = ps.ml[at];
-            src = ps.o + at * HD;
-        }
-        const int cnt = min(32, cdiv(n - base - (W > 1 ? warp : 0), W));
+    for (int base = warp; base < n; base += 32 * W) {
+        float2 ml;
+        const float* src;
+        part<HD>(p, r, base + lane * W, ml, src);
+        const int cnt = min(32, cdiv(n - base, W));
         float wt = 0.0f;
         for (int k0 = 0; k0 < cnt; k0 += 4) {
             float v[4][DPL];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float* sp = (const float*)__shfl_sync(0xffffffffu, (unsigned long long)src, min(k0 + e, cnt - 1));
-                if (HD >= 32 || lane < HD) {
-                    if constexpr (DPL == 4) {
-                        const float4 x = *(const float4*)(sp + lane * 4);
-                        v[e][0] = x.x; v[e][1] = x.y; v[e][2] = x.z; v[e][3] = x.w;
-                    } else if constexpr (DPL == 2) {
-                        const float2 x = *(const float2*)(sp + lane * 2);
-                        v[e][0] = x.x; v[e][1] = x.y;
-                    } else {
-                        v[e][0] = sp[lane];
-                    }
-                }
-            }
+            for (int e = 0; e < 4; ++e)
+                load_dims<DPL, HD>((const float*)__shfl_sync(0xffffffffu, (unsigned long long)src, min(k0 + e, cnt - 1)), lane, v[e]);
             if (k0 == 0) {                                       // the weights, with the first outputs on their way
                 const float top = fmaxf(M, warp_max(ml.x));
-                const float to = top == -INFINITY ? 0.0f : top;  // no partial has seen a key
+                const float to = top == -INFINITY ? 0.0f : top;
                 const float f = ex2(M - to);
                 wt = ex2(ml.x - to);
                 M = top;
@@ -604,36 +718,24 @@ __global__ void __launch_bounds__(256, 4) prefix_attn_join_kernel(const __grid_c
             }
         }
     }
-    if constexpr (W > 1) {                                       // the block's warps, in a fixed order
-        __shared__ float s_acc[W][HD + 2];
-        if (lane == 0) { s_acc[warp][HD] = M; s_acc[warp][HD + 1] = L; }
+    __shared__ float s_acc[W][HD + 2];                           // the block's warps, in a fixed order
+    if (lane == 0) { s_acc[warp][HD] = M; s_acc[warp][HD + 1] = L; }
+    if (HD >= 32 || lane < HD)
+#pragma unroll
+        for (int d = 0; d < DPL; ++d) s_acc[warp][lane * DPL + d] = acc[d];
+    __syncthreads();
+    if (warp > 0) return;
+    for (int w = 1; w < W; ++w) {
+        const float top = fmaxf(M, s_acc[w][HD]);
+        if (top == -INFINITY) continue;
+        const float f = ex2(M - top), fw = ex2(s_acc[w][HD] - top);
+        M = top;
+        L = L * f + s_acc[w][HD + 1] * fw;
         if (HD >= 32 || lane < HD)
 #pragma unroll
-            for (int d = 0; d < DPL; ++d) s_acc[warp][lane * DPL + d] = acc[d];
-        __syncthreads();
-        if (warp > 0) return;
-        for (int w = 1; w < W; ++w) {
-            const float top = fmaxf(M, s_acc[w][HD]);
-            if (top == -INFINITY) continue;
-            const float f = ex2(M - top), fw = ex2(s_acc[w][HD] - top);
-            M = top;
-            L = L * f + s_acc[w][HD + 1] * fw;
-            if (HD >= 32 || lane < HD)
-#pragma unroll
-                for (int d = 0; d < DPL; ++d) acc[d] = acc[d] * f + s_acc[w][lane * DPL + d] * fw;
-        }
+            for (int d = 0; d < DPL; ++d) acc[d] = acc[d] * f + s_acc[w][lane * DPL + d] * fw;
     }
-    const float inv = L > 0.0f ? 1.0f / L : 0.0f;
-    if (HD >= 32 || lane < HD) {
-        T* dst = (T*)p.out + (long long)t * p.o_row + (long long)head * p.o_head + lane * DPL;
-        if constexpr (DPL == 1) *dst = from_f32<T>(acc[0] * inv);
-        else {
-#pragma unroll
-            for (int d = 0; d < DPL; d += 2) *(uint32_t*)(dst + d) = pack2<T>(acc[d] * inv, acc[d + 1] * inv);
-        }
-    }
-    // ln(sum) = (M + log2 L) ln 2
-    if (lane == 0 && p.lse) p.lse[(long long)t * nh + head] = L > 0.0f ? (M + log2f(L)) * 0.6931471805599453f : -INFINITY;
+    put_row<T, DPL, HD>(p, t, head, lane, M, L, acc);
 }
 
 // ---- host -----------------------------------------------------------------------------------
@@ -702,10 +804,11 @@ cudaError_t go_attn(const AttnP& p, const CUtensorMap& km, const CUtensorMap& vm
 
 template <typename T, int HD, int MT>
 cudaError_t go_join(const JoinP& j, const z2b_prefix_attn_args& a, cudaStream_t s) {
-    const long long items = (long long)a.n_rows * a.n_head;
     // a block per row and head while those are fewer than two blocks an SM hold in warps
-    if (items <= 148 * 16) return launch_pdl(prefix_attn_join_kernel<T, HD, MT, 8>, dim3((unsigned)items), dim3(256), 0, s, j);
-    return launch_pdl(prefix_attn_join_kernel<T, HD, MT, 1>, dim3((unsigned)((items + 7) / 8)), dim3(256), 0, s, j);
+    const long long items = (long long)a.n_rows * a.n_head;
+    if (items <= 148 * 16) return launch_pdl(prefix_attn_join_few_kernel<T, HD, MT>, dim3((unsigned)items), dim3(256), 0, s, j);
+    const long long warps = (long long)a.n_rows * ((a.n_head + 3) / 4);
+    return launch_pdl(prefix_attn_join_kernel<T, HD, MT>, dim3((unsigned)((warps + 3) / 4)), dim3(128), 0, s, j);
 }
 
 template <typename T, int HD>
