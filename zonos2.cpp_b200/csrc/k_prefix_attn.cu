@@ -593,12 +593,12 @@ __device__ __forceinline__ void put_row(const JoinP& p, int t, int head, int lan
 }
 
 // Many rows: a warp per row and four heads. Lane 8 g + k takes the statistics of partial k of
-// head g (8 at a time), then the outputs are summed with each lane on its own dims, the four
-// heads' loads in flight together and the first ahead of the weights. Bound: the bytes of the
-// partials once resident, the chain of dependent loads (statistics, outputs) before.
+// head g (8 at a time), then the outputs are summed with each lane on its own dims: those of
+// four heads and KB partials in flight together, and the first ahead of the weights. Bound: the
+// chain of dependent loads (statistics, outputs) and the bytes of the partials.
 template <typename T, int HD, int MT>
 __global__ void __launch_bounds__(128, 4) prefix_attn_join_kernel(const __grid_constant__ JoinP p) {
-    constexpr int DPL = HD >= 32 ? HD / 32 : 1, KU = unit_keys(HD), GH = 4;
+    constexpr int DPL = HD >= 32 ? HD / 32 : 1, KU = unit_keys(HD), GH = 4, KB = DPL == 4 ? 4 : 8;
     const AttnP& a = p.a;
     const int lane = threadIdx.x & 31, nh = a.nkv * a.G, groups = cdiv(nh, GH);
     const int item = blockIdx.x * 4 + (threadIdx.x >> 5), t = item / groups, head0 = (item - t * groups) * GH;
@@ -625,17 +625,20 @@ __global__ void __launch_bounds__(128, 4) prefix_attn_join_kernel(const __grid_c
         part<HD>(p, r, base + k_l, ml, src);
         const int cnt = min(8, most - base);
         float wt = 0.0f;
-        for (int k = 0; k < cnt; ++k) {
-            float v[GH][DPL];
+        for (int k0 = 0; k0 < cnt; k0 += KB) {
+            float v[KB][GH][DPL];
 #pragma unroll
-            for (int h = 0; h < GH; ++h) {
-                const float* sp = (const float*)__shfl_sync(0xffffffffu, (unsigned long long)src, h * 8 + k);
-                const bool has = base + k < __shfl_sync(0xffffffffu, n, h * 8);
+            for (int e = 0; e < KB; ++e)
 #pragma unroll
-                for (int d = 0; d < DPL; ++d) v[h][d] = 0.0f;
-                if (has) load_dims<DPL, HD>(sp, lane, v[h]);
-            }
-            if (k == 0) {
+                for (int h = 0; h < GH; ++h) {
+                    const int from = h * 8 + min(k0 + e, 7);
+                    const float* sp = (const float*)__shfl_sync(0xffffffffu, (unsigned long long)src, from);
+                    const bool has = k0 + e < 8 && base + k0 + e < __shfl_sync(0xffffffffu, n, h * 8);
+#pragma unroll
+                    for (int d = 0; d < DPL; ++d) v[e][h][d] = 0.0f;
+                    if (has) load_dims<DPL, HD>(sp, lane, v[e][h]);
+                }
+            if (k0 == 0) {
                 float top = ml.x, sum;
 #pragma unroll
                 for (int o = 1; o < 8; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
@@ -656,11 +659,13 @@ __global__ void __launch_bounds__(128, 4) prefix_attn_join_kernel(const __grid_c
                 }
             }
 #pragma unroll
-            for (int h = 0; h < GH; ++h) {
-                const float wk = __shfl_sync(0xffffffffu, wt, h * 8 + k);
+            for (int e = 0; e < KB; ++e)
 #pragma unroll
-                for (int d = 0; d < DPL; ++d) acc[h][d] += wk * v[h][d];
-            }
+                for (int h = 0; h < GH; ++h) {                   // outputs that are not there are zeros
+                    const float wk = __shfl_sync(0xffffffffu, wt, h * 8 + min(k0 + e, 7));
+#pragma unroll
+                    for (int d = 0; d < DPL; ++d) acc[h][d] += wk * v[e][h][d];
+                }
         }
     }
 #pragma unroll
