@@ -510,3 +510,61 @@ def test_prefix_attention_many_streams():
     out, lse = ops.prefix_attention(s.kv, q, s.d_off, s.d_lens, s.d_table, s.d_shared, 20, lse=True, err=s.err)
     ops.check(s.err)
     _check_attention(s, q, out, lse)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=str)
+@pytest.mark.parametrize("B", [2, 40], ids=str)
+def test_prefix_attention_small_probabilities(dtype, B):
+    """One key takes nearly all, 4000 others 2^-27 of it each: their share is not lost below f16's
+    range. The probabilities are held times 2^7, so one of 2^-27 is a multiple of 2^-24 off by 2^-25
+    at most: 2^-5 of it; the result (3e-5) by another half step of its type."""
+    P = 4001
+    s = Streams([1] * B, [1] * B, 16, 1, 64, dtype, prefix=P, seed=18)
+    for c in (s.kv.k, s.kv.v):
+        c.zero_()
+    s.kv.v.fill_(1.0)
+    first = int(s.shared[0])
+    s.kv.k[first, 0, 0, 0] = 4.6875
+    s.kv.v[first, 0] = 0.0
+    q = torch.zeros((B, 4, 64), dtype=dtype, device=DEV)
+    q[:, :, 0] = 4.0
+    out = ops.prefix_attention(s.kv, q, s.d_off, s.d_lens, s.d_table, s.d_shared, P, scale=1.0, err=s.err)
+    ops.check(s.err)
+    small = (P - 1 + 1) * math.exp(-18.75)                   # the prefix's other keys and the stream's own
+    want = small / (1 + small)
+    assert ((out.double() - want).abs() <= want * 2.0 ** -5 + max(2.0 ** -25, torch.finfo(dtype).eps / 2 * want)).all()
+
+
+def test_binding_refuses_numbers_out_of_range():
+    s = Streams([1], [4], 16, 2, 64, F16)
+    q = torch.zeros((1, 4, 64), dtype=F16, device=DEV)
+    for n in (-1, 2 ** 40):
+        with pytest.raises(R.Z2BError):
+            ops.prefix_attention(s.kv, q, s.d_off, s.d_lens, s.d_table, s.shared.new_zeros(1 << 4).to(DEV), n)
+        with pytest.raises(R.Z2BError):
+            ops.rope_append(None, s.kv, q, None, None, s.d_off, s.d_lens, s.d_table, prefix_len=n)
+
+
+def test_cache_of_one_head_or_page_in_any_order():
+    """Strides along dimensions of one (a transposed view's) say nothing."""
+    g = _gen(19)
+    k, v = (torch.randn((1, 32, 64), generator=g).to(F16).to(DEV).as_strided((1, 32, 1, 64), (3, 64, 5, 1)) for _ in range(2))
+    kv = ops.PagedKV(k, v)
+    q = torch.randn((1, 4, 64), generator=g).to(F16).to(DEV)
+    out, lse = ops.prefix_attention(kv, q, _i32([0, 1]), _i32([20]), _i32([[0]]), lse=True)
+    plain = ops.PagedKV(k.contiguous().view(1, 32, 1, 64).clone(), v.contiguous().view(1, 32, 1, 64).clone())
+    want, wlse = ops.prefix_attention(plain, q, _i32([0, 1]), _i32([20]), _i32([[0]]), lse=True)
+    assert torch.equal(out, want) and torch.equal(lse, wlse)
+
+
+def test_prefix_attention_unaligned_queries_and_in_place():
+    """q at an odd pair of elements (no 16-byte rows), few rows and many; out may be q itself."""
+    for B in (3, 40):
+        s = Streams([1] * B, [5] * B, 16, 2, 64, BF16, prefix=150, seed=20)
+        buf = torch.randn((B, 2 + 8 * 64), generator=_gen(21)).to(BF16).to(DEV)
+        q = buf[:, 2:].unflatten(1, (8, 64))
+        kept = q.clone()
+        lse = torch.zeros((B, 8), device=DEV)
+        assert ops.prefix_attention(s.kv, q, s.d_off, s.d_lens, s.d_table, s.d_shared, 150, out=q, lse=lse, err=s.err)[0] is q
+        ops.check(s.err)
+        _check_attention(s, kept, q, lse)

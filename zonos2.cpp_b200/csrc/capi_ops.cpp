@@ -24,14 +24,18 @@ struct DeviceGuard {
     ~DeviceGuard() { if (prev >= 0) cudaSetDevice(prev); }
 };
 
-int bad(const char* what) { set_error(what); return Z2B_ERR_ARG; }
-int unsupported(const char* what) { set_error(what); return Z2B_ERR_UNSUPPORTED; }
+// No exception leaves a C entry point, not even for want of memory for the message.
+int fail(int rc, const char* what, const char* more = "") {
+    try { set_error(std::string(what) + more); } catch (...) {}
+    return rc;
+}
+int bad(const char* what) { return fail(Z2B_ERR_ARG, what); }
+int unsupported(const char* what) { return fail(Z2B_ERR_UNSUPPORTED, what); }
 
 int launched(cudaError_t e, const char* op) {
     if (e == cudaSuccess) return Z2B_OK;
     cudaGetLastError();                                  // a refused launch leaves nothing behind
-    set_error(std::string(op) + ": " + cudaGetErrorString(e));
-    return e == cudaErrorNotSupported ? Z2B_ERR_UNSUPPORTED : Z2B_ERR_CUDA;
+    return fail(e == cudaErrorNotSupported ? Z2B_ERR_UNSUPPORTED : Z2B_ERR_CUDA, op, cudaGetErrorString(e));
 }
 
 bool aligned(const void* p, unsigned n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
@@ -117,8 +121,8 @@ int z2b_rope_append(const z2b_rope_append_args* args, void* stream) {
     m = check_rows(a.n_seq, a.row_off, a.seq_len, a.page_table, a.table_stride, a.max_pages);
     if (*m) return bad(m);
     DeviceGuard g(a.device);
-    if (g.rc != cudaSuccess) return launched(g.rc, "rope_append: device");
-    return launched(launch_rope_append(a, (cudaStream_t)stream), "rope_append");
+    if (g.rc != cudaSuccess) return launched(g.rc, "rope_append: device: ");
+    return launched(launch_rope_append(a, (cudaStream_t)stream), "rope_append: ");
 }
 
 static const char* check_attn(const z2b_prefix_attn_args& a, int* rc) {
@@ -136,7 +140,7 @@ static const char* check_attn(const z2b_prefix_attn_args& a, int* rc) {
     // unit and slot numbers are 32-bit
     const long long G = a.n_head / c.n_head_kv, tiles = ((long long)a.n_rows * G + 7) / 8;
     const long long own = ((long long)a.max_pages * c.page_len + 31) / 32 + 1, pf = ((long long)a.prefix_len + 31) / 32 + 1;
-    if (tiles * c.n_head_kv > (1 << 24) || (long long)a.n_seq * c.n_head_kv > (1 << 24) || own > (1 << 24) ||
+    if (tiles * c.n_head_kv > (1 << 24) || (long long)a.n_seq * c.n_head_kv > (1 << 24) || own > (1 << 24) || pf > (1 << 24) ||
         ((long long)a.n_rows + 32) * G * G > 0xffffffffll || (tiles + a.n_seq) * c.n_head_kv * own > 0x7fffffffll || (tiles + 1) * c.n_head_kv * pf > 0x7fffffffll)
         return "prefix_attention: too many rows, streams or pages for one call";
     return "";
@@ -144,9 +148,9 @@ static const char* check_attn(const z2b_prefix_attn_args& a, int* rc) {
 
 size_t z2b_prefix_attention_workspace(const z2b_prefix_attn_args* args) {
     int rc;
-    if (!args) { set_error("prefix_attention: null argument"); return 0; }
+    if (!args) { bad("prefix_attention: null argument"); return 0; }
     const char* m = check_attn(*args, &rc);
-    if (*m) { set_error(m); return 0; }
+    if (*m) { fail(rc, m); return 0; }
     if (args->n_rows == 0 || args->n_seq == 0) return 256;
     return prefix_attention_bytes(*args);
 }
@@ -156,7 +160,7 @@ int z2b_prefix_attention(const z2b_prefix_attn_args* args, void* stream) {
     const z2b_prefix_attn_args& a = *args;
     int rc;
     const char* m = check_attn(a, &rc);
-    if (*m) { set_error(m); return rc; }
+    if (*m) return fail(rc, m);
     const z2b_paged_kv& c = *a.kv;
     if (!aligned(c.k, 16) || !aligned(c.v, 16) || (c.page_stride | c.row_stride | c.head_stride) % 8)
         return bad("prefix_attention: the cache must be 16-byte aligned with strides that are multiples of 8");
@@ -171,8 +175,8 @@ int z2b_prefix_attention(const z2b_prefix_attn_args* args, void* stream) {
     if (!a.workspace || !aligned(a.workspace, 16)) return bad("prefix_attention: the workspace must be 16-byte aligned");
     if (a.workspace_bytes < prefix_attention_bytes(a)) return bad("prefix_attention: the workspace is too small");
     DeviceGuard g(a.device);
-    if (g.rc != cudaSuccess) return launched(g.rc, "prefix_attention: device");
-    return launched(launch_prefix_attention(a, (cudaStream_t)stream), "prefix_attention");
+    if (g.rc != cudaSuccess) return launched(g.rc, "prefix_attention: device: ");
+    return launched(launch_prefix_attention(a, (cudaStream_t)stream), "prefix_attention: ");
 }
 
 int z2b_verify_drafts(const z2b_verify_args* args, void* stream) {
@@ -190,8 +194,8 @@ int z2b_verify_drafts(const z2b_verify_args* args, void* stream) {
         !aligned(a.u_draw, 8) || !aligned(a.tokens, 4) || !aligned(a.n_accepted, 4))
         return bad("verify_drafts: misaligned array");
     DeviceGuard g(a.device);
-    if (g.rc != cudaSuccess) return launched(g.rc, "verify_drafts: device");
-    return launched(launch_verify(a, (cudaStream_t)stream), "verify_drafts");
+    if (g.rc != cudaSuccess) return launched(g.rc, "verify_drafts: device: ");
+    return launched(launch_verify(a, (cudaStream_t)stream), "verify_drafts: ");
 }
 
 }  // extern "C"

@@ -130,7 +130,7 @@ __global__ void __launch_bounds__(32 * max_warps(HD), 1) prefix_attn_kernel(cons
     if (threadIdx.x == 0) { prefetch_map(&kmap); prefetch_map(&vmap); }
     if (!p.after_prefix) pdl_wait();
     pdl_release();                                               // the join reads its streams' extents meanwhile
-    const int last_off = p.row_off[p.n_seq];
+    const int last_off = ld_word(p.row_off + p.n_seq, p.after_prefix);
 
     // ---- the line: offsets of every stream's units and segments, by a block scan
     {
@@ -138,7 +138,7 @@ __global__ void __launch_bounds__(32 * max_warps(HD), 1) prefix_attn_kernel(cons
         const int b0 = min(p.n_seq, (int)threadIdx.x * per), b1 = min(p.n_seq, b0 + per);
         int su = 0, sg = 0;
         for (int b = b0; b < b1; ++b) {
-            const SeqInfo s = seq_info<MT, KU>(p, b);
+            const SeqInfo s = seq_info<MT, KU>(p, b, p.after_prefix);
             if (s.bad && blockIdx.x == 0 && p.err) atomicOr(p.err, Z2B_OPS_BAD_INDEX);
             s_rec[b] = make_int4(su, sg, s.lo, s.n);
             s_len[b] = s.len;
@@ -207,7 +207,7 @@ __global__ void __launch_bounds__(32 * max_warps(HD), 1) prefix_attn_kernel(cons
         page = p.n_pages;                                        // out of the view: the box fills with zeros
         wanted = false;
         if (lane < nb && (ui - gi.unit0) * KU + lane * p.box_rows < gi.klen) {
-            page = gi.pages[pidx];                               // on its way until copy() checks it
+            page = ld_word(gi.pages + pidx, p.after_prefix);     // on its way until copy() checks it
             wanted = true;
         }
     };
@@ -249,8 +249,7 @@ __global__ void __launch_bounds__(32 * max_warps(HD), 1) prefix_attn_kernel(cons
             if (q16) cp_async16(dst, src, live);
             else
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" :: "r"(smem_u32(dst) + 4 * e), "l"(src + (live ? 2 * e : 0)), "r"(live ? 4 : 0) : "memory");
+                for (int e = 0; e < 4; ++e) ((uint32_t*)dst)[e] = live ? (uint32_t)ld_word((const int*)(src + 2 * e), p.after_prefix) : 0u;
         }
         cp_async_commit();
     };
@@ -381,8 +380,6 @@ __global__ void __launch_bounds__(32 * max_warps(HD), 1) prefix_attn_kernel(cons
                     top[nb_][x] *= sc;
                     raise |= top[nb_][x] > m[nb_][x] + LAG;
                 }
-            // a maximum is raised only when it would lag by more than 2^8: sums and O are f32 and the
-            // probabilities stay below that, so nothing overflows, and rescaling becomes rare
             if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
                 for (int nb_ = 0; nb_ < NB; ++nb_) {
@@ -391,8 +388,9 @@ __global__ void __launch_bounds__(32 * max_warps(HD), 1) prefix_attn_kernel(cons
                     for (int x = 0; x < 2; ++x) {
                         f[x] = 1.0f;
                         if (top[nb_][x] > m[nb_][x] + LAG) {
-                            f[x] = ex2(m[nb_][x] - top[nb_][x]);
-                            m[nb_][x] = top[nb_][x];
+                            const float to = top[nb_][x] - P_SHIFT;
+                            f[x] = ex2(m[nb_][x] - to);
+                            m[nb_][x] = to;
                         }
                         l[nb_][x] *= f[x];
                     }
@@ -487,21 +485,21 @@ struct JoinP {
 // the stream's own, each at its row of a slot.
 struct Parts { int n0, n1, slot0, slot1, row0, row1; };
 
-// One row's stream, and the offsets of its units and segments on the line. What depends on the
-// call's inputs alone is read before the wait for the launch ahead: the launches ahead release
-// this one once their own predecessors are done.
-struct RowInfo { SeqInfo s; int i, own_units, unit_b, seg_b; bool live, scan; };
-template <int MT, int KU> __device__ __forceinline__ RowInfo row_info(const AttnP& a, int t) {
+// One row's stream, found ahead of the launch's wait (the launches ahead release this one once
+// their own predecessors are done, so the call's inputs are there; they are read past L1), and the
+// offsets of its units and segments on the line: read from the plan after the wait, or (EARLY)
+// summed by the warp from the inputs, and the caller waits.
+struct RowInfo { SeqInfo s; int i, own_units, unit_b, seg_b; bool live; };
+template <int MT, int KU, bool EARLY> __device__ __forceinline__ RowInfo row_info(const AttnP& a, int t) {
     const int lane = threadIdx.x & 31;
     RowInfo x;
-    const int total = a.row_off[a.n_seq];
-    const int b = warp_find_seq(a.row_off, a.n_seq, t);
-    x.s = seq_info<MT, KU>(a, b);
-    x.own_units = x.unit_b = x.seg_b = 0;
-    x.scan = a.n_seq <= 256;                                     // few streams are summed here, many read from the plan
-    if (x.scan) {
+    const int total = ld_word(a.row_off + a.n_seq, true);
+    const int b = warp_find_seq(a.row_off, a.n_seq, t, true);
+    x.s = seq_info<MT, KU>(a, b, true);
+    if constexpr (EARLY) {
+        x.own_units = x.unit_b = x.seg_b = 0;
         for (int c = lane; c < a.n_seq; c += 32) {
-            const SeqInfo y = seq_info<MT, KU>(a, c);
+            const SeqInfo y = seq_info<MT, KU>(a, c, true);
             const int segs = y.qt * a.nkv, units = y.nt ? segs * (y.nt + SEG_COST) : 0;
             x.own_units += units;
             if (c < b) { x.unit_b += units; x.seg_b += segs; }
@@ -603,13 +601,12 @@ __global__ void __launch_bounds__(128, 4) prefix_attn_join_kernel(const __grid_c
     const int lane = threadIdx.x & 31, nh = a.nkv * a.G, groups = cdiv(nh, GH);
     const int item = blockIdx.x * 4 + (threadIdx.x >> 5), t = item / groups, head0 = (item - t * groups) * GH;
     if (t >= a.n_rows) { pdl_wait(); return; }
-    const RowInfo x = row_info<MT, KU>(a, t);
-    const int g = lane >> 3, k_l = lane & 7;
-    Parts r{0, 0, 0, 0, 0, 0};
-    if (x.live && head0 + g < nh) r = find_parts<MT, KU>(p, x, t, head0 + g);
-    if (x.scan) pdl_wait();
+    const RowInfo x = row_info<MT, KU, false>(a, t);
     pdl_release();
     if (!x.live) return;
+    const int g = lane >> 3, k_l = lane & 7;
+    Parts r{0, 0, 0, 0, 0, 0};
+    if (head0 + g < nh) r = find_parts<MT, KU>(p, x, t, head0 + g);
     const int n = r.n0 + r.n1;
     int most = n;
 #pragma unroll
@@ -676,19 +673,30 @@ __global__ void __launch_bounds__(128, 4) prefix_attn_join_kernel(const __grid_c
 }
 
 // Few rows, whose keys then lie with many workers: a block of eight warps per row and head, warp
-// w taking the partials w, w + 8, ...
+// w taking the partials w, w + 8, ... All blocks are resident while the launch ahead still runs,
+// so warp 0 finds the head's parts meanwhile, where the streams are few enough to sum (each word
+// asked for once a block: by every warp, the words' L2 slice takes 3 us more on 16 streams).
 template <typename T, int HD, int MT>
 __global__ void __launch_bounds__(256, 4) prefix_attn_join_few_kernel(const __grid_constant__ JoinP p) {
     constexpr int DPL = HD >= 32 ? HD / 32 : 1, KU = unit_keys(HD), W = 8;
     const AttnP& a = p.a;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nh = a.nkv * a.G;
     const int t = blockIdx.x / nh, head = blockIdx.x - t * nh;
-    const RowInfo x = row_info<MT, KU>(a, t);
-    Parts r{0, 0, 0, 0, 0, 0};
-    if (x.live) r = find_parts<MT, KU>(p, x, t, head);
-    if (x.scan) pdl_wait();
+    __shared__ Parts s_parts;
+    __shared__ bool s_live;
+    const bool early = a.n_seq <= 256;
+    if (!early) pdl_wait();
+    if (warp == 0) {
+        const RowInfo x = early ? row_info<MT, KU, true>(a, t) : row_info<MT, KU, false>(a, t);
+        Parts y{0, 0, 0, 0, 0, 0};
+        if (x.live) y = find_parts<MT, KU>(p, x, t, head);
+        if (lane == 0) { s_parts = y; s_live = x.live; }
+    }
+    __syncthreads();
+    const Parts r = s_parts;
+    if (early) pdl_wait();
     pdl_release();
-    if (!x.live) return;
+    if (!s_live) return;
     const int n = r.n0 + r.n1;
     float M = -INFINITY, L = 0.0f, acc[DPL];
 #pragma unroll

@@ -13,9 +13,8 @@
 // TMEM (512 columns): S_0, S_1 of 128 each, O_0, O_1 of head_dim each. While one tile's
 // probabilities are taken the tensor core works on the other's products.
 //
-// The maximum is kept behind by up to 2^8 before O is rescaled: sums and O are f32 and P
-// stays below 2^8, so nothing overflows or loses bits, and the rescale (O through registers)
-// becomes rare. l sums the unrounded probabilities.
+// O is rescaled (through registers) only when a row's maximum has run ahead of the one in use
+// (LAG). l sums the unrounded probabilities.
 //
 // Bound: per unit the products of both tiles take 2048 cycles at head_dim 128, and the
 // 2 x 128^2 exponentials the same at 16 per cycle and SM; under the load the SMs run at about
@@ -353,8 +352,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) prefix_tc_kernel(const __grid_c
                 const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sc;
                 const bool raise = top > m + LAG;
                 if (__any_sync(0xffffffffu, raise)) {
-                    const float f = raise ? ex2(m - top) : 1.0f;
-                    if (raise) m = top;
+                    const float f = raise ? ex2(m - (top - P_SHIFT)) : 1.0f;
+                    if (raise) m = top - P_SHIFT;
                     l *= f;
                     if (i > 0) {                                 // these scores were issued after the last O was done
 #pragma unroll

@@ -17,7 +17,11 @@ constexpr int MIN_UNITS = 2;           // line positions per worker at least, be
 // besides its units (queries, the partial result), so that ranges of short segments are not
 // the longest ones.
 constexpr int SEG_COST = 1, TC_SEG_COST = 3;
-constexpr float LAG = 8.0f;            // log2 by which a row's maximum may run ahead of the one in use
+// The reference m of a row's probabilities 2^(s - m) is its maximum less P_SHIFT, and stays until
+// the maximum is LAG above it: probabilities lie below 2^15, within f16, sums and O are f32, so
+// nothing overflows, rescaling O becomes rare, and the shift keeps small probabilities of f16
+// caches off the bottom of its range (2^-31 of the largest is still there).
+constexpr float P_SHIFT = 7.0f, LAG = 15.0f;
 
 struct AttnP {
     const void* q;
@@ -42,9 +46,9 @@ __device__ __forceinline__ int cdiv(int a, int b) { return (a + b - 1) / b; }
 
 // One stream's extent, with offsets and lengths that are out of range cut to nothing.
 struct SeqInfo { int lo, n, len, nt, qt; bool bad; };
-template <int MT, int KU> __device__ __forceinline__ SeqInfo seq_info(const AttnP& p, int b) {
+template <int MT, int KU> __device__ __forceinline__ SeqInfo seq_info(const AttnP& p, int b, bool l2) {
     SeqInfo s;
-    const int lo = p.row_off[b], hi = p.row_off[b + 1], len = p.seq_len[b];
+    const int lo = ld_word(p.row_off + b, l2), hi = ld_word(p.row_off + b + 1, l2), len = ld_word(p.seq_len + b, l2);
     const long long cap = (long long)p.max_pages * p.page_len;
     s.bad = lo < 0 || hi < lo || hi > p.n_rows || len < 0 || len > cap;
     s.lo = lo;

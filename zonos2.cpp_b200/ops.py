@@ -69,7 +69,14 @@ def _packer(cls):
     """struct packer of an argument structure: a quarter of the time its constructor takes, which
     is a good part of a small call."""
     code = {_I: "i", _L: "q", _P: "P", _F: "f", _Z: "N"}
-    return struct.Struct("@" + "".join(code[f] for _, f in cls._fields_)).pack
+    pack = struct.Struct("@" + "".join(code[f] for _, f in cls._fields_)).pack
+
+    def packed(*values):
+        try:
+            return pack(*values)
+        except struct.error as e:
+            _refuse(f"a number is out of range or not one: {e}")
+    return packed
 
 
 _pack_append, _pack_attn, _pack_verify = _packer(RopeAppendArgs), _packer(PrefixAttnArgs), _packer(VerifyArgs)
@@ -146,7 +153,12 @@ class PagedKV:
             _refuse("kv: the dims of a head must be contiguous, and no size zero")
         self.k, self.v, self.device, self.dtype = k, v, k.device, k.dtype
         self.n_pages, self.page_len, self.n_head_kv, self.head_dim = k.shape
-        self.view = PagedKVView(k.data_ptr(), v.data_ptr(), _TYPE[k.dtype], *k.shape, *k.stride()[:3])
+        # a stride along a dimension of one says nothing: it reads as if packed
+        sp, sr, sh, _ = k.stride()
+        sh = sh if self.n_head_kv > 1 else self.head_dim
+        sr = sr if self.page_len > 1 else sh * self.n_head_kv
+        sp = sp if self.n_pages > 1 else self.page_len * self.n_head_kv * self.head_dim
+        self.view = PagedKVView(k.data_ptr(), v.data_ptr(), _TYPE[k.dtype], *k.shape, sp, sr, sh)
         self._idx, self._at, self._scale = k.get_device(), ctypes.addressof(self.view), 1.0 / math.sqrt(self.head_dim)
         self._bytes = {}                # workspace bytes by sizes
 
@@ -193,7 +205,10 @@ def rope_append(rope: Rope | None, kv: PagedKV, q, k, v, row_off, seq_len, page_
         qr, qh, qp = _rows(q, n, nh, kv, dt, "q")
         if out is None:
             out = _empty_like(q)
-        outr, outh, outp = _rows(out, n, nh, kv, dt, "out")
+            outr, outh, _ = out.stride()
+            outp = out.data_ptr()
+        else:
+            outr, outh, outp = _rows(out, n, nh, kv, dt, "out")
     elif out is not None:
         _refuse("rope_append: out without q")
     if k is not None:
@@ -224,7 +239,10 @@ def prefix_attention(kv: PagedKV, q, row_off, seq_len, page_table, prefix_pages=
     qr, qh, qp = _rows(q, n, nh, kv, kv.dtype, "q")
     if out is None:
         out = _empty_like(q)
-    outr, outh, outp = _rows(out, n, nh, kv, kv.dtype, "out")
+        outr, outh, _ = out.stride()
+        outp = out.data_ptr()
+    else:
+        outr, outh, outp = _rows(out, n, nh, kv, kv.dtype, "out")
     if lse is True:
         lse = q.new_empty((n, nh), dtype=_F32)
     elif lse is False:
