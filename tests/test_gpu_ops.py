@@ -487,6 +487,15 @@ def test_python_refusals():
     for f in bad:
         with pytest.raises(R.Z2BError):
             f()
+    grad = q.clone().requires_grad_()                        # no operator has a backward pass
+    for f in (lambda: ops.prefix_attention(s.kv, grad, *meta), lambda: ops.rope_append(None, s.kv, grad, None, None, *meta),
+              lambda: ops.verify_drafts(torch.ones((1, 1, 1, 4), device=DEV, requires_grad=True), None, s.d_lens.new_zeros((1, 0, 1)),
+                                        torch.zeros((1, 0, 1), dtype=torch.float64, device=DEV),
+                                        torch.zeros((1, 1, 1), dtype=torch.float64, device=DEV))):
+        with pytest.raises(R.Z2BError):
+            f()
+        with torch.no_grad():
+            f()
     none = ops.prefix_attention(s.kv, q[:0], _i32([0, 0]), s.d_lens, s.d_table)
     assert none.shape == (0, 4, 64)
 

@@ -13,13 +13,14 @@ torch = pytest.importorskip("torch")
 
 import z2b.ops as ops
 import z2b.runtime as R
+from tests import ops_args as args
 
 ARG, UNSUPPORTED = 1, 7
 BUF = 1 << 20                       # an address that is aligned and never read
 
 
 def _call(fn, a):
-    L = ops._lib()
+    L = args.library()
     return getattr(L, fn)(ctypes.addressof(a), None), L.z2b_last_error().decode()
 
 
@@ -36,7 +37,7 @@ def _append(view=None, rope=None, **kw):
              v=BUF, row_off=BUF, seq_len=BUF, page_table=BUF, table_stride=2, max_pages=2,
              rope=None if rope is None else ctypes.addressof(rope))
     d.update(kw)
-    a = ops.RopeAppendArgs(**d)
+    a = args.RopeAppendArgs(**d)
     a._keep = (v, rope)
     return a
 
@@ -47,7 +48,7 @@ def _attn(view=None, **kw):
              q_row=256, q_head=64, o_row=256, o_head=64, row_off=BUF, seq_len=BUF, page_table=BUF, table_stride=2, max_pages=2,
              prefix_pages=BUF, workspace=BUF, workspace_bytes=1 << 40)
     d.update(kw)
-    a = ops.PrefixAttnArgs(**d)
+    a = args.PrefixAttnArgs(**d)
     a._keep = v
     return a
 
@@ -56,7 +57,7 @@ def _verify(**kw):
     d = dict(device=0, type=0, n_seq=2, max_draft=3, n_codebooks=2, vocab=100, p=BUF, q=BUF, draft=BUF, u_accept=BUF,
              u_draw=BUF, tokens=BUF, n_accepted=BUF)
     d.update(kw)
-    return ops.VerifyArgs(**d)
+    return args.VerifyArgs(**d)
 
 
 BAD_VIEWS = [dict(k=None), dict(v=None), dict(type=0), dict(type=5), dict(n_pages=0), dict(page_len=0), dict(n_head_kv=0),
@@ -120,7 +121,7 @@ def test_nothing_to_do_is_not_an_error():
 
 
 def test_null_arguments():
-    L = ops._lib()
+    L = args.library()
     for fn in ("z2b_rope_append", "z2b_prefix_attention", "z2b_verify_drafts"):
         assert getattr(L, fn)(None, None) == ARG
     assert L.z2b_prefix_attention_workspace(None) == 0
@@ -129,7 +130,7 @@ def test_null_arguments():
 
 
 def test_workspace_grows_with_the_call():
-    L = ops._lib()
+    L = args.library()
 
     def size(**kw):
         a = _attn(**kw)
@@ -174,10 +175,3 @@ def test_rope_table_against_decimals(kw):
             assert abs(decimal.Decimal(int(t.step[i])) - want) <= want * decimal.Decimal(16 * 2.0 ** -53) + 1
     assert t.mag == pytest.approx(0.1 * math.log(16.0) + 1.0 if kw.get("scaling") == "by_parts" else 1.0, rel=2.0 ** -23)
 
-
-def test_packed_arguments_match_the_structures():
-    """The binding packs argument structures by format strings; they are the C layout byte for byte."""
-    for cls, pack in ((ops.RopeAppendArgs, ops._pack_append), (ops.PrefixAttnArgs, ops._pack_attn), (ops.VerifyArgs, ops._pack_verify)):
-        values = [0.5 if f is ctypes.c_float else 3 + 7 * i for i, (_, f) in enumerate(cls._fields_)]
-        packed = pack(*values)
-        assert bytes(cls(*values))[: len(packed)] == packed and ctypes.sizeof(cls) - len(packed) < 8

@@ -4,15 +4,19 @@ libz2b.so        the decode-step library: GGUF loader, tile repack, sm_100a kern
                  batch runtime and the C ABI declared in include/z2b.h; the DAC decoder
                  (include/z2b_dac.h).
 libz2b_synth.so  host-only synthetic GGUF writer (include/z2b_tools.h).
+_ops.so          the Python binding of include/z2b_ops.h for torch tensors (module z2b._ops, used
+                 by z2b.ops); the one part compiled against torch, left out where there is none.
 
 Objects go to zonos2.cpp_b200/_build/ and are rebuilt when a source or header is newer.
 """
 from __future__ import annotations
 
 import concurrent.futures as cf
+import importlib.util
 import os
 import subprocess
 import sys
+import sysconfig
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG)
@@ -24,6 +28,7 @@ ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 LIB = os.path.join(PKG, "libz2b.so")
 SYNTH_LIB = os.path.join(PKG, "libz2b_synth.so")
+OPS_LIB = os.path.join(PKG, "_ops.so")
 
 HOST_COMMON = ["gguf.cpp", "quant.cpp"]
 Z2B_HOST = ["repack.cpp", "model.cpp", "runtime.cpp", "capi.cpp", "dac.cpp", "capi_dac.cpp", "prompt.cpp",
@@ -98,13 +103,29 @@ def build_z2b(verbose=False):
     return LIB
 
 
+def build_ops():
+    spec = importlib.util.find_spec("torch")
+    if spec is None:
+        return None
+    src = os.path.join(CSRC, "py_ops.cpp")
+    if _stale(OPS_LIB, [src, os.path.join(INCLUDE, "z2b_ops.h")]):
+        torch = spec.submodule_search_locations[0]
+        libs = os.path.join(torch, "lib")
+        _run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-I" + os.path.join(torch, "include"),
+              "-I" + os.path.join(torch, "include", "torch", "csrc", "api", "include"), "-I/usr/local/cuda/include",
+              "-I" + sysconfig.get_paths()["include"], src, "-o", OPS_LIB, "-L" + libs, "-ltorch_python", "-ltorch",
+              "-ltorch_cpu", "-lc10", "-lc10_cuda", "-ltorch_cuda", "-L" + PKG, "-lz2b", "-Wl,-rpath,$ORIGIN"])
+    return OPS_LIB
+
+
 def build_all(verbose=False):
     build_synth()
     build_z2b(verbose)
+    build_ops()
 
 
 if __name__ == "__main__":
     which = sys.argv[1] if len(sys.argv) > 1 else "all"
     v = "-v" in sys.argv
-    {"synth": build_synth, "z2b": lambda: build_z2b(v), "all": lambda: build_all(v)}[which]()
+    {"synth": build_synth, "z2b": lambda: build_z2b(v), "ops": build_ops, "all": lambda: build_all(v)}[which]()
     print("ok")
