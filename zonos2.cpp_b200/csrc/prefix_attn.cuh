@@ -60,19 +60,22 @@ template <int MT, int KU> __device__ __forceinline__ SeqInfo seq_info(const Attn
 }
 
 // A line of W positions cut into equal ranges: worker i's begins at floor(W i / workers). W is
-// below 2^31 and i * workers below 2^31, so 32-bit arithmetic is exact: W i / workers =
-// i (W / workers) + i (W % workers) / workers.
+// below 2^31 and workers at most 2^11, so 32-bit arithmetic is exact: W i / workers =
+// i (W / workers) + i (W % workers) / workers, and the last quotient, of a number x with
+// x workers < 2^32, is the high word of x ceil(2^32 / workers).
 struct Cut {
     int workers, each, rest;
+    uint32_t inv;
     __device__ __forceinline__ Cut(int W, int most) {
         workers = max(1, min(most, W / MIN_UNITS));
-        each = W / workers;
+        each = (int)((unsigned)W / (unsigned)workers);
         rest = W - each * workers;
+        inv = workers > 1 ? 0xffffffffu / (unsigned)workers + 1u : 0u;
     }
-    __device__ __forceinline__ int begin(int i) const { return i * each + (int)((unsigned)(i * rest) / (unsigned)workers); }
+    __device__ __forceinline__ int begin(int i) const { return i * each + (int)__umulhi((unsigned)(i * rest), inv); }
     // The worker that holds position u: an f32 guess, off by one at most, put right exactly.
     __device__ __forceinline__ int owner(int u, int W) const {
-        int i = min(workers - 1, (int)((float)u * (float)workers / (float)W));
+        int i = min(workers - 1, (int)__fdividef((float)u * (float)workers, (float)W));
         while (begin(i) > u) --i;
         while (begin(i + 1) <= u) ++i;
         return i;
