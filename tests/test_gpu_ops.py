@@ -214,7 +214,7 @@ ATTNS = [
     ([1], [5000], 64, 2, 1, 128, F16, 0, False, 0),                      # one long stream over many CTAs
     ([20] * 4, [20, 33, 90, 64], 16, 2, 1, 128, BF16, 500, False, 0),
     ([9, 17], [64, 128], 40, 12, 2, 16, F16, 0, False, 0),
-    # prefixes of many rows (256-row tiles): borders of tiles and units, tiles half empty, wide groups
+    # prefixes of many rows
     ([1] * 20, [2] * 20, 256, 16, 4, 128, F16, 128, False, 0),           # 80 rows a key head, one unit
     ([1] * 33, [1] * 33, 64, 16, 2, 64, BF16, 129, False, 5),            # 264 rows: eight in the second tile
     ([5] * 13, [70] * 13, 16, 6, 2, 64, F16, 257, True, 0),              # 195 rows, pages of 16
@@ -503,10 +503,10 @@ def test_python_refusals():
 @pytest.mark.parametrize("scale", [0.0, -0.2, 1.0], ids=str)
 def test_prefix_attention_scales(scale):
     """A scale of zero (all keys alike) and a negative one, few rows and many."""
-    for B in (2, 30):
-        s = Streams([1] * B, [3] * B, 16, 2, 64, F16, prefix=140, seed=14)
+    for B, P in ((2, 140), (30, 8800)):
+        s = Streams([1] * B, [3] * B, 16, 2, 64, F16, prefix=P, seed=14)
         q = torch.randn((B, 8, 64), generator=_gen(15)).to(F16).to(DEV)
-        out, lse = ops.prefix_attention(s.kv, q, s.d_off, s.d_lens, s.d_table, s.d_shared, 140, scale=scale, lse=True, err=s.err)
+        out, lse = ops.prefix_attention(s.kv, q, s.d_off, s.d_lens, s.d_table, s.d_shared, P, scale=scale, lse=True, err=s.err)
         ops.check(s.err)
         _check_attention(s, q, out, lse, scale=scale)
 
@@ -522,12 +522,11 @@ def test_prefix_attention_many_streams():
 
 
 @pytest.mark.parametrize("dtype", [F16, BF16], ids=str)
-@pytest.mark.parametrize("B", [2, 40], ids=str)
-def test_prefix_attention_small_probabilities(dtype, B):
-    """One key takes nearly all, 4000 others 2^-27 of it each: their share is not lost below f16's
+@pytest.mark.parametrize("B,P", [(2, 4001), (40, 14001)], ids=str)
+def test_prefix_attention_small_probabilities(dtype, B, P):
+    """One key takes nearly all, thousands of others 2^-27 of it each: their share is not lost below f16's
     range. The probabilities are held times 2^7, so one of 2^-27 is a multiple of 2^-24 off by 2^-25
     at most: 2^-5 of it; the result (3e-5) by another half step of its type."""
-    P = 4001
     s = Streams([1] * B, [1] * B, 16, 1, 64, dtype, prefix=P, seed=18)
     for c in (s.kv.k, s.kv.v):
         c.zero_()
@@ -568,12 +567,59 @@ def test_cache_of_one_head_or_page_in_any_order():
 
 def test_prefix_attention_unaligned_queries_and_in_place():
     """q at an odd pair of elements (no 16-byte rows), few rows and many; out may be q itself."""
-    for B in (3, 40):
-        s = Streams([1] * B, [5] * B, 16, 2, 64, BF16, prefix=150, seed=20)
+    for B, P in ((3, 150), (40, 6600)):
+        s = Streams([1] * B, [5] * B, 16, 2, 64, BF16, prefix=P, seed=20)
         buf = torch.randn((B, 2 + 8 * 64), generator=_gen(21)).to(BF16).to(DEV)
         q = buf[:, 2:].unflatten(1, (8, 64))
         kept = q.clone()
         lse = torch.zeros((B, 8), device=DEV)
-        assert ops.prefix_attention(s.kv, q, s.d_off, s.d_lens, s.d_table, s.d_shared, 150, out=q, lse=lse, err=s.err)[0] is q
+        assert ops.prefix_attention(s.kv, q, s.d_off, s.d_lens, s.d_table, s.d_shared, P, out=q, lse=lse, err=s.err)[0] is q
         ops.check(s.err)
         _check_attention(s, kept, q, lse)
+
+
+@pytest.mark.parametrize("counts,page,nh,nkv,hd,dtype,prefix,pad", [
+    ([1] * 8, 64, 16, 4, 128, F16, 16400, 0),                # 32 rows a key head: one tile half full
+    ([1] * 40, 256, 16, 4, 64, BF16, 3300, 3),               # 160 rows: two tiles, the second a quarter full
+    ([5] * 13, 16, 6, 2, 64, F16, 13500, 0),                 # 195 rows, pages of 16, the last unit of 60 keys
+    ([1] * 100, 8, 6, 1, 128, BF16, 3501, 0),                # 600 rows: three segments of the one head, pages of 8
+    ([3, 0, 90], 48, 4, 1, 128, F16, 5700, 9),               # a prompt chunk over the prefix
+    ([1] * 65, 32, 2, 1, 64, BF16, 16200, 0),                # 130 rows: two of them in the second tile
+    ([1] * 700, 16, 32, 8, 64, F16, 100, 0),                 # 2800 rows over less than one unit
+], ids=str)
+def test_prefix_attention_long_prefix(counts, page, nh, nkv, hd, dtype, prefix, pad):
+    """Prefixes long enough for the 256-row tiles of the tensor cores, at tile and unit borders."""
+    s = Streams(counts, [n + i % 5 for i, n in enumerate(counts)], page, nkv, hd, dtype, prefix=1, pad=pad, seed=23)
+    s.prefix, need = prefix, -(-prefix // page)              # one page after another, drawn at once
+    k, v = (torch.randn((need + s.kv.n_pages, page, nkv, hd), generator=_gen(24 + i)).to(dtype).to(DEV) for i in range(2))
+    for new, old in ((k, s.kv.k), (v, s.kv.v)):
+        new[need:] = old
+        tail = need * page - prefix
+        if tail:
+            new[need - 1, page - tail:] = math.nan
+    s.kv = ops.PagedKV(k, v)
+    s.table, s.shared = s.table + need, torch.arange(need, dtype=torch.int32)
+    s.d_table, s.d_shared = s.table.to(DEV), s.shared.to(DEV)
+    q = (torch.randn((s.rows, nh, hd), generator=_gen(26)) * 1.5).to(dtype).to(DEV)
+    out, lse = torch.full_like(q, 5.0), torch.full((s.rows, nh), 5.0, device=DEV)
+    ops.prefix_attention(s.kv, q, s.d_off, s.d_lens, s.d_table, s.d_shared, prefix, out=out, lse=lse, err=s.err)
+    ops.check(s.err)
+    pick = [0, s.total // 2, s.total - 1]                    # rows checked against 64 bits
+    b_of = [next(b for b in range(len(counts)) if s.off[b + 1] > t) for t in pick]
+    for t, b in zip(pick, b_of):
+        one = Streams([1], [1], page, nkv, hd, dtype)
+        one.kc, one.prefix, one.kv = s.kc, prefix, s.kv
+        sees = s.lens[b] - counts[b] + (t - s.off[b]) + 1
+        one.off, one.lens, one.total = [0, 1], [sees], 1
+        one.table, one.shared = s.table[b:b + 1], s.shared
+        _check_attention(one, q[t:t + 1], out[t:t + 1], lse[t:t + 1])
+    # the other rows: the same rows as calls of three (whose prefix the warp-level kernel takes) agree
+    for t, b in ((s.total // 3, None), (s.total - 2, None)):
+        b = next(b for b in range(len(counts)) if s.off[b + 1] > t)
+        sees = s.lens[b] - counts[b] + (t - s.off[b]) + 1
+        want, wl = ops.prefix_attention(s.kv, q[t:t + 1], _i32([0, 1]), _i32([sees]), s.d_table[b:b + 1], s.d_shared, prefix, lse=True)
+        spread = 4 * torch.finfo(dtype).eps * want.double().abs().amax() + 2e-3      # two roundings of P and of the result each
+        assert (out[t].double() - want[0].double()).abs().max() <= spread and (lse[t] - wl[0]).abs().max() <= 1e-3
+    assert (out[s.total:] == 5.0).all() and (lse[s.total:] == 5.0).all()
+    again = ops.prefix_attention(s.kv, q, s.d_off, s.d_lens, s.d_table, s.d_shared, prefix)
+    assert torch.equal(out[: s.total], again[: s.total])
