@@ -770,8 +770,10 @@ HostPlan host_plan(const z2b_prefix_attn_args& a) {
     HostPlan h{};
     const int nkv = a.kv->n_head_kv, hd = a.kv->head_dim;
     h.G = a.n_head / nkv;
-    // rows of one stream and key head, on average: the smallest tile that holds them. head_dim 128
-    // keeps 16 (32 rows do not fit the registers); a second row tile then finds its keys in L2
+    // rows of one stream and key head, on average: the smallest tile that holds them (32 streams of up
+    // to 3000 keys, 16 rows each, tiles of 8 / 16: 30 / 27 us at head_dim 64, 40 / 37 at 128; 32 rows,
+    // tiles of 8 / 32 at 64: 34 / 29, of 8 / 16 at 128: 51 / 38). head_dim 128 keeps 16: 32 rows do not
+    // fit the registers, a second row tile finds its keys in L2
     const long long rows = (long long)((a.n_rows + a.n_seq - 1) / a.n_seq) * h.G;
     h.nb = rows <= 8 ? 1 : rows <= 16 || hd > 64 ? 2 : 4;
     h.warps = max_warps(hd);                                     // fewer where the line's streams need the room
@@ -822,9 +824,11 @@ cudaError_t go_attn(const AttnP& p, const CUtensorMap& km, const CUtensorMap& vm
 
 template <typename T, int HD, int MT>
 cudaError_t go_join(const JoinP& j, const z2b_prefix_attn_args& a, cudaStream_t s) {
-    // a block per row and head while those are fewer than two blocks an SM hold in warps
+    // a block per row and head, or a warp per four heads of a row: streams of 16 heads with up to 200
+    // own keys, block / warp, in us: 32 items 8.9 / 11.4, 512: 11 / 13.3, 1024: 16.7 / 16.0, 2048: 28 / 19;
+    // with up to 4000: 512: 30 / 36, 1024: 55 / 55, 2048: 101 / 93
     const long long items = (long long)a.n_rows * a.n_head;
-    if (items <= 148 * 16) return launch_pdl(prefix_attn_join_few_kernel<T, HD, MT>, dim3((unsigned)items), dim3(256), 0, s, j);
+    if (items <= 148 * 6) return launch_pdl(prefix_attn_join_few_kernel<T, HD, MT>, dim3((unsigned)items), dim3(256), 0, s, j);
     const long long warps = (long long)a.n_rows * ((a.n_head + 3) / 4);
     return launch_pdl(prefix_attn_join_kernel<T, HD, MT>, dim3((unsigned)((warps + 3) / 4)), dim3(128), 0, s, j);
 }

@@ -210,9 +210,11 @@ cudaError_t launch_rope_append(const z2b_rope_append_args& a, cudaStream_t s) {
     const int side = units >= 32 ? 1 : 32 / units;
     const int heads = p.nh + (p.k ? 2 * p.nkv : 0);
     const int iters = (heads + side - 1) / side;
-    // a row's heads over `split` warps while that still finds idle schedulers (148 SMs x 8 warps)
+    // a row's heads over `split` warps while that finds idle schedulers (four warps an SM). Rows of
+    // 32 + 2 x 8 heads of 128 dims, one warp each / split, in us: 1: 5.6 / 3.1, 64: 6.1 / 3.9, 256: 6.2 /
+    // 4.6; up to eight warps an SM instead, 1024 rows: 7.4 / 8.4
     int split = 1;
-    while (split < iters && (long long)p.n_rows * split < 148 * 8) ++split;
+    while (split < iters && (long long)p.n_rows * split < 148 * 4) ++split;
     const dim3 grid((p.n_rows + WARPS - 1) / WARPS, split);
     if (a.type == Z2B_TYPE_F32)
         return c.type == Z2B_TYPE_F16 ? go<float, __half>(p, vec, grid, s) : go<float, __nv_bfloat16>(p, vec, grid, s);

@@ -10,7 +10,8 @@
 // drawn token: the kept tokens cost one gathered value each, and no other row is read. One
 // CTA, or a cluster of them for large vocabularies, takes one (stream, codebook): every CTA
 // finds the run's end for itself (a handful of gathers). Then
-//   small rows: a thread holds up to EACH consecutive entries; one block scan finds the draw;
+//   small rows: a thread holds up to EACH consecutive entries; one block scan finds the draw (1026
+//   entries: 3.1 us, where a first pass for the sum and a second for the draw took 4.6);
 //   large rows: the row is split over the cluster, each warp summing one contiguous share with
 //   lanes side by side; the totals are exchanged through distributed shared memory, and the one
 //   CTA whose range holds the target scans the one warp's share that does.
@@ -305,8 +306,10 @@ template <typename T> cudaError_t go_type(VerifyP P, cudaStream_t s) {
     const long long items = (long long)a.n_seq * a.n_codebooks;
     if (a.vocab <= 32 * SMALL_WARPS * EACH) return go<T, SMALL_WARPS>(P, a.q != nullptr, dim3((unsigned)items), s);
     // CTAs per row: enough that one CTA's share is a few thousand entries, while all clusters
-    // are resident together (four of these CTAs an SM, 148 SMs)
-    while (P.cluster < MAX_CLUSTER && a.vocab / P.cluster > 4096 && items * P.cluster * 2 <= 592) P.cluster *= 2;
+    // are resident together (two CTAs an SM, 148 SMs). One CTA / a cluster by this rule, in us:
+    // 1 stream, vocabulary 10007: 6.6 / 5.4, 50021: 14.7 / 6.4, 200003: 42 / 9.2; 32 streams, 10007:
+    // 6.6 / 5.7, 50021: 15 / 8.4; 128 streams, 50021: 26 / 17.5, 10007: 6.8 / 7.5 (four each: 12)
+    while (P.cluster < MAX_CLUSTER && a.vocab / P.cluster > 4096 && items * P.cluster * 2 <= 296) P.cluster *= 2;
     return go<T, LARGE_WARPS>(P, a.q != nullptr, dim3((unsigned)(items * P.cluster)), s);
 }
 
