@@ -19,7 +19,8 @@
  * be captured into a CUDA graph. The calling thread's current device is left as it was.
  * Strides count elements. `err`, when not NULL, is a uint32 word on the device that the
  * kernels OR their findings into, never clearing it: Z2B_OPS_BAD_INDEX for offsets, lengths
- * or token ids out of range (the row is skipped, the token refused), Z2B_OPS_BAD_PAGE for a
+ * or token ids out of range (the row is skipped, the token refused; offsets that descend:
+ * z2b_prefix_attention skips every row), Z2B_OPS_BAD_PAGE for a
  * page id outside the cache (its keys read as zeros, its rows are not stored),
  * Z2B_OPS_TIMEOUT for a bounded wait that ran out. No input is dereferenced before it is
  * checked, with or without `err`.

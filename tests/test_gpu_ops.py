@@ -623,3 +623,24 @@ def test_prefix_attention_long_prefix(counts, page, nh, nkv, hd, dtype, prefix, 
     assert (out[s.total:] == 5.0).all() and (lse[s.total:] == 5.0).all()
     again = ops.prefix_attention(s.kv, q, s.d_off, s.d_lens, s.d_table, s.d_shared, prefix)
     assert torch.equal(out[: s.total], again[: s.total])
+
+
+@pytest.mark.parametrize("B,pages", [(4, 2), (300, 2), (512, 4096)], ids=str)
+def test_prefix_attention_descending_offsets(B, pages):
+    """Offsets that rise and drop by turns name every row many times over (the largest case: more units
+    of work than 32 bits count). Recorded, and no row is written, few streams and many."""
+    rows = 4096 if pages > 2 else 24
+    kv = ops.PagedKV(*(torch.zeros((3, 64, 8, 16), dtype=F16, device=DEV) for _ in range(2)))
+    q = torch.zeros((rows, 64 if pages > 2 else 8, 16), dtype=F16, device=DEV)
+    err = torch.zeros(1, dtype=torch.int32, device=DEV)
+    off = _i32([0, rows] * (B // 2) + [0])
+    lens, table = _i32([pages * 64] * B), torch.zeros((B, pages), dtype=torch.int32, device=DEV)
+    for last in (0, rows):
+        off[-1] = last
+        for prefix in (0, 100):
+            err.zero_()
+            out = torch.full_like(q, 5.0)
+            lse = torch.full(q.shape[:2], 6.0, device=DEV)
+            ops.prefix_attention(kv, q, off, lens, table, _i32([1, 2]), prefix, out=out, lse=lse, err=err)
+            assert int(err) == ops.BAD_INDEX
+            assert (out == 5.0).all() and (lse == 6.0).all()

@@ -136,24 +136,26 @@ __global__ void __launch_bounds__(32 * max_warps(HD), 1) prefix_attn_kernel(cons
     {
         const int per = cdiv(p.n_seq, blockDim.x);
         const int b0 = min(p.n_seq, (int)threadIdx.x * per), b1 = min(p.n_seq, b0 + per);
-        int su = 0, sg = 0;
+        unsigned su = 0, sg = 0;
+        int drops = 0;
         for (int b = b0; b < b1; ++b) {
             const SeqInfo s = seq_info<MT, KU>(p, b, p.after_prefix);
+            drops |= s.drops;
             if (s.bad && blockIdx.x == 0 && p.err) atomicOr(p.err, Z2B_OPS_BAD_INDEX);
             s_rec[b] = make_int4(su, sg, s.lo, s.n);
             s_len[b] = s.len;
             su += s.nt ? s.qt * p.nkv * (s.nt + SEG_COST) : 0;
             sg += s.qt * p.nkv;
         }
-        int iu = su, ig = sg;
+        unsigned iu = su, ig = sg;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const int a = __shfl_up_sync(0xffffffffu, iu, o), c = __shfl_up_sync(0xffffffffu, ig, o);
+            const unsigned a = __shfl_up_sync(0xffffffffu, iu, o), c = __shfl_up_sync(0xffffffffu, ig, o);
             if (lane >= o) { iu += a; ig += c; }
         }
         if (lane == 31) { s_scan[0][warp] = iu; s_scan[1][warp] = ig; }
-        __syncthreads();
-        int eu = iu - su, eg = ig - sg;
+        drops = __syncthreads_or(drops);
+        unsigned eu = iu - su, eg = ig - sg;
         for (int w = 0; w < warp; ++w) { eu += s_scan[0][w]; eg += s_scan[1][w]; }
         for (int b = b0; b < b1; ++b) {
             s_rec[b].x += eu;
@@ -161,8 +163,8 @@ __global__ void __launch_bounds__(32 * max_warps(HD), 1) prefix_attn_kernel(cons
             if (blockIdx.x == 0) { p.plan[b] = s_rec[b].x; p.plan[p.n_seq + 1 + b] = s_rec[b].y; }
         }
         if (threadIdx.x == blockDim.x - 1) {
-            s_rec[p.n_seq] = make_int4(eu + su, eg + sg, 0, 0);
-            if (blockIdx.x == 0) { p.plan[p.n_seq] = eu + su; p.plan[2 * p.n_seq + 1] = eg + sg; }
+            s_rec[p.n_seq] = make_int4(drops ? 0 : eu + su, 0, 0, 0);
+            if (blockIdx.x == 0) p.plan[p.n_seq] = drops ? -1 : (int)(eu + su);
         }
     }
     Line ln;
@@ -434,9 +436,7 @@ __global__ void __launch_bounds__(32 * max_warps(HD), 1) prefix_attn_kernel(cons
 
         // ---- the segment's (or the range's) end: one partial result
         const int slot = g.seg + me;
-        const bool fits = slot < p.max_slots;                    // false only for offsets that do not ascend
-        if (!fits && p.err && lane == 0) atomicOr(p.err, Z2B_OPS_BAD_INDEX);
-        const int rows = fits ? min(MT, g.n * p.G - g.j * MT) : 0;       // live rows of the tile
+        const int rows = min(MT, g.n * p.G - g.j * MT);          // live rows of the tile
         float* po = p.part_o + (size_t)slot * MT * HD;
         float2* pm = p.part_ml + (size_t)slot * MT;
 #pragma unroll
@@ -470,7 +470,7 @@ __global__ void __launch_bounds__(32 * max_warps(HD), 1) prefix_attn_kernel(cons
 struct PartSet {                        // partial results of one launch
     const float* o;
     const float2* ml;
-    int mt, keys, workers, max_slots, row_tiles;   // rows of a partial, keys of a unit, ..., row tiles of the prefix in it
+    int mt, keys, workers, slots, row_tiles;       // rows of a partial, keys of a unit, ..., row tiles of the prefix in it
 };
 struct JoinP {
     AttnP a;
@@ -489,7 +489,7 @@ struct Parts { int n0, n1, slot0, slot1, row0, row1; };
 // their own predecessors are done, so the call's inputs are there; they are read past L1), and the
 // offsets of its units and segments on the line: read from the plan after the wait, or (EARLY)
 // summed by the warp from the inputs, and the caller waits.
-struct RowInfo { SeqInfo s; int i, own_units, unit_b, seg_b; bool live; };
+struct RowInfo { SeqInfo s; int i; unsigned own_units, unit_b, seg_b; bool taken, live; };
 template <int MT, int KU, bool EARLY> __device__ __forceinline__ RowInfo row_info(const AttnP& a, int t) {
     const int lane = threadIdx.x & 31;
     RowInfo x;
@@ -498,9 +498,11 @@ template <int MT, int KU, bool EARLY> __device__ __forceinline__ RowInfo row_inf
     x.s = seq_info<MT, KU>(a, b, true);
     if constexpr (EARLY) {
         x.own_units = x.unit_b = x.seg_b = 0;
+        bool drops = false;
         for (int c = lane; c < a.n_seq; c += 32) {
             const SeqInfo y = seq_info<MT, KU>(a, c, true);
-            const int segs = y.qt * a.nkv, units = y.nt ? segs * (y.nt + SEG_COST) : 0;
+            drops |= y.drops;
+            const unsigned segs = y.qt * a.nkv, units = y.nt ? segs * (y.nt + SEG_COST) : 0u;
             x.own_units += units;
             if (c < b) { x.unit_b += units; x.seg_b += segs; }
         }
@@ -510,14 +512,16 @@ template <int MT, int KU, bool EARLY> __device__ __forceinline__ RowInfo row_inf
             x.unit_b += __shfl_xor_sync(0xffffffffu, x.unit_b, o);
             x.seg_b += __shfl_xor_sync(0xffffffffu, x.seg_b, o);
         }
+        x.taken = !__any_sync(0xffffffffu, drops);
     } else {
         pdl_wait();
         x.own_units = a.plan[a.n_seq];
+        x.taken = a.plan[a.n_seq] >= 0;
         x.unit_b = a.plan[b];
         x.seg_b = a.plan[a.n_seq + 1 + b];
     }
     x.i = t - x.s.lo;
-    x.live = t < total && !x.s.bad && x.i >= 0 && x.i < x.s.n;   // else padding, which stays as it is
+    x.live = x.taken && t < total && !x.s.bad && x.i >= 0 && x.i < x.s.n;   // else padding, which stays as it is
     return x;
 }
 
@@ -537,7 +541,6 @@ template <int MT, int KU> __device__ __forceinline__ Parts find_parts(const Join
         r.n0 = cp.owner(first + nt - 1, Wp) - c0 + 1;
         r.slot0 = seg + c0;
         r.row0 = row - j * p.pf.mt;
-        if (r.slot0 + r.n0 > p.pf.max_slots) r.n0 = 0;
     }
     if (x.s.nt > 0) {
         const int row = x.i * a.G + g, js = h * x.s.qt + row / MT;
@@ -546,7 +549,6 @@ template <int MT, int KU> __device__ __forceinline__ Parts find_parts(const Join
         r.n1 = cut.owner(first + x.s.nt - 1, positions) - c0 + 1;
         r.slot1 = a.pf_row_tiles * a.nkv + x.seg_b + js + c0;
         r.row1 = row % MT;
-        if (r.slot1 + r.n1 > p.own.max_slots) r.n1 = 0;          // only for offsets that do not ascend
     }
     return r;
 }
@@ -789,19 +791,19 @@ HostPlan host_plan(const z2b_prefix_attn_args& a) {
     const int pf_tiles = a.prefix_len > 0 && !h.pf_tc ? (int)((R + mt - 1) / mt) : 0;
     h.own = PartSet{nullptr, nullptr, mt, unit_keys(hd), 148 * h.warps, 0, pf_tiles};
     const long long segs = ((R + mt - 1) / mt + a.n_seq + pf_tiles) * nkv;
-    h.own.max_slots = (int)(segs + h.own.workers);
+    h.own.slots = (int)(segs + h.own.workers);
     h.pf = h.own;
     size_t n = up((size_t)2 * (a.n_seq + 1) * 4);
-    h.off_own_ml = n; n += up((size_t)h.own.max_slots * mt * 8);
-    h.off_own_o = n; n += up((size_t)h.own.max_slots * mt * hd * 4);
+    h.off_own_ml = n; n += up((size_t)h.own.slots * mt * 8);
+    h.off_own_o = n; n += up((size_t)h.own.slots * mt * hd * 4);
     if (h.pf_tc) {
         const int tiles = (int)((R + TC_ROWS - 1) / TC_ROWS);
         // a multiple of the row tiles, where that leaves few SMs idle: the row tiles are cut alike then,
         // so the CTAs that read the same keys do so at the same time and all but one find them in L2
         const int ctas = tiles <= 148 && 148 % tiles * 20 <= 148 ? 148 - 148 % tiles : 148;
         h.pf = PartSet{nullptr, nullptr, TC_ROWS, TC_KEYS, ctas, tiles * nkv + ctas, tiles};
-        h.off_pf_ml = n; n += up((size_t)h.pf.max_slots * TC_ROWS * 8);
-        h.off_pf_o = n; n += up((size_t)h.pf.max_slots * TC_ROWS * hd * 4);
+        h.off_pf_ml = n; n += up((size_t)h.pf.slots * TC_ROWS * 8);
+        h.off_pf_o = n; n += up((size_t)h.pf.slots * TC_ROWS * hd * 4);
     }
     h.bytes = n;
     return h;
@@ -852,7 +854,6 @@ cudaError_t go_all(const z2b_prefix_attn_args& a, HostPlan h, cudaStream_t s) {
             AttnP f = p;
             cut_boxes(f, TC_KEYS, HD);
             f.pf_row_tiles = h.pf.row_tiles;
-            f.max_slots = h.pf.max_slots;
             h.pf.ml = f.part_ml = (float2*)(ws + h.off_pf_ml);
             h.pf.o = f.part_o = (float*)(ws + h.off_pf_o);
             if (!make_page_map(&km, c.k, c, f) || !make_page_map(&vm, c.v, c, f)) return cudaErrorNotSupported;
@@ -864,7 +865,6 @@ cudaError_t go_all(const z2b_prefix_attn_args& a, HostPlan h, cudaStream_t s) {
         return cudaErrorNotSupported;
     p.pf_row_tiles = h.own.row_tiles;
     p.after_prefix = h.pf_tc;
-    p.max_slots = h.own.max_slots;
     h.own.ml = p.part_ml = (float2*)(ws + h.off_own_ml);
     h.own.o = p.part_o = (float*)(ws + h.off_own_o);
     e = h.nb == 1 ? go_attn<T, HD, 1>(p, km, vm, h.warps, s) : cudaSuccess;

@@ -398,19 +398,18 @@ __global__ void __launch_bounds__(TC_THREADS, 1) prefix_tc_kernel(const __grid_c
             if (!ok) break;
             tc_fence_after();
             const int slot = seg + (int)blockIdx.x;
-            const bool put = live && slot < p.max_slots;
             float* po = p.part_o + ((size_t)slot * TC_ROWS + t * 128 + row) * HD;
 #pragma unroll
             for (int k = 0; k < HD; k += 32) {
                 uint32_t o[32];
                 tmem_ld32(to + k, o);
                 tmem_wait_ld();
-                if (put)
+                if (live)
 #pragma unroll
                     for (int e = 0; e < 32; e += 4)
                         *(uint4*)(po + k + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
             }
-            if (put) p.part_ml[(size_t)slot * TC_ROWS + t * 128 + row] = make_float2(m, l);
+            if (live) p.part_ml[(size_t)slot * TC_ROWS + t * 128 + row] = make_float2(m, l);
             tc_fence_before();
         }
     }

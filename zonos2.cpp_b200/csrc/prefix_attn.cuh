@@ -34,22 +34,24 @@ struct AttnP {
                                        // unit's keys), and how many 64-dim halves it holds
     float scale2;                      // scale * log2(e)
     int pf_row_tiles;                  // row tiles of the prefix in this launch (0: none)
-    int max_slots;
     int after_prefix;                  // 1: the launch before is the prefix's, which this one runs beside
-    float* part_o;                     // [max_slots][rows of a segment][head_dim]
-    float2* part_ml;                   // [max_slots][rows of a segment] (m in log2 units, l)
+    float* part_o;                     // [slots][rows of a segment][head_dim]
+    float2* part_ml;                   // [slots][rows of a segment] (m in log2 units, l)
     int* plan;                         // [2][n_seq + 1] unit and segment offsets of the streams, written for the join
 };
 
 __device__ __forceinline__ int div_g(const AttnP& p, int x) { return p.G == 1 ? x : (int)__umulhi((uint32_t)x, p.g_mul); }
 __device__ __forceinline__ int cdiv(int a, int b) { return (a + b - 1) / b; }
 
-// One stream's extent, with offsets and lengths that are out of range cut to nothing.
-struct SeqInfo { int lo, n, len, nt, qt; bool bad; };
+// One stream's extent, with offsets and lengths that are out of range cut to nothing. Where no
+// stream's offsets drop, the streams' rows are disjoint, which bounds all sums over them; where one
+// does, no stream's rows are taken.
+struct SeqInfo { int lo, n, len, nt, qt; bool bad, drops; };
 template <int MT, int KU> __device__ __forceinline__ SeqInfo seq_info(const AttnP& p, int b, bool l2) {
     SeqInfo s;
     const int lo = ld_word(p.row_off + b, l2), hi = ld_word(p.row_off + b + 1, l2), len = ld_word(p.seq_len + b, l2);
     const long long cap = (long long)p.max_pages * p.page_len;
+    s.drops = hi < lo;
     s.bad = lo < 0 || hi < lo || hi > p.n_rows || len < 0 || len > cap;
     s.lo = lo;
     s.n = s.bad ? 0 : hi - lo;
