@@ -113,7 +113,8 @@ typedef struct z2b_rope_append_args {
 
 /* Rotate q into q_out and k into the cache, and store v, in one launch. Angles are exact to
  * f32 at any 32-bit position; the products are f32 and rounded once to their destination's
- * type. Rows of two streams that name the same cache row leave either one there. */
+ * type. Of rows that name the same cache row parts of any stay. With k NULL only q turns: the
+ * pages are not looked at, and max_pages may be 0. */
 int z2b_rope_append(const z2b_rope_append_args* args, void* stream);
 
 /* ---- attention over a shared prefix ---------------------------------------------------- */
@@ -121,7 +122,7 @@ typedef struct z2b_prefix_attn_args {
     int32_t device;
     int32_t n_rows, n_seq, n_head;     /* n_head a multiple of the cache's n_head_kv */
     int32_t prefix_len;                /* shared rows, >= 0 */
-    float scale;                       /* on q . k, usually 1 / sqrt(head_dim) */
+    float scale;                       /* on q . k, usually 1 / sqrt(head_dim); any sign, twice it finite */
     const z2b_paged_kv* kv;            /* host; head_dim 16, 32, 64 or 128; page_len a multiple of 8;
                                           k, v 16-byte aligned, strides multiples of 8 */
     const void* q;                     /* [n_rows][n_head][head_dim], the cache's type */
@@ -147,7 +148,8 @@ typedef struct z2b_prefix_attn_args {
  * behind seq_len and prefix_len may hold anything; those before must be finite. The result
  * does not depend on timing: the same call gives the same bits. */
 int z2b_prefix_attention(const z2b_prefix_attn_args* args, void* stream);
-/* Workspace bytes of a call with these sizes (pointers are not read); 0 for bad sizes. */
+/* Workspace bytes of a call with these sizes and this cache (no other pointer is looked at); 0 for
+ * bad ones. */
 size_t z2b_prefix_attention_workspace(const z2b_prefix_attn_args* args);
 
 /* ---- verification of drafts ------------------------------------------------------------ */
@@ -173,7 +175,8 @@ typedef struct z2b_verify_args {
  * each refused token of it is replaced by a draw from max(p - q, 0) (from p where that is
  * zero everywhere); when all drafts are kept, one frame more is drawn from p. Frames then
  * follow the target's distribution exactly. A draw takes the first token whose running sum
- * (64 bits) exceeds u_draw * total. Entries that are not numbers count as zero. */
+ * (64 bits) exceeds u_draw * total; a row of p without any mass gives -1. A p(x) or q(x) that is
+ * not a number refuses its token, a difference that is not a number counts as zero in a draw. */
 int z2b_verify_drafts(const z2b_verify_args* args, void* stream);
 
 #ifdef __cplusplus

@@ -2,6 +2,7 @@
 sizes, layouts and masks where they can go wrong, and their findings on bad metadata."""
 from __future__ import annotations
 
+import copy
 import math
 
 import pytest
@@ -644,3 +645,37 @@ def test_prefix_attention_descending_offsets(B, pages):
             ops.prefix_attention(kv, q, off, lens, table, _i32([1, 2]), prefix, out=out, lse=lse, err=err)
             assert int(err) == ops.BAD_INDEX
             assert (out == 5.0).all() and (lse == 6.0).all()
+
+
+def test_copies_of_views_and_rotations():
+    """A copied cache view is of the copied tensors, a copied rotation outlives its original."""
+    s = Streams([3], [5], 8, 2, 32, F16, filled=False)
+    q, k, v = _rows(s, 4, 32, F16, 1), _rows(s, 2, 32, F16, 2), _rows(s, 2, 32, F16, 3)
+    rope, kv = copy.deepcopy(ops.Rope(32, base=500.0)), copy.deepcopy(s.kv)
+    before = s.kv.k.clone()
+    got = ops.rope_append(rope, kv, q, k, v, s.d_off, s.d_lens, s.d_table)
+    assert torch.equal(s.kv.k.view(torch.int16), before.view(torch.int16))
+    want = ops.rope_append(ops.Rope(32, base=500.0), s.kv, q, k, v, s.d_off, s.d_lens, s.d_table)
+    assert torch.equal(got, want) and torch.equal(kv.k.view(torch.int16), s.kv.k.view(torch.int16))
+
+
+def test_rotating_queries_without_pages():
+    """With no keys to store the table may be empty."""
+    s = Streams([3, 2], [5, 9], 8, 2, 32, F16, filled=False)
+    q = _rows(s, 4, 32, F16, 1)
+    got = ops.rope_append(ops.Rope(32), s.kv, q, None, None, s.d_off, s.d_lens, s.d_table[:, :0], err=s.err)
+    ops.check(s.err)
+    assert torch.equal(got, ops.rope_append(ops.Rope(32), s.kv, q, None, None, s.d_off, s.d_lens, s.d_table))
+
+
+def test_results_that_share_memory_or_want_gradients():
+    s = Streams([2], [4], 16, 2, 64, F16)
+    q = torch.zeros((2, 4, 64), dtype=F16, device=DEV)
+    meta = (s.d_off, s.d_lens, s.d_table)
+    for out in (q[:1].expand(2, 4, 64), q[:, :1].expand(2, 4, 64), q.clone().requires_grad_()):
+        with pytest.raises(R.Z2BError):
+            ops.prefix_attention(s.kv, q, *meta, out=out)
+        with pytest.raises(R.Z2BError):
+            ops.rope_append(None, s.kv, q, None, None, *meta, out=out)
+    with pytest.raises(R.Z2BError):
+        ops.PagedKV(s.kv.k.clone().requires_grad_(), s.kv.v.clone().requires_grad_())

@@ -175,3 +175,18 @@ def test_rope_table_against_decimals(kw):
             assert abs(decimal.Decimal(int(t.step[i])) - want) <= want * decimal.Decimal(16 * 2.0 ** -53) + 1
     assert t.mag == pytest.approx(0.1 * math.log(16.0) + 1.0 if kw.get("scaling") == "by_parts" else 1.0, rel=2.0 ** -23)
 
+
+
+def test_sizes_that_32_bits_do_not_number():
+    """Rows, heads, and the prefix's and the streams' units together."""
+    for bad in (dict(n_rows=(1 << 30) + 1), dict(n_head=(1 << 20) + 1)):
+        assert _call("z2b_rope_append", _append(**bad))[0] == UNSUPPORTED
+    # 2048 tiles of 8 rows, and 2^19 units of 32 keys: 2049 (2^19 + 1) > 2^30 for the prefix or the pages, both over 2^31
+    half = dict(n_rows=1 << 13, n_seq=1, n_head=2, max_pages=1, table_stride=1 << 20, prefix_len=1 << 24)
+    both = dict(half, max_pages=1 << 20)
+    L = args.library()
+    for kw, fits in ((half, True), (both, False)):
+        a = _attn(_view(n_head_kv=1), **kw)
+        assert (L.z2b_prefix_attention_workspace(ctypes.addressof(a)) > 0) == fits
+    assert _call("z2b_prefix_attention", _attn(_view(n_head_kv=1), **both))[0] == UNSUPPORTED
+    assert _call("z2b_prefix_attention", _attn(scale=3e38))[0] == ARG

@@ -114,6 +114,8 @@ int z2b_rope_append(const z2b_rope_append_args* args, void* stream) {
         return bad("rope_append: the rotation does not fit head_dim");
     if (a.kv->head_dim > 1024) return unsupported("rope_append: head_dim above 1024");
     if (a.n_seq > OPS_MAX_SEQ) return unsupported("rope_append: more than 4096 streams");
+    if (a.n_rows > (1 << 30) || a.n_head > (1 << 20) || a.kv->n_head_kv > (1 << 20))    // row and head numbers are 32-bit
+        return unsupported("rope_append: too many rows or heads for one call");
     const unsigned e = type_size(a.type);
     if (!aligned(a.q, e) || !aligned(a.q_out, e) || !aligned(a.k, e) || !aligned(a.v, e) || !aligned(a.pos, 4))
         return bad("rope_append: misaligned array");
@@ -141,7 +143,7 @@ static const char* check_attn(const z2b_prefix_attn_args& a, int* rc) {
     const long long G = a.n_head / c.n_head_kv, tiles = ((long long)a.n_rows * G + 7) / 8;
     const long long own = ((long long)a.max_pages * c.page_len + 31) / 32 + 1, pf = ((long long)a.prefix_len + 31) / 32 + 1;
     if (tiles * c.n_head_kv > (1 << 24) || (long long)a.n_seq * c.n_head_kv > (1 << 24) || own > (1 << 24) || pf > (1 << 24) ||
-        ((long long)a.n_rows + 32) * G * G > 0xffffffffll || (tiles + a.n_seq) * c.n_head_kv * own > 0x7fffffffll || (tiles + 1) * c.n_head_kv * pf > 0x7fffffffll)
+        ((long long)a.n_rows + 32) * G * G > 0xffffffffll || ((tiles + a.n_seq) * own + (tiles + 1) * pf) * c.n_head_kv > 0x7fffffffll)
         return "prefix_attention: too many rows, streams or pages for one call";
     return "";
 }
@@ -164,7 +166,7 @@ int z2b_prefix_attention(const z2b_prefix_attn_args* args, void* stream) {
     const z2b_paged_kv& c = *a.kv;
     if (!aligned(c.k, 16) || !aligned(c.v, 16) || (c.page_stride | c.row_stride | c.head_stride) % 8)
         return bad("prefix_attention: the cache must be 16-byte aligned with strides that are multiples of 8");
-    if (!std::isfinite(a.scale)) return bad("prefix_attention: scale must be finite");
+    if (!std::isfinite(a.scale * 2.0f)) return bad("prefix_attention: scale must be finite, and twice it");
     if (a.n_rows == 0 || a.n_seq == 0) return Z2B_OK;
     if (!a.q || !a.out) return bad("prefix_attention: null q or out");
     if (!aligned(a.q, 4) || !aligned(a.out, 4) || (a.q_row | a.q_head | a.o_row | a.o_head) % 2 || !aligned(a.lse, 4))

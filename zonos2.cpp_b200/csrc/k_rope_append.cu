@@ -75,7 +75,7 @@ __global__ void __launch_bounds__(32 * WARPS) rope_append_ops_kernel(const __gri
     const int lo = p.row_off[b], n = p.row_off[b + 1] - lo, len = p.seq_len[b];
     if (t >= total) return;                                          // padding stays as it is
     const long long r = (long long)len - n + (t - lo);               // cache row
-    if (t < lo || t - lo >= n || r < 0 || r >= (long long)p.max_pages * p.page_len) {
+    if (t < lo || t - lo >= n || r < 0 || (p.k && r >= (long long)p.max_pages * p.page_len)) {
         if (lane == 0 && p.err) atomicOr(p.err, Z2B_OPS_BAD_INDEX);
         return;
     }

@@ -9,7 +9,9 @@ tensor of one element on the device that the kernels OR ``BAD_INDEX``, ``BAD_PAG
 
 Rows are packed over the streams: stream b owns rows [row_off[b], row_off[b + 1]) of q
 [rows][heads][head_dim], rows from row_off[-1] on are padding and stay as they are, seq_len[b]
-counts the stream's cached rows with the new ones, and page_table[b] lists its pages.
+counts the stream's cached rows with the new ones, and page_table[b] lists its pages. There is no
+backward pass: inputs that want gradients are refused, and autograd does not see what is written in
+place (the pages, `out`, `lse`).
 """
 from __future__ import annotations
 
@@ -73,6 +75,10 @@ class Rope:
         rc = f(self._at, int(rot_dim), _LAYOUT[layout], float(base), _SCALING[scaling], float(factor), int(orig_ctx))
         if rc:
             raise Z2BError(rc, lib().z2b_last_error().decode(errors="replace"))
+        self._args = (rot_dim, base, layout, scaling, factor, orig_ctx)
+
+    def __reduce__(self):               # a copy has a table, and its address, of its own
+        return Rope, self._args
 
 
 class PagedKV:
@@ -86,6 +92,8 @@ class PagedKV:
             _refuse("kv: f16 or bf16 CUDA tensors are wanted")
         if k.stride(3) != 1 or 0 in k.shape:
             _refuse("kv: the dims of a head must be contiguous, and no size zero")
+        if k.requires_grad or v.requires_grad:
+            _refuse("kv: the pages are written in place, without a gradient")
         self.k, self.v, self.device, self.dtype = k, v, k.device, k.dtype
         self.n_pages, self.page_len, self.n_head_kv, self.head_dim = k.shape
         # a stride along a dimension of one says nothing: it reads as if packed
@@ -95,6 +103,9 @@ class PagedKV:
         sp = sp if self.n_pages > 1 else self.page_len * self.n_head_kv * self.head_dim
         self.view = PagedKVView(k.data_ptr(), v.data_ptr(), _TYPE[k.dtype], *k.shape, sp, sr, sh)
         self._idx, self._at, self._scale = k.get_device(), ctypes.addressof(self.view), 1.0 / math.sqrt(self.head_dim)
+
+    def __reduce__(self):               # a copy's view is of the copied tensors
+        return PagedKV, (self.k, self.v)
 
 
 def rope_append(rope: Rope | None, kv: PagedKV, q, k, v, row_off, seq_len, page_table, prefix_len: int = 0, pos=None,
