@@ -10,7 +10,8 @@ The directory name is not an identifier, so load it under the name ``z2b``::
     spec.loader.exec_module(z2b)
 
 Submodules: ``z2b.runtime`` (ctypes binding of include/z2b.h), ``z2b.synth``
-(synthetic GGUF files), ``z2b.build`` (nvcc build recipe).
+(synthetic GGUF files), ``z2b.build`` (nvcc build recipe), ``z2b.ops`` (the operators of
+include/z2b_ops.h on torch CUDA tensors).
 """
 import os
 
