@@ -679,3 +679,13 @@ def test_results_that_share_memory_or_want_gradients():
             ops.rope_append(None, s.kv, q, None, None, *meta, out=out)
     with pytest.raises(R.Z2BError):
         ops.PagedKV(s.kv.k.clone().requires_grad_(), s.kv.v.clone().requires_grad_())
+
+
+@pytest.mark.parametrize("lens", [[30001, 27000], [5000, 3], [1, 1]], ids=str)
+def test_prefix_attention_long_own_behind_long_prefix(lens):
+    """A prefix with a launch of its own, and own keys that outlast it, end with it and hardly are there."""
+    s = Streams([1, 1], lens, 64, 1, 64, BF16, prefix=32768, seed=40)
+    q = torch.randn((2, 32, 64), generator=_gen(41)).to(BF16).to(DEV)
+    out, lse = ops.prefix_attention(s.kv, q, s.d_off, s.d_lens, s.d_table, s.d_shared, 32768, lse=True, err=s.err)
+    ops.check(s.err)
+    _check_attention(s, q, out, lse)

@@ -33,6 +33,7 @@ __host__ __device__ constexpr int unit_keys(int hd) { return 32; }
 __host__ __device__ constexpr int ring_stages(int hd) { return hd == 128 ? 2 : hd == 64 ? 3 : hd == 32 ? 6 : 8; }
 __host__ __device__ constexpr int max_warps(int hd) { return hd == 128 ? 6 : 8; }
 constexpr int MAX_SMEM = 226 * 1024;   // dynamic shared memory of a launch
+constexpr int CTAS = 148;              // one per SM
 
 // Shared-memory tile of KU rows of one key head: rows of RB bytes (at most 128: head_dim 128
 // is two halves), 16-byte chunks XOR-swizzled as the TMA box writes them.
@@ -175,12 +176,21 @@ __global__ void __launch_bounds__(32 * max_warps(HD), 1) prefix_attn_kernel(cons
     ln.pf_units = p.pf_row_tiles * p.nkv * (ln.pf_nt + SEG_COST);
     __syncthreads();
     const int W = ln.pf_units + s_rec[p.n_seq].x;
-    const Cut cut(W, gridDim.x * nw);
-    const int me = warp * gridDim.x + blockIdx.x;                // few workers: one per SM first
-    int u = 0, u1 = 0;
-    if (me < cut.workers) {
-        u = cut.begin(me);
-        u1 = cut.begin(me + 1);
+    const Cuts cuts(p, W, gridDim.x, nw);
+    int me, u = 0, u1 = 0;                                       // few workers: one per SM first
+    if ((int)blockIdx.x < p.early) {
+        me = warp * p.early + blockIdx.x;
+        if (me < cuts.a.workers) {
+            u = cuts.a.begin(me);
+            u1 = cuts.a.begin(me + 1);
+        }
+    } else {
+        const int i = warp * (gridDim.x - p.early) + blockIdx.x - p.early;
+        me = cuts.na + i;
+        if (i < cuts.b.workers) {
+            u = cuts.mid + cuts.b.begin(i);
+            u1 = cuts.mid + cuts.b.begin(i + 1);
+        }
     }
 
     // ---- the copies, NS units ahead of the products: a box of K and one of V per run of rows
@@ -530,23 +540,30 @@ template <int MT, int KU> __device__ __forceinline__ Parts find_parts(const Join
     const int h = div_g(a, head), g = head - h * a.G;
     const int pf_units = a.pf_row_tiles * a.nkv * (cdiv(a.prefix_len, KU) + SEG_COST);
     const int positions = pf_units + x.own_units;
-    const Cut cut(positions, p.own.workers);
+    const Cuts cuts(a, positions, CTAS, p.own.workers / CTAS);
     Parts r{0, 0, 0, 0, 0, 0};
     if (a.prefix_len > 0) {
         const int nt = cdiv(a.prefix_len, p.pf.keys), row = t * a.G + g, j = row / p.pf.mt, seg = p.pf_apart ? j * a.nkv + h : h * p.pf.row_tiles + j;
         const int cost = p.pf_apart ? TC_SEG_COST : SEG_COST, first = seg * (nt + cost) + cost;
-        const int Wp = p.pf_apart ? p.pf.row_tiles * a.nkv * (nt + cost) : positions;
-        const Cut cp(Wp, p.pf.workers);
-        const int c0 = cp.owner(first, Wp);
-        r.n0 = cp.owner(first + nt - 1, Wp) - c0 + 1;
+        int c0, c1;
+        if (p.pf_apart) {
+            const int Wp = p.pf.row_tiles * a.nkv * (nt + cost);
+            const Cut cp(Wp, p.pf.workers);
+            c0 = cp.owner(first, Wp);
+            c1 = cp.owner(first + nt - 1, Wp);
+        } else {
+            c0 = cuts.owner(first);
+            c1 = cuts.owner(first + nt - 1);
+        }
+        r.n0 = c1 - c0 + 1;
         r.slot0 = seg + c0;
         r.row0 = row - j * p.pf.mt;
     }
     if (x.s.nt > 0) {
         const int row = x.i * a.G + g, js = h * x.s.qt + row / MT;
         const int first = pf_units + x.unit_b + js * (x.s.nt + SEG_COST) + SEG_COST;
-        const int c0 = cut.owner(first, positions);
-        r.n1 = cut.owner(first + x.s.nt - 1, positions) - c0 + 1;
+        const int c0 = cuts.owner(first);
+        r.n1 = cuts.owner(first + x.s.nt - 1) - c0 + 1;
         r.slot1 = a.pf_row_tiles * a.nkv + x.seg_b + js + c0;
         r.row1 = row % MT;
     }
@@ -757,6 +774,7 @@ __global__ void __launch_bounds__(256, 4) prefix_attn_join_few_kernel(const __gr
 struct HostPlan {
     int G, nb, warps;                   // blocks of 8 rows in an own segment, warps of a CTA
     PartSet own, pf;                    // pointers unset
+    int early, head_start;              // as in AttnP
     bool pf_tc;                         // the prefix has a launch of its own, on tcgen05
     size_t off_own_ml, off_own_o, off_pf_ml, off_pf_o, bytes;
 };
@@ -767,6 +785,16 @@ size_t attn_smem(int hd, int nb, int warps, int n_seq) {
 }
 
 size_t up(size_t x) { return (x + 255) & ~(size_t)255; }
+
+// The prefix on tcgen05 fills an SM, its own keys' kernel another's: the first is kept to all SMs but
+// PF_LEAVES, where the second starts beside it (the tensor cores are power-bound and lose less than
+// their share of SMs, HBM would idle). While a CTA there takes one of its units an early CTA takes
+// some OWN_PER_PF; what the early ones do not get through, all SMs share when the prefix is done.
+// None / 36 left, us: 256 streams, 32 heads of 128, prefix 32768, own up to 600: 198 / 177; 64, 16 heads,
+// 8192, up to 200: 48 / 38; up to 4000: 105 / 93; 64 x 5 rows of 64 dims, 4097, up to 300: 42 / 40; with
+// next to no own keys it costs: 256, 32768, up to 8: 97 / 94 at 128, 71 / 80 at 64. 16, 24, 32, 40 left, the
+// first of these at 12 units: 219 (the early CTAs end last), 214, 182, 181.
+constexpr int PF_LEAVES = 36, OWN_PER_PF = 16;
 
 HostPlan host_plan(const z2b_prefix_attn_args& a) {
     HostPlan h{};
@@ -789,7 +817,7 @@ HostPlan host_plan(const z2b_prefix_attn_args& a) {
     // at head_dim 64: R 64: 9 / 17, 10 / 17, 18 / 18, 41 / 26; R 256: 17 / 24, 23 / 25, 48 / 27, 142 / 37
     h.pf_tc = hd >= 64 && R >= 32 && (double)a.n_rows * a.n_head * a.prefix_len >= 2097152.0;
     const int pf_tiles = a.prefix_len > 0 && !h.pf_tc ? (int)((R + mt - 1) / mt) : 0;
-    h.own = PartSet{nullptr, nullptr, mt, unit_keys(hd), 148 * h.warps, 0, pf_tiles};
+    h.own = PartSet{nullptr, nullptr, mt, unit_keys(hd), CTAS * h.warps, 0, pf_tiles};
     const long long segs = ((R + mt - 1) / mt + a.n_seq + pf_tiles) * nkv;
     h.own.slots = (int)(segs + h.own.workers);
     h.pf = h.own;
@@ -800,7 +828,9 @@ HostPlan host_plan(const z2b_prefix_attn_args& a) {
         const int tiles = (int)((R + TC_ROWS - 1) / TC_ROWS);
         // a multiple of the row tiles, where that leaves few SMs idle: the row tiles are cut alike then,
         // so the CTAs that read the same keys do so at the same time and all but one find them in L2
-        const int ctas = tiles <= 148 && 148 % tiles * 20 <= 148 ? 148 - 148 % tiles : 148;
+        const int most = CTAS - PF_LEAVES, ctas = tiles <= most && most % tiles * 20 <= most ? most - most % tiles : most;
+        h.early = CTAS - ctas;
+        h.head_start = (int)((long long)OWN_PER_PF * tiles * nkv * ((a.prefix_len + TC_KEYS - 1) / TC_KEYS + TC_SEG_COST) / ctas);
         h.pf = PartSet{nullptr, nullptr, TC_ROWS, TC_KEYS, ctas, tiles * nkv + ctas, tiles};
         h.off_pf_ml = n; n += up((size_t)h.pf.slots * TC_ROWS * 8);
         h.off_pf_o = n; n += up((size_t)h.pf.slots * TC_ROWS * hd * 4);
@@ -820,7 +850,7 @@ cudaError_t go_attn(const AttnP& p, const CUtensorMap& km, const CUtensorMap& vm
         if (e != cudaSuccess) return e;
         if (dev < 64) opted.fetch_or(1ull << dev, std::memory_order_relaxed);
     }
-    return launch_pdl(prefix_attn_kernel<T, HD, NB>, dim3(148), dim3(32 * warps),
+    return launch_pdl(prefix_attn_kernel<T, HD, NB>, dim3(CTAS), dim3(32 * warps),
                       attn_smem(HD, NB, warps, p.n_seq), s, p, km, vm);
 }
 
@@ -865,6 +895,8 @@ cudaError_t go_all(const z2b_prefix_attn_args& a, HostPlan h, cudaStream_t s) {
         return cudaErrorNotSupported;
     p.pf_row_tiles = h.own.row_tiles;
     p.after_prefix = h.pf_tc;
+    p.early = h.early;
+    p.head_start = h.head_start;
     h.own.ml = p.part_ml = (float2*)(ws + h.off_own_ml);
     h.own.o = p.part_o = (float*)(ws + h.off_own_o);
     e = h.nb == 1 ? go_attn<T, HD, 1>(p, km, vm, h.warps, s) : cudaSuccess;

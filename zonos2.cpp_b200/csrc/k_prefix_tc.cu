@@ -18,8 +18,8 @@
 //
 // Bound: per unit the products of both tiles take 2048 cycles at head_dim 128, and the
 // 2 x 128^2 exponentials the same at 16 per cycle and SM; under the load the SMs run at about
-// 1.5 GHz. 1024 rows of each of 8 key heads over 32768 keys (137 GFLOP) take 125 us, 1.1
-// PFLOP/s, 67% of measured cuBLAS bf16. Tried on that case and slower: two blocks of 64 scores
+// 1.5 GHz. 1024 rows of each of 8 key heads over 32768 keys (137 GFLOP) take 125 us on
+// all SMs, 1.1 PFLOP/s, 67% of measured cuBLAS bf16. Tried on that case and slower: two blocks of 64 scores
 // a tile in place of one of 128, so that scores never wait for the product that frees them
 // (+14 us: 64 keys are fed at 3/4 rate, 6 KB of operands per 32 cycles from shared memory);
 // reading the scores twice to spare registers (+10 us); a quarter of the exponentials by a

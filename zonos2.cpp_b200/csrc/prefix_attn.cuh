@@ -35,6 +35,7 @@ struct AttnP {
     float scale2;                      // scale * log2(e)
     int pf_row_tiles;                  // row tiles of the prefix in this launch (0: none)
     int after_prefix;                  // 1: the launch before is the prefix's, which this one runs beside
+    int early, head_start;             // CTAs that find an SM while that one runs, and line positions each gets through meanwhile
     float* part_o;                     // [slots][rows of a segment][head_dim]
     float2* part_ml;                   // [slots][rows of a segment] (m in log2 units, l)
     int* plan;                         // [2][n_seq + 1] unit and segment offsets of the streams, written for the join
@@ -74,6 +75,7 @@ struct Cut {
         rest = W - each * workers;
         inv = workers > 1 ? 0xffffffffu / (unsigned)workers + 1u : 0u;
     }
+    __device__ __forceinline__ Cut() {}
     __device__ __forceinline__ int begin(int i) const { return i * each + (int)__umulhi((unsigned)(i * rest), inv); }
     // The worker that holds position u: an f32 guess, off by one at most, put right exactly.
     __device__ __forceinline__ int owner(int u, int W) const {
@@ -82,6 +84,23 @@ struct Cut {
         while (begin(i + 1) <= u) ++i;
         return i;
     }
+};
+
+// The line of the own kernel: workers of the first p.early CTAs take [0, mid), which their head
+// start makes longer ranges, the others [mid, W). Worker numbers go along the line.
+struct Cuts {
+    Cut a, b;
+    int W, mid, na;
+    __device__ __forceinline__ Cuts(const AttnP& p, int W_, int ctas, int warps) : W(W_), mid(0), na(0) {
+        if (p.early > 0) {
+            const long long lead = (long long)p.early * p.head_start;
+            mid = W <= lead ? W : (int)(lead + (W - lead) * p.early / ctas);
+            a = Cut(mid, p.early * warps);
+            na = a.workers;
+        }
+        b = Cut(W - mid, (ctas - p.early) * warps);
+    }
+    __device__ __forceinline__ int owner(int u) const { return u < mid ? a.owner(u, mid) : na + b.owner(u - mid, W - mid); }
 };
 
 template <typename T> __device__ __forceinline__ void mma_t(float* d, const uint32_t* a, uint32_t b0, uint32_t b1);
