@@ -810,11 +810,11 @@ HostPlan host_plan(const z2b_prefix_attn_args& a) {
     while (attn_smem(hd, h.nb, h.warps, a.n_seq) > MAX_SMEM) --h.warps;
     const long long R = (long long)a.n_rows * h.G;
     const int mt = 8 * h.nb;
-    // The prefix on tcgen05 costs a launch and its filling (8 us), on the line a read of its keys per
+    // The prefix on tcgen05 costs a launch and its filling (6 us), on the line a read of its keys per
     // row tile. Calls of 4 key heads, head_dim 128, line / tcgen05 in us, R rows a key head, prefixes of
-    // 512, 2048, 8192, 32768: R 16: 9 / 14, 11 / 15, 14 / 20, 25 / 32; R 32: 10 / 15, 11 / 15, 16 / 21,
-    // 36 / 33; R 64: 11 / 20, 13 / 20, 22 / 22, 61 / 36; R 256: 20 / 30, 31 / 31, 70 / 35, 218 / 50; and
-    // at head_dim 64: R 64: 9 / 17, 10 / 17, 18 / 18, 41 / 26; R 256: 17 / 24, 23 / 25, 48 / 27, 142 / 37
+    // 512, 2048, 8192, 32768: R 16: 9 / 15, 11 / 15, 14 / 17, 25 / 32; R 32: 10 / 15, 11 / 16, 16 / 18,
+    // 36 / 32; R 64: 11 / 16, 13 / 17, 22 / 19, 61 / 34; R 256: 20 / 29, 31 / 33, 70 / 38, 218 / 55; and
+    // at head_dim 64: R 64: 9 / 14, 10 / 14, 18 / 16, 41 / 27; R 256: 17 / 23, 23 / 25, 48 / 27, 142 / 40
     h.pf_tc = hd >= 64 && R >= 32 && (double)a.n_rows * a.n_head * a.prefix_len >= 2097152.0;
     const int pf_tiles = a.prefix_len > 0 && !h.pf_tc ? (int)((R + mt - 1) / mt) : 0;
     h.own = PartSet{nullptr, nullptr, mt, unit_keys(hd), CTAS * h.warps, 0, pf_tiles};
