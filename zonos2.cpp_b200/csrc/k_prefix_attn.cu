@@ -790,10 +790,11 @@ size_t up(size_t x) { return (x + 255) & ~(size_t)255; }
 // PF_LEAVES, where the second starts beside it (the tensor cores are power-bound and lose less than
 // their share of SMs, HBM would idle). While a CTA there takes one of its units an early CTA takes
 // some OWN_PER_PF; what the early ones do not get through, all SMs share when the prefix is done.
-// None / 36 left, us: 256 streams, 32 heads of 128, prefix 32768, own up to 600: 198 / 177; 64, 16 heads,
-// 8192, up to 200: 48 / 38; up to 4000: 105 / 93; 64 x 5 rows of 64 dims, 4097, up to 300: 42 / 40; with
-// next to no own keys it costs: 256, 32768, up to 8: 97 / 94 at 128, 71 / 80 at 64. 16, 24, 32, 40 left, the
-// first of these at 12 units: 219 (the early CTAs end last), 214, 182, 181.
+// None / 36 left, us: 256 streams, 32 heads of 128, prefix 32768, own up to 600: 198 / 177 (212 / 206
+// over hundreds of passes, when the clocks have fallen); 64, 16 heads, 8192, up to 200: 48 / 38; up to
+// 4000: 105 / 93; 64 x 5 rows of 64 dims, 4097, up to 300: 42 / 40. With next to no own keys 64 dims
+// lose (256, 32768, up to 8: 71 / 80; 128 dims: 97 / 94). 16, 24, 32, 40 left, the first of these at 12
+// units: 219 (the early CTAs end last), 214, 182, 181.
 constexpr int PF_LEAVES = 36, OWN_PER_PF = 16;
 
 HostPlan host_plan(const z2b_prefix_attn_args& a) {
