@@ -20,7 +20,7 @@
  * Strides count elements. `err`, when not NULL, is a uint32 word on the device that the
  * kernels OR their findings into, never clearing it: Z2B_OPS_BAD_INDEX for offsets, lengths
  * or token ids out of range (the row is skipped, the token refused; offsets that descend:
- * z2b_prefix_attention skips every row), Z2B_OPS_BAD_PAGE for a
+ * z2b_prefix_attention skips every row) and for u_draw outside [0, 1), Z2B_OPS_BAD_PAGE for a
  * page id outside the cache (its keys read as zeros, its rows are not stored),
  * Z2B_OPS_TIMEOUT for a bounded wait that ran out. No input is dereferenced before it is
  * checked, with or without `err`.
@@ -163,7 +163,7 @@ typedef struct z2b_verify_args {
     const int32_t* draft;              /* [n_seq][max_draft][n_codebooks] token ids */
     const int32_t* n_draft;            /* [n_seq] drafted frames, 0..max_draft, or NULL: max_draft each */
     const double* u_accept;            /* [n_seq][max_draft][n_codebooks] uniforms in [0, 1) */
-    const double* u_draw;              /* [n_seq][max_draft + 1][n_codebooks] */
+    const double* u_draw;              /* [n_seq][max_draft + 1][n_codebooks], in [0, 1) too */
     int32_t* tokens;                   /* [n_seq][max_draft + 1][n_codebooks]: accepted frames, one more frame, -1 behind */
     int32_t* n_accepted;               /* [n_seq] */
     int64_t p_seq, p_frame, p_book, q_seq, q_frame, q_book;   /* strides; vocab is contiguous */
@@ -175,7 +175,8 @@ typedef struct z2b_verify_args {
  * each refused token of it is replaced by a draw from max(p - q, 0) (from p where that is
  * zero everywhere); when all drafts are kept, one frame more is drawn from p. Frames then
  * follow the target's distribution exactly. A draw takes the first token whose running sum
- * (64 bits) exceeds u_draw * total; a row of p without any mass gives -1. A p(x) or q(x) that is
+ * (64 bits) exceeds u_draw * total; a u_draw below 0 counts as 0, any other outside [0, 1) draws
+ * the last token with mass; a row of p without any mass gives -1. A p(x) or q(x) that is
  * not a number refuses its token, a difference that is not a number counts as zero in a draw. */
 int z2b_verify_drafts(const z2b_verify_args* args, void* stream);
 

@@ -32,6 +32,8 @@ namespace cg = cooperative_groups;
 constexpr int MAX_CLUSTER = 8;          // CTAs per row: the portable cluster size
 constexpr int EACH = 8;                 // entries of a small row that a thread holds
 constexpr int SMALL_WARPS = 8, LARGE_WARPS = 12;
+// A draw's answer where it is no token: the row has no mass at all, or another CTA has the token.
+constexpr int NO_MASS = -1, ELSEWHERE = -2;
 
 struct VerifyP {
     z2b_verify_args a;
@@ -62,8 +64,8 @@ template <int WARPS> struct DrawShared {
     int found, last;
 };
 
-// The drawn token of a row of at most 32 WARPS EACH entries, or -1 when the mass is zero
-// everywhere. Called by the whole CTA; all threads get it.
+// The drawn token of a row of at most 32 WARPS EACH entries, or NO_MASS. r in [0, 1]. Called by
+// the whole CTA; all threads get it.
 template <typename T, bool HAS_Q, bool SUB, int WARPS>
 __device__ int draw_small(const T* p, const T* q, int V, int drafted, double r, DrawShared<WARPS>& sh) {
     const int w = threadIdx.x >> 5, lane = threadIdx.x & 31, each = (V + 32 * WARPS - 1) / (32 * WARPS);
@@ -89,7 +91,7 @@ __device__ int draw_small(const T* p, const T* q, int V, int drafted, double r, 
         if (i == w) before = total;
         total += sh.warp_tot[i];
     }
-    if (!(total > 0.0)) return -1;
+    if (!(total > 0.0)) return NO_MASS;
     const double target = r * total;
     before += inc - mine;
     if (mine > 0.0) {
@@ -110,9 +112,11 @@ __device__ int draw_small(const T* p, const T* q, int V, int drafted, double r, 
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
 
-// The drawn token, or -1 when the mass is zero everywhere. Called by every thread of the
-// cluster, all of whose CTAs have started; all get the same `total`, only the CTA whose range
-// holds the target a token (the others -2). `set`: 0 for a cluster's first draw, 1 for its second.
+// The drawn token, r in [0, 1]. Called by every thread of the cluster, all of whose CTAs have
+// started. NO_MASS comes from the cluster's total alone, so that its CTAs agree whether another draw
+// (with its barriers) follows; else the CTA whose range holds the target gets the token and the others
+// ELSEWHERE. That range has mass: the target is at least 0, so a range whose sum takes the running
+// total past it adds to it. `set`: 0 for a cluster's first draw, 1 for its second.
 template <typename T, bool HAS_Q, bool SUB, int WARPS>
 __device__ int draw_large(const T* p, const T* q, int V, int drafted, double r, int rank, int n_cta, int set, DrawShared<WARPS>& sh) {
     constexpr int THREADS = 32 * WARPS;
@@ -149,7 +153,7 @@ __device__ int draw_large(const T* p, const T* q, int V, int drafted, double r, 
         cta[i] = i < n_cta ? sh.cta[set][i] : 0.0;
         total += cta[i];
     }
-    if (!(total > 0.0)) return -1;
+    if (!(total > 0.0)) return NO_MASS;
     const double target = r * total;
     double run = 0.0;
 #pragma unroll
@@ -160,7 +164,7 @@ __device__ int draw_large(const T* p, const T* q, int V, int drafted, double r, 
     }
     const bool past = owner < 0;                                 // rounding left the target at the total
     if (past) owner = tail;
-    if (owner != rank) return -2;
+    if (owner != rank) return ELSEWHERE;
     int share_w = -1, tail_w = 0;
     double run_w = base;
     for (int i = 0; i < WARPS; ++i) {
@@ -270,19 +274,23 @@ __global__ void __launch_bounds__(32 * WARPS) verify_kernel(const __grid_constan
         if (rank == 0 && threadIdx.x == 0) out[end * C] = x;
         return;
     }
-    const double r = a.u_draw[((long long)b * (N + 1) + end) * C + c];
+    double r = a.u_draw[((long long)b * (N + 1) + end) * C + c];
+    if (!(r >= 0.0 && r < 1.0)) {                                // below: the first token with mass, else the last
+        if (rank == 0 && threadIdx.x == 0 && a.err) atomicOr(a.err, Z2B_OPS_BAD_INDEX);
+        r = r < 0.0 ? 0.0 : 1.0;
+    }
     const T* pr = p + end * a.p_frame + c * a.p_book;
     const T* qr = HAS_Q && end < n ? q + end * a.q_frame + c * a.q_book : nullptr;
-    int tok = -1;
+    int tok = NO_MASS;
     if constexpr (WARPS == SMALL_WARPS) {
         if (end < n) tok = draw_small<T, HAS_Q, true, WARPS>(pr, qr, V, x, r, sh);
-        if (tok == -1) tok = draw_small<T, HAS_Q, false, WARPS>(pr, nullptr, V, -1, r, sh);
+        if (tok == NO_MASS) tok = draw_small<T, HAS_Q, false, WARPS>(pr, nullptr, V, -1, r, sh);
     } else {
         if (end < n) tok = draw_large<T, HAS_Q, true, WARPS>(pr, qr, V, x, r, rank, n_cta, 0, sh);
-        if (tok == -1) tok = draw_large<T, HAS_Q, false, WARPS>(pr, nullptr, V, -1, r, rank, n_cta, 1, sh);
+        if (tok == NO_MASS) tok = draw_large<T, HAS_Q, false, WARPS>(pr, nullptr, V, -1, r, rank, n_cta, 1, sh);
     }
-    // -1: a row without any mass has no token; its first CTA says so
-    if (threadIdx.x == 0 && (tok >= 0 || (tok == -1 && rank == 0))) out[end * C] = tok;
+    // a row without any mass has no token (-1); its first CTA says so
+    if (threadIdx.x == 0 && (tok >= 0 || (tok == NO_MASS && rank == 0))) out[end * C] = tok;
 }
 
 template <typename T, int WARPS> cudaError_t go(const VerifyP& P, bool has_q, dim3 grid, cudaStream_t s) {

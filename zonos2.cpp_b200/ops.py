@@ -54,7 +54,7 @@ def check(err):
     """Raise Z2BError when a kernel has recorded a finding in `err` (synchronises)."""
     bits = int(err.item())
     if bits:
-        names = [n for b, n in ((TIMEOUT, "a bounded wait ran out"), (BAD_INDEX, "an offset, length or token id out of range"),
+        names = [n for b, n in ((TIMEOUT, "a bounded wait ran out"), (BAD_INDEX, "an offset, length, token id or number drawn with out of range"),
                                 (BAD_PAGE, "a page id outside the cache")) if bits & b]
         raise Z2BError(6, ", ".join(names))
 
