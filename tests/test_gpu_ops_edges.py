@@ -73,3 +73,31 @@ def test_verify_second_draw_of_a_cluster(B, C):
     tok, kept = ops.verify_drafts(*_dev(p, q, draft, u, r))
     want = ops_ref.verify(p, q, draft, u, r, None)
     assert (want[1] == 0).all() and torch.equal(tok.cpu(), want[0]) and torch.equal(kept.cpu(), want[1])
+
+
+@pytest.mark.parametrize("V", [1026, 5000, 40007], ids=str)       # rows in threads, in one CTA, in a cluster
+def test_verify_never_draws_a_token_without_mass(V):
+    """Numbers at every border of the running sums: whichever side of it rounding puts a sum, the token
+    drawn has mass, and is one of the two that meet there. Probabilities over 40 orders of magnitude, so that
+    the order of the sums does round."""
+    g = _gen(V)
+    p = torch.softmax(torch.randn(V, generator=g) * 12, -1)
+    q = torch.softmax(torch.randn(V, generator=g) * 12, -1)
+    left = (p.double() - q.double()).clamp(min=0)
+    some = left.nonzero().flatten()
+    pick = some[torch.linspace(0, len(some) - 1, 500).long()]
+    r0 = left.cumsum(0)[pick] / left.sum()
+    r = torch.cat([(r0 + k * 2.0 ** -53).clamp(0, 1 - 2.0 ** -53) for k in (-2, -1, 0, 1, 2)])
+    B = len(r)
+    p2, q2 = (x.to(DEV).expand(B, n, 1, V) for x, n in ((p, 2), (q, 1)))
+    draft = torch.full((B, 1, 1), int(q.argmax()), dtype=torch.int32)
+    u, rr = torch.ones((B, 1, 1), dtype=F64), torch.zeros((B, 2, 1), dtype=F64)
+    rr[:, 0, 0] = r
+    assert p[q.argmax()] <= q.max()                           # u = 1 refuses it
+    tok, kept = ops.verify_drafts(p2, q2, *_dev(draft, u, rr))
+    tok = tok[:, 0, 0].cpu().long()
+    assert (kept == 0).all() and (left[tok] > 0).all()
+    # the sum up to the token, and ahead of it, against the target: off by V roundings of 2^-53 of the total
+    cum, slack = left.cumsum(0), V * 2.0 ** -53 * left.sum()
+    target = r * left.sum()
+    assert (cum[tok] >= target - slack).all() and (cum[tok] - left[tok] <= target + slack).all()

@@ -17,7 +17,8 @@
 //   CTA whose range holds the target scans the one warp's share that does.
 //
 // The sums are f64 over exact differences of the inputs, so where they are split does not
-// move a draw except within 1e-15 of a border; u * q and the comparison are f64 as well.
+// move a draw except within 1e-15 of a border, and never to an entry without mass; u * q and the
+// comparison are f64 as well.
 #include "launch.cuh"
 #include "ops.cuh"
 #include "ops.h"
@@ -99,7 +100,8 @@ __device__ int draw_small(const T* p, const T* q, int V, int drafted, double r, 
 #pragma unroll
         for (int i = 0; i < EACH; ++i) {
             before += x[i];
-            if (x[i] > 0.0) last = lo + i;
+            if (!(x[i] > 0.0)) continue;                         // rounding may leave `before` past the target here already
+            last = lo + i;
             if (before > target && first == 0x7fffffff) first = lo + i;
         }
         if (first != 0x7fffffff) atomicMin(&sh.found, first);
@@ -209,11 +211,12 @@ __device__ int draw_large(const T* p, const T* q, int V, int drafted, double r, 
 #pragma unroll
         for (int i = 0; i < EACH; ++i) {
             before += x[i];
-            if (before > target && first == 0x7fffffff) first = tlo + i;
+            if (x[i] > 0.0 && before > target && first == 0x7fffffff) first = tlo + i;
         }
         for (int i = tlo + EACH; i < thi && first == 0x7fffffff; ++i) {
-            before += left_at<T, HAS_Q, SUB>(p, q, i, drafted);
-            if (before > target) first = i;
+            const double y = left_at<T, HAS_Q, SUB>(p, q, i, drafted);
+            before += y;
+            if (y > 0.0 && before > target) first = i;
         }
         atomicMin(&sh.found, first);
     }
