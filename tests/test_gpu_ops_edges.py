@@ -101,3 +101,66 @@ def test_verify_never_draws_a_token_without_mass(V):
     cum, slack = left.cumsum(0), V * 2.0 ** -53 * left.sum()
     target = r * left.sum()
     assert (cum[tok] >= target - slack).all() and (cum[tok] - left[tok] <= target + slack).all()
+
+
+# ------------------------------------------------------------------------- rope_append
+def _three_streams():
+    g = _gen(3)
+    k, v = (torch.randn((8, 4, 1, 32), generator=g).to(F16).to(DEV) for _ in range(2))
+    q, kn, vn = (torch.randn((4, h, 32), generator=g).to(F16).to(DEV) for h in (2, 1, 1))
+    return ops.PagedKV(k, v), _i32([6, 7, 8]), _i32([[0, 1], [2, 3], [4, 5]]), q, kn, vn
+
+
+@pytest.mark.parametrize("off,stored", [
+    # offsets; (row, stream, cache row) of the rows of streams whose own offsets are sound
+    ([0, 1, 2, 5], [(0, 0, 5), (1, 1, 6)]),                  # the last stream ends behind the rows
+    ([0, 1, 9, 12], [(0, 0, 5)]), ([0, 4, 4, 6], [(0, 0, 2), (1, 0, 3), (2, 0, 4), (3, 0, 5)]),
+    ([-1, 1, 2, 3], [(1, 1, 6), (2, 2, 7)]),                 # the first begins ahead of them
+    ([0, 2, 1, 1], []), ([0, 2, 1, 4], [(0, 0, 4), (2, 2, 6), (3, 2, 7)]), ([2, 1, 0, 0], []),      # descending
+    ([0, 1, 2, -5], []), ([0, 9, 9, 9], []), ([-9, -8, -7, -6], []), ([5, 4, 4, 4], []),
+    ([0, 2 ** 31 - 1, 2 ** 31 - 1, 2 ** 31 - 1], []), ([-2 ** 31, 1, 2, 3], [(1, 1, 6), (2, 2, 7)])], ids=str)
+def test_rope_append_bad_offsets(off, stored):
+    """Offsets out of range or descending are recorded; the rows of streams that they belong to turn
+    nothing and store nothing, and no cached row changes but those of the sound streams."""
+    kv, lens, table, q, k, v = _three_streams()
+    want_k, want_v, want_q = kv.k.clone(), kv.v.clone(), torch.full_like(q, 5.0)
+    for t, b, r in stored:
+        page = int(table[b, r // 4])
+        want_k[page, r % 4], want_v[page, r % 4], want_q[t] = k[t], v[t], q[t]
+    for err in (_word(), None):                              # the same rows with and without the word
+        out = torch.full_like(q, 5.0)
+        ops.rope_append(None, kv, q, k, v, _i32(off), lens, table, out=out, err=err)
+        assert torch.equal(kv.k, want_k) and torch.equal(kv.v, want_v) and torch.equal(out, want_q)
+        assert err is None or int(err) == ops.BAD_INDEX
+
+
+def test_rope_append_many_bad_offsets():
+    """One descent among many streams, wherever it lies, is recorded."""
+    B = 300
+    kv = ops.PagedKV(*(torch.zeros((3, 4, 1, 32), dtype=F16, device=DEV) for _ in range(2)))
+    q = torch.zeros((B, 1, 32), dtype=F16, device=DEV)
+    for at in (0, 1, 31, 32, 150, 298, 299):
+        off = torch.arange(B + 1)
+        off[at + 1:] -= 2
+        if at == 0:
+            off[0] = 1
+        off.clamp_(min=0)
+        err = _word()
+        ops.rope_append(None, kv, q, None, None, _i32(off), _i32([4] * B), _i32([[1]] * B), err=err)
+        assert int(err) == (ops.BAD_INDEX if (off[1:] < off[:-1]).any() else 0), at
+
+
+def test_rope_append_rows_ahead_of_the_first_stream():
+    """row_off[0] above 0: the rows ahead of it belong to no stream, which is no fault."""
+    kv, lens, table, q, k, v = _three_streams()
+    was, err, out = kv.k.clone(), _word(), torch.full_like(q, 5.0)
+    ops.rope_append(None, kv, q, k, v, _i32([1, 2, 2, 3]), lens, table, out=out, err=err)
+    ops.check(err)
+    assert (out[0] == 5).all() and (out[3] == 5).all() and torch.equal(out[1:3], q[1:3])
+    was[1, 1], was[5, 3] = k[1], k[2]
+    assert torch.equal(kv.k, was)
+    pages = ops.PagedKV(*(x.reshape(4, 8, 1, 32) for x in (kv.k, kv.v)))        # pages of 8 for the attention
+    o, lse = ops.prefix_attention(pages, q, _i32([1, 2, 2, 3]), lens, _i32([[0], [1], [2]]), out=torch.full_like(q, 5.0),
+                                  lse=torch.full((4, 2), 6.0, device=DEV), err=err)
+    ops.check(err)
+    assert (o[0] == 5).all() and (o[3] == 5).all() and (lse[0] == 6).all() and (lse[3] == 6).all()

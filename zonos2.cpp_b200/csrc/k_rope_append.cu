@@ -72,10 +72,21 @@ __global__ void __launch_bounds__(32 * WARPS) rope_append_ops_kernel(const __gri
     if (t >= p.n_rows) return;
     const int total = p.row_off[p.n_seq];
     const int b = warp_find_seq(p.row_off, p.n_seq, t);
-    const int lo = p.row_off[b], n = p.row_off[b + 1] - lo, len = p.seq_len[b];
-    if (t >= total) return;                                          // padding stays as it is
-    const long long r = (long long)len - n + (t - lo);               // cache row
-    if (t < lo || t - lo >= n || r < 0 || (p.k && r >= (long long)p.max_pages * p.page_len)) {
+    const int lo = p.row_off[b], hi = p.row_off[b + 1], len = p.seq_len[b];
+    if (p.err && t == 0 && blockIdx.y == 0) {                        // offsets that no row need come across
+        bool bad = lane == 0 && (p.row_off[0] < 0 || total > p.n_rows);
+        for (int i = lane; i < p.n_seq; i += 32) bad |= p.row_off[i + 1] < p.row_off[i];
+        if (bad) atomicOr(p.err, Z2B_OPS_BAD_INDEX);
+    }
+    // a stream whose offsets cannot be is left out whole; offsets that descend may still name a row
+    // for a stream whose own are sound
+    if (lo < 0 || hi < lo || hi > total || hi > p.n_rows || (t < lo && b > 0)) {
+        if (lane == 0 && p.err) atomicOr(p.err, Z2B_OPS_BAD_INDEX);
+        return;
+    }
+    if (t < lo || t >= total) return;                                // ahead of the first stream, padding: stays as it is
+    const long long r = (long long)len - (hi - lo) + (t - lo);       // cache row
+    if (t >= hi || r < 0 || (p.k && r >= (long long)p.max_pages * p.page_len)) {
         if (lane == 0 && p.err) atomicOr(p.err, Z2B_OPS_BAD_INDEX);
         return;
     }

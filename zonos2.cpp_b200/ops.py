@@ -8,8 +8,8 @@ tensor of one element on the device that the kernels OR ``BAD_INDEX``, ``BAD_PAG
 ``TIMEOUT`` into; ``check(err)`` reads it (which synchronises) and raises.
 
 Rows are packed over the streams: stream b owns rows [row_off[b], row_off[b + 1]) of q
-[rows][heads][head_dim], rows from row_off[-1] on are padding and stay as they are, seq_len[b]
-counts the stream's cached rows with the new ones, and page_table[b] lists its pages. There is no
+[rows][heads][head_dim], rows ahead of row_off[0] and from row_off[-1] on are padding and stay as they
+are, seq_len[b] counts the stream's cached rows with the new ones, and page_table[b] lists its pages. There is no
 backward pass: inputs that want gradients are refused, and autograd does not see what is written in
 place (the pages, `out`, `lse`).
 """
