@@ -164,3 +164,21 @@ def test_rope_append_rows_ahead_of_the_first_stream():
                                   lse=torch.full((4, 2), 6.0, device=DEV), err=err)
     ops.check(err)
     assert (o[0] == 5).all() and (o[3] == 5).all() and (lse[0] == 6).all() and (lse[3] == 6).all()
+
+
+# ------------------------------------------------------------------------- prefix_attention
+@pytest.mark.parametrize("B,P", [(3, 40), (200, 40), (40, 8800)], ids=str)        # joined by blocks, by warps; tall prefix
+def test_prefix_attention_of_queries_that_are_not_numbers(B, P):
+    """A query with an entry that is not a number has a result and an lse that are not, and no other row does."""
+    g, page = _gen(5), 16
+    np_ = -(-P // page)
+    k, v = (torch.randn((np_ + B, page, 2, 64), generator=g).to(F16).to(DEV) for _ in range(2))
+    q = torch.randn((B, 8, 64), generator=g).to(F16).to(DEV)
+    args = (_i32(range(B + 1)), _i32([5] * B), _i32(range(np_, np_ + B))[:, None], _i32(range(np_)), P)
+    out, lse = ops.prefix_attention(ops.PagedKV(k, v), q, *args, lse=True)
+    q[1, 3, 5] = math.nan
+    got, glse = ops.prefix_attention(ops.PagedKV(k, v), q, *args, lse=True)
+    assert torch.isnan(got[1, 3]).all() and torch.isnan(glse[1, 3])
+    rest = torch.ones((B, 8), dtype=torch.bool, device=DEV)
+    rest[1, 3] = False
+    assert torch.equal(got[rest], out[rest]) and torch.equal(glse[rest], lse[rest])

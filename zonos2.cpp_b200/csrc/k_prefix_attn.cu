@@ -596,7 +596,9 @@ template <int DPL, int HD> __device__ __forceinline__ void load_dims(const float
 
 template <typename T, int DPL, int HD>
 __device__ __forceinline__ void put_row(const JoinP& p, int t, int head, int lane, float M, float L, const float (&acc)[DPL]) {
-    const float inv = L > 0.0f ? 1.0f / L : 0.0f;
+    // a row that saw no key has a sum of 0; one that is not a number (a query's, or a partial result that
+    // is missing) makes all of the row so
+    const float inv = L == 0.0f ? 0.0f : 1.0f / L;
     if (HD >= 32 || lane < HD) {
         T* dst = (T*)p.out + (long long)t * p.o_row + (long long)head * p.o_head + lane * DPL;
         if constexpr (DPL == 1) *dst = from_f32<T>(acc[0] * inv);
@@ -606,7 +608,7 @@ __device__ __forceinline__ void put_row(const JoinP& p, int t, int head, int lan
         }
     }
     // ln(sum) = (M + log2 L) ln 2
-    if (lane == 0 && p.lse) p.lse[(long long)t * (p.a.nkv * p.a.G) + head] = L > 0.0f ? (M + log2f(L)) * 0.6931471805599453f : -INFINITY;
+    if (lane == 0 && p.lse) p.lse[(long long)t * (p.a.nkv * p.a.G) + head] = L == 0.0f ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
 }
 
 // Many rows: a warp per row and four heads. Lane 8 g + k takes the statistics of partial k of
@@ -759,7 +761,7 @@ __global__ void __launch_bounds__(256, 4) prefix_attn_join_few_kernel(const __gr
     if (warp > 0) return;
     for (int w = 1; w < W; ++w) {
         const float top = fmaxf(M, s_acc[w][HD]);
-        if (top == -INFINITY) continue;
+        if (top == -INFINITY) { L += s_acc[w][HD + 1]; continue; }       // no key seen: a sum of 0, or none
         const float f = ex2(M - top), fw = ex2(s_acc[w][HD] - top);
         M = top;
         L = L * f + s_acc[w][HD + 1] * fw;
