@@ -68,6 +68,9 @@ int z2b_test_dequant(uint32_t type, int64_t rows, int64_t k, const void* gguf_ro
  * the device error word it left (DERR_WAIT_TIMEOUT = 1), *elapsed_ns = how long the
  * wait took. No fault, no trap. */
 int z2b_test_wait_timeout(uint32_t polls, uint32_t* err_word, uint32_t* outcome, uint64_t* elapsed_ns);
+/* Limits the waits of z2b_prefix_attention calls from now on to `polls` (0: each gives up at once, as
+ * if its copy or product never came; negative: the usual limit). Process-wide. */
+void z2b_test_attn_wait_polls(int polls);
 int z2b_test_gemv(uint32_t type, int64_t rows, int64_t k, const void* gguf_rows, const uint16_t* x_f16,
                   int n_tok, float* out);
 

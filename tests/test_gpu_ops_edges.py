@@ -182,3 +182,42 @@ def test_prefix_attention_of_queries_that_are_not_numbers(B, P):
     rest = torch.ones((B, 8), dtype=torch.bool, device=DEV)
     rest[1, 3] = False
     assert torch.equal(got[rest], out[rest]) and torch.equal(glse[rest], lse[rest])
+
+
+def _many(B, P, hd=64, nh=8, nkv=2, own=5, dtype=F16, page=16, seed=6):
+    """B decode rows behind one prefix: cache, queries and the arguments after them."""
+    g, np_, per = _gen(seed), -(-P // page), -(-own // page)
+    k, v = (torch.randn((np_ + B * per, page, nkv, hd), generator=g).to(dtype).to(DEV) for _ in range(2))
+    q = torch.randn((B, nh, hd), generator=g).to(dtype).to(DEV)
+    table = torch.arange(np_, np_ + B * per, dtype=torch.int32, device=DEV).reshape(B, per)
+    return ops.PagedKV(k, v), q, (_i32(range(B + 1)), _i32([own] * B), table, _i32(range(np_)), P)
+
+
+@pytest.fixture
+def wait_polls():
+    f = R.lib().z2b_test_attn_wait_polls
+    yield f
+    torch.cuda.synchronize()
+    f(-1)
+
+
+# joined by blocks, by warps; a tall prefix of few and of many units a CTA, with and without own keys
+WAITS = [(2, 40, 64, 5), (3, 0, 32, 900), (200, 40, 128, 5), (40, 6600, 64, 5), (40, 6600, 128, 300), (200, 16000, 128, 40)]
+
+
+@pytest.mark.parametrize("B,P,hd,own", WAITS, ids=str)
+def test_prefix_attention_waits_that_run_out(wait_polls, B, P, hd, own):
+    """Every wait gives up at once: TIMEOUT is recorded, the call ends with its copies and products done,
+    and the next one is right."""
+    kv, q, args = _many(B, P, hd, own=own)
+    want = ops.prefix_attention(kv, q, *args)
+    torch.cuda.synchronize()
+    for _ in range(3):
+        err = _word()
+        wait_polls(0)
+        ops.prefix_attention(kv, q, *args, err=err)
+        wait_polls(-1)
+        assert int(err) == ops.TIMEOUT
+        with pytest.raises(R.Z2BError):
+            ops.check(err)
+        assert torch.equal(ops.prefix_attention(kv, q, *args), want)

@@ -23,6 +23,7 @@
 #include "launch.cuh"
 #include "ops.h"
 #include "prefix_attn.cuh"
+#include "../../include/z2b_tools.h"
 
 namespace z2b {
 namespace {
@@ -331,7 +332,7 @@ __global__ void __launch_bounds__(32 * max_warps(HD), 1) prefix_attn_kernel(cons
             const int key0 = (u - g.unit0) * KU;
             if (key0 >= g.lim_max) { u = end; break; }           // no row of the tile sees the rest
             const int st = it % NS;
-            dead = __any_sync(0xffffffffu, !mbar_wait(&full[st], (it / NS) & 1, p.err));
+            dead = __any_sync(0xffffffffu, !mbar_wait(&full[st], (it / NS) & 1, p.err, p.polls));
             if (dead) break;
             ++it;
             uint8_t* kt = ring + (size_t)st * STAGE;
@@ -799,6 +800,8 @@ size_t up(size_t x) { return (x + 255) & ~(size_t)255; }
 // units: 219 (the early CTAs end last), 214, 182, 181.
 constexpr int PF_LEAVES = 36, OWN_PER_PF = 16;
 
+std::atomic<int> g_polls{-1};           // limit of a wait set by a test, or negative
+
 HostPlan host_plan(const z2b_prefix_attn_args& a) {
     HostPlan h{};
     const int nkv = a.kv->n_head_kv, hd = a.kv->head_dim;
@@ -877,6 +880,8 @@ cudaError_t go_all(const z2b_prefix_attn_args& a, HostPlan h, cudaStream_t s) {
     p.n_rows = a.n_rows; p.n_seq = a.n_seq; p.nkv = c.n_head_kv; p.G = h.G; p.page_len = c.page_len; p.n_pages = c.n_pages;
     p.max_pages = a.max_pages; p.prefix_len = a.prefix_len;
     p.g_mul = (uint32_t)((0x100000000ull + h.G - 1) / h.G);
+    const int polls = g_polls.load(std::memory_order_relaxed);
+    p.polls = polls < 0 ? kMaxWaitPolls : (uint32_t)polls;
     p.scale2 = a.scale * 1.4426950408889634f;
     uint8_t* ws = (uint8_t*)a.workspace;
     p.plan = (int*)ws;
@@ -933,3 +938,5 @@ cudaError_t launch_prefix_attention(const z2b_prefix_attn_args& a, cudaStream_t 
 }
 
 }  // namespace z2b
+
+extern "C" void z2b_test_attn_wait_polls(int polls) { z2b::g_polls.store(polls, std::memory_order_relaxed); }

@@ -185,7 +185,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) prefix_tc_kernel(const __grid_c
 #pragma unroll 1
                 for (int isv = 0; isv < 2 && ok; ++isv) {
                     const int st = it % stages, use = it / stages;
-                    ok = __all_sync(0xffffffffu, use == 0 || wait_ab(&kv_empty[st], (use - 1) & 1, p.err, &s_abort));
+                    ok = __all_sync(0xffffffffu, use == 0 || wait_ab(&kv_empty[st], (use - 1) & 1, p.err, &s_abort, p.polls));
                     if (!ok) break;
                     if (lane == 0) mbar_expect_tx(&kv_full[st], TILE);
                     __syncwarp();
@@ -201,8 +201,9 @@ __global__ void __launch_bounds__(TC_THREADS, 1) prefix_tc_kernel(const __grid_c
                 }
             }
         }
-        // after a wait that ran out, the copies in flight still land in this CTA's memory
-        if (lane == 0 && !ok)
+        // copies in flight land in this CTA's memory, also where another warp's wait has run out and
+        // nobody reads them any more: the CTA outlives them
+        if (lane == 0)
             for (int k = max(0, it - stages); k < it; ++k) mbar_wait(&kv_full[k % stages], (k / stages) & 1, nullptr, 1u << 16);
         __syncwarp();
     } else if (warp == 9) {
@@ -213,7 +214,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) prefix_tc_kernel(const __grid_c
         int segs[2] = {0, 0}, ct[2] = {0, 0};                    // segments and units done of each row tile
         bool ok = true;
         auto wait = [&](uint64_t* bar, int phase) {
-            if (ok) ok = __all_sync(0xffffffffu, wait_ab(bar, phase & 1, p.err, &s_abort));
+            if (ok) ok = __all_sync(0xffffffffu, wait_ab(bar, phase & 1, p.err, &s_abort, p.polls));
             return ok;
         };
         auto scores = [&](int t, int idx, bool last) {           // S_t = Q_t K^T; `last`: K's stage is free after it
@@ -319,7 +320,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) prefix_tc_kernel(const __grid_c
             if (lane == 0) mbar_arrive(&q_full[t]);
             float m = -INFINITY, l = 0.0f;
             for (int i = 0; i < n; ++i, ++c) {
-                ok = __all_sync(0xffffffffu, wait_ab(&s_full[t], ct & 1, p.err, &s_abort));
+                ok = __all_sync(0xffffffffu, wait_ab(&s_full[t], ct & 1, p.err, &s_abort, p.polls));
                 if (!ok) break;
                 ++ct;
                 tc_fence_after();
@@ -328,7 +329,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) prefix_tc_kernel(const __grid_c
                     // V rows behind the last key may hold anything: zero times that is not zero. Each tile
                     // clears them before its go-ahead, whichever comes first.
                     const int vi = 2 * c + 1;
-                    ok = __all_sync(0xffffffffu, wait_ab(&kv_full[vi % stages], (vi / stages) & 1, p.err, &s_abort));
+                    ok = __all_sync(0xffffffffu, wait_ab(&kv_full[vi % stages], (vi / stages) & 1, p.err, &s_abort, p.polls));
                     if (!ok) break;
                     if (row >= keys)
 #pragma unroll
@@ -394,7 +395,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) prefix_tc_kernel(const __grid_c
                 l += x + y;
             }
             if (!ok) break;
-            ok = __all_sync(0xffffffffu, wait_ab(&pv_done[t], (ct - 1) & 1, p.err, &s_abort));
+            ok = __all_sync(0xffffffffu, wait_ab(&pv_done[t], (ct - 1) & 1, p.err, &s_abort, p.polls));
             if (!ok) break;
             tc_fence_after();
             const int slot = seg + (int)blockIdx.x;

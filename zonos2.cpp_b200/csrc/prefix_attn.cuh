@@ -28,6 +28,7 @@ struct AttnP {
     long long q_row, q_head, table_stride;
     const int *row_off, *seq_len, *table, *prefix_pages;
     uint32_t* err;
+    uint32_t polls;                    // limit of a wait
     int n_rows, n_seq, nkv, G, page_len, n_pages, max_pages, prefix_len;
     uint32_t g_mul;                    // ceil(2^32 / G), for quotients by G of numbers x with x G < 2^32
     int box_rows, box_halves;          // rows of one TMA box (a power of two that divides page_len, at most a

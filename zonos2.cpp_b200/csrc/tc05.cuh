@@ -78,8 +78,9 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, float (&v)[16]) {
 }
 
 // Bounded wait that also gives up as soon as another role of the block has given up.
-__device__ __forceinline__ bool wait_ab(uint64_t* bar, uint32_t parity, uint32_t* err, volatile int* ab) {
-    for (uint32_t i = 0; i < kMaxWaitPolls; ++i) {
+__device__ __forceinline__ bool wait_ab(uint64_t* bar, uint32_t parity, uint32_t* err, volatile int* ab,
+                                        uint32_t max_polls = kMaxWaitPolls) {
+    for (uint32_t i = 0; i < max_polls; ++i) {
         if (mbar_try_wait(bar, parity)) return true;
         if (*ab) return false;
     }
