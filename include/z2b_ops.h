@@ -22,7 +22,8 @@
  * or token ids out of range (the row is skipped, the token refused; offsets that descend:
  * z2b_prefix_attention skips every row) and for u_draw outside [0, 1), Z2B_OPS_BAD_PAGE for a
  * page id outside the cache (its keys read as zeros, its rows are not stored),
- * Z2B_OPS_TIMEOUT for a bounded wait that ran out. No input is dereferenced before it is
+ * Z2B_OPS_TIMEOUT for a bounded wait that ran out (the results that needed it are not
+ * numbers, with or without `err`). No input is dereferenced before it is
  * checked, with or without `err`.
  *
  * Rows: stream b of n_seq owns the packed rows [row_off[b], row_off[b+1]) of the n_rows rows

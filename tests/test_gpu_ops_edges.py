@@ -221,3 +221,16 @@ def test_prefix_attention_waits_that_run_out(wait_polls, B, P, hd, own):
         with pytest.raises(R.Z2BError):
             ops.check(err)
         assert torch.equal(ops.prefix_attention(kv, q, *args), want)
+
+
+@pytest.mark.parametrize("B,P,hd,own", WAITS, ids=str)
+def test_prefix_attention_results_of_waits_that_run_out(wait_polls, B, P, hd, own):
+    """What a wait that ran out leaves cannot pass for a result, also without the error word, and whatever
+    the workspace held before."""
+    kv, q, args = _many(B, P, hd, own=own)
+    for _ in range(2):                                       # the second with the first's good partial results
+        wait_polls(0)
+        out, lse = ops.prefix_attention(kv, q, *args, lse=True)
+        wait_polls(-1)
+        assert torch.isnan(out).all() and torch.isnan(lse).all()
+        ops.prefix_attention(kv, q, *args)

@@ -332,8 +332,13 @@ __global__ void __launch_bounds__(32 * max_warps(HD), 1) prefix_attn_kernel(cons
             const int key0 = (u - g.unit0) * KU;
             if (key0 >= g.lim_max) { u = end; break; }           // no row of the tile sees the rest
             const int st = it % NS;
-            dead = __any_sync(0xffffffffu, !mbar_wait(&full[st], (it / NS) & 1, p.err, p.polls));
-            if (dead) break;
+            if (!dead) dead = __any_sync(0xffffffffu, !mbar_wait(&full[st], (it / NS) & 1, p.err, p.polls));
+            if (dead) {                                          // this and the range's other segments: not numbers
+#pragma unroll
+                for (int nb_ = 0; nb_ < NB; ++nb_) l[nb_][0] = l[nb_][1] = NAN;
+                u = end;
+                break;
+            }
             ++it;
             uint8_t* kt = ring + (size_t)st * STAGE;
             const uint32_t ks = smem_u32(kt);
@@ -443,7 +448,6 @@ __global__ void __launch_bounds__(32 * max_warps(HD), 1) prefix_attn_kernel(cons
             __syncwarp();
             copy();
         }
-        if (dead) break;
 
         // ---- the segment's (or the range's) end: one partial result
         const int slot = g.seg + me;

@@ -291,7 +291,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) prefix_tc_kernel(const __grid_c
         const bool q16 = ((reinterpret_cast<uintptr_t>(p.q) | (uintptr_t)(p.q_row * 2) | (uintptr_t)(p.q_head * 2)) & 15) == 0;
         int c = 0, ct = 0;
         bool ok = true;
-        for (int u = u0; u < u1 && ok;) {
+        for (int u = u0; u < u1;) {
             const int seg = u / size, end = min(u1, (seg + 1) * size), unit0 = seg * size + TC_SEG_COST;
             const int n = end - max(u, unit0), key_first = (max(u, unit0) - unit0) * TC_KEYS;
             const int j = seg / p.nkv, h = seg % p.nkv, nl = live_tiles(j, live_rows);
@@ -301,6 +301,9 @@ __global__ void __launch_bounds__(TC_THREADS, 1) prefix_tc_kernel(const __grid_c
             // Q_t: this thread's row, swizzled by 16-byte chunks
             const int r = j * TC_ROWS + t * 128 + row;
             const bool live = r < live_rows;
+            const size_t at = (size_t)(seg + (int)blockIdx.x) * TC_ROWS + t * 128 + row;         // of this row's partial result
+            auto missing = [&] { if (live) p.part_ml[at] = make_float2(NAN, NAN); };            // a wait ran out
+            if (!ok) { missing(); continue; }
             {
                 const T* src = (const T*)p.q + (long long)(r / p.G) * p.q_row + (long long)(h * p.G + r % p.G) * p.q_head;
 #pragma unroll
@@ -394,12 +397,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1) prefix_tc_kernel(const __grid_c
                 un2(add2(sum[0], sum[1]), x, y);
                 l += x + y;
             }
-            if (!ok) break;
-            ok = __all_sync(0xffffffffu, wait_ab(&pv_done[t], (ct - 1) & 1, p.err, &s_abort, p.polls));
-            if (!ok) break;
+            if (ok) ok = __all_sync(0xffffffffu, wait_ab(&pv_done[t], (ct - 1) & 1, p.err, &s_abort, p.polls));
+            if (!ok) { missing(); continue; }
             tc_fence_after();
-            const int slot = seg + (int)blockIdx.x;
-            float* po = p.part_o + ((size_t)slot * TC_ROWS + t * 128 + row) * HD;
+            float* po = p.part_o + at * HD;
 #pragma unroll
             for (int k = 0; k < HD; k += 32) {
                 uint32_t o[32];
@@ -410,7 +411,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) prefix_tc_kernel(const __grid_c
                     for (int e = 0; e < 32; e += 4)
                         *(uint4*)(po + k + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
             }
-            if (live) p.part_ml[(size_t)slot * TC_ROWS + t * 128 + row] = make_float2(m, l);
+            if (live) p.part_ml[at] = make_float2(m, l);
             tc_fence_before();
         }
     }
