@@ -76,7 +76,8 @@ typedef struct z2b_rope {
 
 /* Fill `out`. rot_dim even, 2..Z2B_ROPE_MAX_DIM (the first rot_dim dims of a head turn, the
  * others pass); base > 1; factor > 0, and 1 with SCALE_NONE; orig_ctx > 0 is read with
- * SCALE_BY_PARTS only; SCALE_NTK needs rot_dim > 2. Host only. */
+ * SCALE_BY_PARTS only; SCALE_NTK needs rot_dim > 2. The scaled base and frequencies have to be
+ * finite and the factor on cos and sin positive. Host only. */
 int z2b_rope_init(z2b_rope* out, int rot_dim, int layout, double base, int scaling, double factor, int orig_ctx);
 
 /* ---- paged cache --------------------------------------------------------------------- */

@@ -79,10 +79,12 @@ int z2b_rope_init(z2b_rope* out, int rot_dim, int layout, double base, int scali
     if (scaling == Z2B_ROPE_SCALE_BY_PARTS && orig_ctx <= 0) return bad("rope_init: SCALE_BY_PARTS needs orig_ctx");
     const double two_pi = 6.283185307179586476925286766559;
     if (scaling == Z2B_ROPE_SCALE_NTK) base *= std::pow(factor, (double)rot_dim / (rot_dim - 2));
+    if (!(base > 0.0) || !std::isfinite(base)) return bad("rope_init: the factor takes the base out of range");
     z2b_rope r{};
     r.rot_dim = rot_dim;
     r.layout = layout;
     r.mag = scaling == Z2B_ROPE_SCALE_BY_PARTS ? (float)(0.1 * std::log(factor) + 1.0) : 1.0f;
+    if (!(r.mag > 0.0f)) return bad("rope_init: the factor leaves no positive magnitude");
     for (int i = 0; i < rot_dim / 2; ++i) {
         double w = std::pow(base, -2.0 * i / rot_dim);           // radians per position
         if (scaling == Z2B_ROPE_SCALE_LINEAR) w /= factor;
@@ -92,6 +94,7 @@ int z2b_rope_init(z2b_rope* out, int rot_dim, int layout, double base, int scali
             w = w / factor * (1.0 - keep) + w * keep;
         }
         double t = w / two_pi;
+        if (!std::isfinite(t)) return bad("rope_init: the factor takes a frequency out of range");
         t -= std::floor(t);                                      // whole turns change nothing
         const double top = std::ldexp(t, 64);                    // exact: a power of two
         r.step[i] = top >= 18446744073709551616.0 ? 0 : (uint64_t)top;
