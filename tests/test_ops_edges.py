@@ -34,3 +34,11 @@ def test_rotations_at_the_edge(kw):
     """Factors below 1 and far ones that still have a table."""
     t = ops.Rope(**{"rot_dim": 64, **kw}).table
     assert t.rot_dim == kw.get("rot_dim", 64) and math.isfinite(t.mag) and t.mag > 0
+
+
+@pytest.mark.parametrize("kw", [dict(rot_dim=2 ** 32 + 64), dict(rot_dim=-2 ** 32 + 64), dict(scaling="by_parts", factor=2.0, orig_ctx=2 ** 32 + 8192),
+                                dict(scaling="by_parts", factor=2.0, orig_ctx=2 ** 64)], ids=str)
+def test_rotation_sizes_beyond_32_bits(kw):
+    """Numbers that would wrap to others on their way into C."""
+    with pytest.raises(R.Z2BError):
+        ops.Rope(**{"rot_dim": 64, **kw})

@@ -68,6 +68,8 @@ class Rope:
                  factor: float = 1.0, orig_ctx: int = 0):
         if layout not in _LAYOUT or scaling not in _SCALING:
             _refuse("rope: layout is 'interleaved' or 'half', scaling 'none', 'linear', 'ntk' or 'by_parts'")
+        if not all(0 <= int(x) < 2 ** 31 for x in (rot_dim, orig_ctx)):      # ctypes would wrap them
+            _refuse("rope: rot_dim and orig_ctx are numbers from 0 to 2^31 - 1")
         self.table = RopeTable()
         self._at = ctypes.addressof(self.table)
         f = lib().z2b_rope_init
