@@ -42,3 +42,16 @@ def test_rotation_sizes_beyond_32_bits(kw):
     """Numbers that would wrap to others on their way into C."""
     with pytest.raises(R.Z2BError):
         ops.Rope(**{"rot_dim": 64, **kw})
+
+
+def test_head_numbers_that_32_bits_do_not_divide():
+    """Head numbers are divided by the group size in 32 bits: n_head times the group stays below 2^32.
+    8191 query heads to each of 64 key heads still fit, of 65 they do not."""
+    L = args.library()
+    for nkv, fits in ((64, True), (65, False)):
+        n = 8191 * nkv
+        a = _attn(_view(n_head_kv=nkv, head_dim=16, row_stride=16 * nkv, head_stride=16, page_stride=256 * nkv), n_rows=1, n_seq=1,
+                  n_head=n, q_row=16 * n, q_head=16, o_row=16 * n, o_head=16)
+        assert (L.z2b_prefix_attention_workspace(ctypes.addressof(a)) > 0) == fits
+        if not fits:
+            assert _call("z2b_prefix_attention", a)[0] == UNSUPPORTED

@@ -142,11 +142,12 @@ static const char* check_attn(const z2b_prefix_attn_args& a, int* rc) {
         return "prefix_attention: head_dim must be 16, 32, 64 or 128";
     if (c.page_len % 8) return "prefix_attention: page_len must be a multiple of 8";
     if (a.n_seq > OPS_MAX_SEQ) return "prefix_attention: more than 4096 streams";
-    // unit and slot numbers are 32-bit
+    // unit and slot numbers are 32-bit; rows x heads of a key head, and head numbers, are divided by the
+    // group size G by a 32-bit multiplication that is exact while number x G is below 2^32
     const long long G = a.n_head / c.n_head_kv, tiles = ((long long)a.n_rows * G + 7) / 8;
     const long long own = ((long long)a.max_pages * c.page_len + 31) / 32 + 1, pf = ((long long)a.prefix_len + 31) / 32 + 1;
     if (tiles * c.n_head_kv > (1 << 24) || (long long)a.n_seq * c.n_head_kv > (1 << 24) || own > (1 << 24) || pf > (1 << 24) ||
-        ((long long)a.n_rows + 32) * G * G > 0xffffffffll || ((tiles + a.n_seq) * own + (tiles + 1) * pf) * c.n_head_kv > 0x7fffffffll)
+        ((long long)a.n_rows + 32) * G * G > 0xffffffffll || a.n_head * G > 0xffffffffll || ((tiles + a.n_seq) * own + (tiles + 1) * pf) * c.n_head_kv > 0x7fffffffll)
         return "prefix_attention: too many rows, streams or pages for one call";
     return "";
 }
