@@ -234,3 +234,33 @@ def test_prefix_attention_results_of_waits_that_run_out(wait_polls, B, P, hd, ow
         wait_polls(-1)
         assert torch.isnan(out).all() and torch.isnan(lse).all()
         ops.prefix_attention(kv, q, *args)
+
+
+# ------------------------------------------------------------------------- gradients
+def test_gradients_of_either_mode_are_refused():
+    """A tangent would be lost without a word; so would the gradient of an lse."""
+    from torch.autograd import forward_ad
+    kv, lens, table, q, k, v = _three_streams()
+    pages = ops.PagedKV(*(x.reshape(4, 8, 1, 32) for x in (kv.k, kv.v)))
+    off, eight = _i32([0, 2, 3, 4]), _i32([[0], [1], [2]])
+    p, draft = torch.full((1, 2, 1, 4), 0.25, device=DEV), torch.zeros((1, 1, 1), dtype=torch.int32, device=DEV)
+    u, r = torch.zeros((1, 1, 1), dtype=F64, device=DEV), torch.zeros((1, 2, 1), dtype=F64, device=DEV)
+    calls = [                                                # each with the tensor that carries the tangent
+        (q, lambda x: ops.prefix_attention(pages, x, off, lens, eight)), (q, lambda x: ops.rope_append(None, kv, x, k, v, off, lens, table)),
+        (k, lambda x: ops.rope_append(None, kv, q, x, v, off, lens, table)), (v, lambda x: ops.rope_append(None, kv, q, k, x, off, lens, table)),
+        (q, lambda x: ops.rope_append(None, kv, q, k, v, off, lens, table, out=x)),
+        (q, lambda x: ops.prefix_attention(pages, q, off, lens, eight, out=x)),
+        (torch.zeros((4, 2), device=DEV), lambda x: ops.prefix_attention(pages, q, off, lens, eight, lse=x)),
+        (p, lambda x: ops.verify_drafts(x, None, draft, u, r)), (p[:, :1], lambda x: ops.verify_drafts(p, x, draft, u, r)),
+        (pages.k, lambda x: ops.PagedKV(x, pages.v)), (pages.v, lambda x: ops.PagedKV(pages.k, x))]
+    for x, f in calls:
+        f(x)
+        with forward_ad.dual_level():
+            dual = forward_ad.make_dual(x, torch.ones_like(x))
+            with pytest.raises(R.Z2BError):
+                f(dual)
+            with torch.no_grad(), pytest.raises(R.Z2BError):     # which forward mode does not heed
+                f(dual)
+            f(forward_ad.unpack_dual(dual).primal)
+    with pytest.raises(R.Z2BError):
+        calls[6][1](torch.zeros((4, 2), device=DEV, requires_grad=True))

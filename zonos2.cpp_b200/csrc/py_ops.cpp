@@ -61,8 +61,10 @@ int device_of(const at::Tensor& t, const char* what) {
 void same_device(const at::Tensor& t, int device, const char* what) {
     if (!t.is_cuda() || t.device().index() != device) refuse(std::string(what) + ": not on the call's device");
 }
+// Gradients of either mode; forward mode has no switch to call under, its tensors are taken apart first.
 void no_grad(const at::Tensor& t, const char* what) {
     if (t.requires_grad() && at::GradMode::is_enabled()) refuse(std::string(what) + ": there is no backward pass; call under torch.no_grad()");
+    if (t._fw_grad(0).defined()) refuse(std::string(what) + ": there is no forward-mode gradient; pass the tensor without its tangent");
 }
 
 // A result that the caller gives: no two of its rows or heads may share memory.
@@ -233,7 +235,10 @@ PyObject* prefix_attention(PyObject*, PyObject* const* v, Py_ssize_t n_args) {
         if (want_lse) {
             made_lse = fresh({n, nh}, at::kFloat, a.device);
             a.lse = (float*)made_lse.data_ptr();
-        } else if (v[10] != Py_None && v[10] != Py_False) a.lse = (float*)array(tensor(v[10], "lse"), at::kFloat, {n, nh}, a.device, "lse");
+        } else if (v[10] != Py_None && v[10] != Py_False) {
+            a.lse = (float*)array(tensor(v[10], "lse"), at::kFloat, {n, nh}, a.device, "lse");
+            no_grad(tensor(v[10], "lse"), "lse");
+        }
         a.err = err_word(v[11], a.device);
         a.workspace_bytes = z2b_prefix_attention_workspace(&a);      // 0: the call below says what is wrong with the sizes
         const at::Tensor ws = fresh({(int64_t)a.workspace_bytes}, at::kByte, a.device);

@@ -10,8 +10,8 @@ tensor of one element on the device that the kernels OR ``BAD_INDEX``, ``BAD_PAG
 Rows are packed over the streams: stream b owns rows [row_off[b], row_off[b + 1]) of q
 [rows][heads][head_dim], rows ahead of row_off[0] and from row_off[-1] on are padding and stay as they
 are, seq_len[b] counts the stream's cached rows with the new ones, and page_table[b] lists its pages. There is no
-backward pass: inputs that want gradients are refused, and autograd does not see what is written in
-place (the pages, `out`, `lse`).
+backward pass and no forward-mode gradient: tensors that want one or carry a tangent are refused, and
+autograd does not see what is written in place (the pages, `out`, `lse`).
 """
 from __future__ import annotations
 
@@ -19,6 +19,7 @@ import ctypes
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _ops                      # the compiled binding, built with the library
 from .runtime import Z2BError, lib
@@ -94,7 +95,7 @@ class PagedKV:
             _refuse("kv: f16 or bf16 CUDA tensors are wanted")
         if k.stride(3) != 1 or 0 in k.shape:
             _refuse("kv: the dims of a head must be contiguous, and no size zero")
-        if k.requires_grad or v.requires_grad:
+        if k.requires_grad or v.requires_grad or any(forward_ad.unpack_dual(x).tangent is not None for x in (k, v)):
             _refuse("kv: the pages are written in place, without a gradient")
         self.k, self.v, self.device, self.dtype = k, v, k.device, k.dtype
         self.n_pages, self.page_len, self.n_head_kv, self.head_dim = k.shape
