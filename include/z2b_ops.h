@@ -115,7 +115,8 @@ typedef struct z2b_rope_append_args {
 
 /* Rotate q into q_out and k into the cache, and store v, in one launch. Angles are exact to
  * f32 at any 32-bit position; the products are f32 and rounded once to their destination's
- * type. Of rows that name the same cache row parts of any stay. With k NULL only q turns: the
+ * type. Of rows that name the same cache row parts of any stay. q_out is q itself or apart from q, k and
+ * v, and no two places of q_out, or of the cache that is stored to, share memory. With k NULL only q turns: the
  * pages are not looked at, and max_pages may be 0. */
 int z2b_rope_append(const z2b_rope_append_args* args, void* stream);
 
@@ -145,7 +146,7 @@ typedef struct z2b_prefix_attn_args {
 
 /* out[t] = softmax(scale q[t] . K) V over the prefix_len shared rows and the rows of the
  * stream's own pages up to the row's own; a row that sees none gives zeros and an lse of
- * -infinity. Products of 16-bit operands, sums and softmax statistics in f32, the
+ * -infinity. No two rows or heads of out share memory; it may lie across q. Products of 16-bit operands, sums and softmax statistics in f32, the
  * probabilities rounded to the cache's type for their product with V. Cache rows at or
  * behind seq_len and prefix_len may hold anything; those before must be finite. The result
  * does not depend on timing: the same call gives the same bits. */

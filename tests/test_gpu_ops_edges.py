@@ -264,3 +264,34 @@ def test_gradients_of_either_mode_are_refused():
             f(forward_ad.unpack_dual(dual).primal)
     with pytest.raises(R.Z2BError):
         calls[6][1](torch.zeros((4, 2), device=DEV, requires_grad=True))
+
+
+# ------------------------------------------------------------------------- shared memory
+def test_tensors_that_share_memory():
+    """What rope_append writes shares no memory with what it reads or writes beside it; slices of one buffer
+    pass, and pages that are only read may be anything."""
+    g = _gen(9)
+    kv, lens, table, q, k, v = _three_streams()
+    meta = (_i32([0, 2, 3, 4]), lens, table)
+    buf = torch.randn(4096, generator=g).to(F16).to(DEV)
+    pages = buf[:2048].view(8, 2, 4, 1, 32)
+    one = ops.PagedKV(pages[:, 0], pages[:, 1])              # keys and values by turns
+    for f in (lambda: ops.rope_append(None, kv, q, None, None, *meta, out=buf.as_strided((4, 2, 32), (48, 32, 1))),
+              lambda: ops.rope_append(None, kv, buf[:256].view(4, 2, 32), None, None, *meta, out=buf[64:320].view(4, 2, 32)),
+              lambda: ops.rope_append(None, kv, q, buf[:128].view(4, 1, 32), v, *meta, out=buf[:256].view(4, 2, 32)),
+              lambda: ops.rope_append(None, ops.PagedKV(kv.k, kv.k), q, k, v, *meta),
+              lambda: ops.rope_append(None, ops.PagedKV(*(buf[x:x + 1024].view(8, 4, 1, 32) for x in (0, 32))), q, k, v, *meta),
+              lambda: ops.rope_append(None, ops.PagedKV(*(x[:1].expand(8, -1, -1, -1) for x in (kv.k, kv.v))), q, k, v, *meta)):
+        with pytest.raises(R.Z2BError):
+            f()
+    want = ops.rope_append(ops.Rope(32), kv, q, k, v, *meta)
+    fused = torch.cat((q, k, v), 1)                          # rows of [q | k | v], q turned in place
+    got = ops.rope_append(ops.Rope(32), one, fused[:, :2], fused[:, 2:3], fused[:, 3:], *meta, out=fused[:, :2])
+    assert torch.equal(got, want) and torch.equal(fused[:, 2:3], k)
+    for b, r in ((0, 4), (0, 5), (1, 6), (2, 7)):
+        at = int(table[b, r // 4]), r % 4
+        assert torch.equal(one.k[at], kv.k[at]) and torch.equal(one.v[at], kv.v[at])
+    same = ops.PagedKV(*(x.reshape(4, 8, 1, 32)[:1].expand(4, -1, -1, -1) for x in (kv.k, kv.k)))
+    a = ops.prefix_attention(same, q, meta[0], lens, _i32([[0], [1], [2]]))
+    b = ops.prefix_attention(ops.PagedKV(*(same.k.contiguous() for _ in range(2))), q, meta[0], lens, _i32([[0], [1], [2]]))
+    assert torch.equal(a, b)

@@ -55,3 +55,70 @@ def test_head_numbers_that_32_bits_do_not_divide():
         assert (L.z2b_prefix_attention_workspace(ctypes.addressof(a)) > 0) == fits
         if not fits:
             assert _call("z2b_prefix_attention", a)[0] == UNSUPPORTED
+
+
+# ------------------------------------------------------------------------- shared memory
+NO_DEVICE = 1 << 20                 # what is not refused ends at the device, which is not there
+
+
+def _elements(at, dims):
+    """Element numbers of a box as a list."""
+    out = [at]
+    for stride, n in dims:
+        out = [x + stride * i for x in out for i in range(n)]
+    return out
+
+
+def _append_boxes(q, o, k, v, kc, vc, kv_strides, rows=3, heads=2, nkv=2, hd=4, pages=2, page_len=3):
+    """rope_append with arrays (first element, row stride, head stride) of f16 in one address space of
+    elements, the cache's two (first element) with strides (page, row, head)."""
+    at = lambda e: (1 << 30) + 2 * e  # noqa: E731
+    ps, rs, hs = kv_strides
+    view = ops.PagedKVView(k=at(kc), v=at(vc), type=1, n_pages=pages, page_len=page_len, n_head_kv=nkv, head_dim=hd,
+                           page_stride=ps, row_stride=rs, head_stride=hs)
+    a = args.RopeAppendArgs(device=NO_DEVICE, type=1, n_rows=rows, n_seq=1, n_head=heads, kv=ctypes.addressof(view), q=at(q[0]),
+                            q_out=at(o[0]), k=at(k[0]), v=at(v[0]), q_row=q[1], q_head=q[2], o_row=o[1], o_head=o[2], k_row=k[1],
+                            k_head=k[2], v_row=v[1], v_head=v[2], row_off=BUF, seq_len=BUF, page_table=BUF, table_stride=2, max_pages=2)
+    rc, msg = _call("z2b_rope_append", a)
+    qe, oe = (_elements(x[0], [(x[1], rows), (x[2], heads), (1, hd)]) for x in (q, o))
+    ke, ve = (_elements(x[0], [(x[1], rows), (x[2], nkv), (1, hd)]) for x in (k, v))
+    ce, de = (_elements(x, [(ps, pages), (rs, page_len), (hs, nkv), (1, hd)]) for x in (kc, vc))
+    shared = len(set(oe)) < len(oe) or (qe != oe and set(qe) & set(oe)) or set(oe) & set(ke + ve) or len(set(ce)) < len(ce) or set(ce) & set(de)
+    return rc, msg, bool(shared)
+
+
+def test_append_refuses_shared_memory_and_nothing_else():
+    """Against a count of the elements themselves: boxes at random places and strides, nested and not."""
+    import random
+    rng = random.Random(5)
+    seen = {True: 0, False: 0}
+    for n in range(4000):
+        pick = lambda far: (rng.randrange(far), rng.choice((0, 4, 5, 8, 12, 16, 24, 40, 100)), rng.choice((0, 3, 4, 8, 12, 13, 50)))  # noqa: E731
+        q = (rng.randrange(40), rng.choice((8, 16, 24, 32)), rng.choice((4, 8, 12, 24)))
+        o = q if n % 4 == 0 else pick(120) if n % 4 == 1 else (q[0] + rng.randrange(-8, 300), q[1], q[2])
+        k, v = ((rng.randrange(60, 400), q[1], 4) for _ in range(2))
+        cache = rng.choice(((24, 8, 4), (48, 16, 4), (24, 4, 12), (48, 8, 4), (20, 8, 4), (0, 8, 4), (7, 21, 4), (26, 9, 4), (9, 18, 4)))
+        rc, msg, shared = _append_boxes(q, o, k, v, 1000, 1000 + rng.choice((0, 4, 8, 12, 24, 48, 100, -24, 23)), cache)
+        seen[shared] += 1
+        assert (rc == ARG) == shared, (q, o, k, v, cache, msg)
+        assert not shared or "share memory" in msg or "lies across" in msg
+    assert min(seen.values()) > 300
+
+
+def test_append_takes_slices_of_one_buffer():
+    """q turned in place, k and v beside it, and keys and values of one cache buffer in turn: by page, by row, by head."""
+    q, k, v = (0, 24, 4), (8, 24, 4), (16, 24, 4)
+    for cache, apart in (((48, 8, 4), 24), ((48, 16, 4), 8), ((48, 16, 8), 4), ((24, 8, 4), 48)):
+        rc, msg, shared = _append_boxes(q, q, k, v, 1000, 1000 + apart, cache)
+        assert not shared and rc != ARG, msg
+
+
+def test_attention_refuses_results_that_share_memory():
+    view = dict(n_head_kv=2, head_dim=64)
+    for (row, head), ok in (((256, 64), True), ((64, 192), True), ((192, 128), True), ((128, 64), True), ((96, 64), False), ((64, 128), False), ((0, 64), False), ((256, 32), False)):
+        a = _attn(_view(**view), device=NO_DEVICE, n_rows=3, n_head=2, o_row=row, o_head=head, workspace_bytes=1 << 40)
+        rc, msg = _call("z2b_prefix_attention", a)
+        assert (rc == ARG) == (not ok), (row, head, msg)
+    # the keys may be the values there, and pages may repeat: they are only read
+    a = _attn(_view(page_stride=0, **view), device=NO_DEVICE, workspace_bytes=1 << 40)
+    assert _call("z2b_prefix_attention", a)[0] != ARG

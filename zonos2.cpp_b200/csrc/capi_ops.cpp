@@ -6,7 +6,9 @@
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
+#include <initializer_list>
 #include <string>
+#include <utility>
 
 using namespace z2b;
 
@@ -41,6 +43,92 @@ int launched(cudaError_t e, const char* op) {
 bool aligned(const void* p, unsigned n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 unsigned type_size(int t) { return t == Z2B_TYPE_F32 ? 4 : 2; }
 bool act_type(int t) { return t == Z2B_TYPE_F32 || t == Z2B_TYPE_F16 || t == Z2B_TYPE_BF16; }
+
+// ---- shared memory. An array is a box of elements at sum of i_d * stride_d, 0 <= i_d < n_d; two of
+// its elements, or elements of two arrays, are the same where the differences x_d of their indices
+// solve sum of stride_d x_d = delta. The strides of usual arrays nest (each is at least what the smaller
+// ones span), which leaves a candidate or two per dim; others are searched, up to a limit.
+struct Var { long long stride, lo, hi; };       // a difference of indices and its range
+
+// Whether var[0..n) (strides descending, positive) reach delta. Out of `steps`: taken as no.
+bool reaches(const Var* v, int n, long long delta, int* steps) {
+    if (n == 0) return delta == 0;
+    long long lo = 0, hi = 0;                    // what the later ones span
+    for (int i = 1; i < n; ++i) { lo += v[i].stride * v[i].lo; hi += v[i].stride * v[i].hi; }
+    const long long s = v->stride, a = delta - hi, b = delta - lo;
+    long long x = a > 0 ? (a + s - 1) / s : -(-a / s), end = b >= 0 ? b / s : -((-b + s - 1) / s);
+    x = std::max(x, v->lo);
+    end = std::min(end, v->hi);
+    for (; x <= end; ++x) {
+        if (--*steps < 0) return false;
+        if (reaches(v + 1, n - 1, delta - s * x, steps)) return true;
+    }
+    return false;
+}
+
+struct Box {
+    const void* p;
+    int n = 0;
+    long long stride[4], len[4], last = 0;       // last: offset of the last element
+    bool real = true;                            // false: it ends beyond any address, there is nothing to compare
+    Box(const void* p_, std::initializer_list<std::pair<long long, long long>> dims) : p(p_) {
+        __int128 end = 0;
+        for (const auto& d : dims) {
+            if (d.second <= 1) continue;         // a dim of one has no stride
+            stride[n] = d.first;
+            len[n++] = d.second;
+            end += (__int128)d.first * (d.second - 1);
+        }
+        real = end >= 0 && end < 1ll << 56;
+        if (real) last = (long long)end;
+    }
+    bool same_place(const Box& o) const {
+        return p == o.p && n == o.n && std::equal(stride, stride + n, o.stride) && std::equal(len, len + n, o.len);
+    }
+};
+bool steeper(const Var& a, const Var& b) { return a.stride > b.stride; }
+
+// Some element has two indices.
+bool shares_itself(const Box& b) {
+    Var v[4];
+    for (int i = 0; i < b.n; ++i) {
+        if (b.stride[i] <= 0) return true;
+        v[i] = Var{b.stride[i], 1 - b.len[i], b.len[i] - 1};
+    }
+    if (!b.real) return false;
+    std::sort(v, v + b.n, steeper);
+    long long span = 0;
+    bool nest = true;
+    for (int i = b.n - 1; i >= 0; --i) { nest &= v[i].stride > span; span += v[i].stride * v[i].hi; }
+    if (nest) return false;
+    int steps = 1 << 16;
+    for (int i = 0; i < b.n; ++i) {              // the first dim in which the two indices differ
+        const Var all = v[i];
+        v[i].lo = 1;
+        if (reaches(v + i, b.n - i, 0, &steps)) return true;
+        v[i] = all;
+    }
+    return false;
+}
+
+// Some element of one is an element of the other; both of `size` bytes an element, aligned to it.
+bool share(const Box& a, const Box& b, int size) {
+    const long long d = (long long)((uintptr_t)b.p - (uintptr_t)a.p) / size;
+    if (!a.real || !b.real || d > a.last || -d > b.last) return false;
+    Var v[8];
+    int n = 0;
+    for (int i = 0; i < a.n; ++i) if (a.stride[i] > 0) v[n++] = Var{a.stride[i], 0, a.len[i] - 1};
+    for (int i = 0; i < b.n; ++i) {
+        if (b.stride[i] <= 0) continue;          // an input's dim without a stride stays where it is
+        int j = 0;
+        while (j < n && v[j].stride != b.stride[i]) ++j;
+        if (j == n) v[n++] = Var{b.stride[i], 0, 0};
+        v[j].lo -= b.len[i] - 1;                 // equal strides: one difference
+    }
+    std::sort(v, v + n, steeper);
+    int steps = 1 << 16;
+    return reaches(v, n, d, &steps);
+}
 
 // What both cache operators ask of the view; empty when it is sound.
 const char* check_kv(const z2b_paged_kv* c) {
@@ -125,6 +213,22 @@ int z2b_rope_append(const z2b_rope_append_args* args, void* stream) {
     if (a.n_rows == 0 || a.n_seq == 0 || (a.n_head == 0 && !a.k)) return Z2B_OK;
     m = check_rows(a.n_seq, a.row_off, a.seq_len, a.page_table, a.table_stride, a.max_pages);
     if (*m) return bad(m);
+    // rows are turned and stored at the same time, in any order
+    const z2b_paged_kv& c = *a.kv;
+    const Box out(a.n_head ? a.q_out : nullptr, {{a.o_row, a.n_rows}, {a.o_head, a.n_head}, {1, c.head_dim}});
+    if (out.p) {
+        const Box q(a.q, {{a.q_row, a.n_rows}, {a.q_head, a.n_head}, {1, c.head_dim}});
+        if (shares_itself(out)) return bad("rope_append: rows or heads of q_out share memory");
+        if (!out.same_place(q) && share(out, q, e)) return bad("rope_append: q_out lies across q");
+    }
+    if (a.k) {
+        const Box k(a.k, {{a.k_row, a.n_rows}, {a.k_head, c.n_head_kv}, {1, c.head_dim}});
+        const Box v(a.v, {{a.v_row, a.n_rows}, {a.v_head, c.n_head_kv}, {1, c.head_dim}});
+        if (out.p && (share(out, k, e) || share(out, v, e))) return bad("rope_append: q_out lies across k or v");
+        const Box kc(c.k, {{c.page_stride, c.n_pages}, {c.row_stride, c.page_len}, {c.head_stride, c.n_head_kv}, {1, c.head_dim}});
+        const Box vc(c.v, {{c.page_stride, c.n_pages}, {c.row_stride, c.page_len}, {c.head_stride, c.n_head_kv}, {1, c.head_dim}});
+        if (shares_itself(kc) || share(kc, vc, 2)) return bad("rope_append: pages, rows, heads or keys and values of the cache share memory");
+    }
     DeviceGuard g(a.device);
     if (g.rc != cudaSuccess) return launched(g.rc, "rope_append: device: ");
     return launched(launch_rope_append(a, (cudaStream_t)stream), "rope_append: ");
@@ -180,6 +284,8 @@ int z2b_prefix_attention(const z2b_prefix_attn_args* args, void* stream) {
     if (a.prefix_len > 0 && !a.prefix_pages) return bad("prefix_attention: null prefix_pages");
     if (!a.workspace || !aligned(a.workspace, 16)) return bad("prefix_attention: the workspace must be 16-byte aligned");
     if (a.workspace_bytes < prefix_attention_bytes(a)) return bad("prefix_attention: the workspace is too small");
+    if (shares_itself(Box(a.out, {{a.o_row, a.n_rows}, {a.o_head, a.n_head}, {1, c.head_dim}})))
+        return bad("prefix_attention: rows or heads of out share memory");
     DeviceGuard g(a.device);
     if (g.rc != cudaSuccess) return launched(g.rc, "prefix_attention: device: ");
     return launched(launch_prefix_attention(a, (cudaStream_t)stream), "prefix_attention: ");

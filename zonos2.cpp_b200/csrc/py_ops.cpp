@@ -67,13 +67,6 @@ void no_grad(const at::Tensor& t, const char* what) {
     if (t._fw_grad(0).defined()) refuse(std::string(what) + ": there is no forward-mode gradient; pass the tensor without its tangent");
 }
 
-// A result that the caller gives: no two of its rows or heads may share memory.
-void result(const at::Tensor& t, const char* what) {
-    no_grad(t, what);
-    for (int64_t d = 0; d + 1 < t.dim(); ++d)
-        if (t.size(d) > 1 && t.stride(d) == 0) refuse(std::string(what) + ": rows or heads share memory");
-}
-
 // A contiguous array of `dtype` and that shape.
 void* array(const at::Tensor& t, at::ScalarType dtype, at::IntArrayRef shape, int device, const char* what) {
     same_device(t, device, what);
@@ -164,7 +157,7 @@ PyObject* rope_append(PyObject*, PyObject* const* v, Py_ssize_t n_args) {
                 out = &made;
             }
             a.q_out = rows(*out, n, a.n_head, hd, dt, a.device, "out", &a.o_row, &a.o_head);
-            result(*out, "out");
+            no_grad(*out, "out");
         } else if (out) refuse("rope_append: out without q");
         if (k) {
             no_grad(*k, "k");
@@ -230,7 +223,7 @@ PyObject* prefix_attention(PyObject*, PyObject* const* v, Py_ssize_t n_args) {
             out = &made;
         }
         a.out = rows(*out, n, nh, hd, dt, a.device, "out", &a.o_row, &a.o_head);
-        result(*out, "out");
+        no_grad(*out, "out");
         const bool want_lse = v[10] == Py_True;
         if (want_lse) {
             made_lse = fresh({n, nh}, at::kFloat, a.device);

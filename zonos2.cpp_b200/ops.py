@@ -86,7 +86,8 @@ class Rope:
 
 class PagedKV:
     """The K and V pages of one layer: tensors [pages][page_len][kv heads][head_dim] (any strides
-    with the dims of a head together), f16 or bf16, of the same strides."""
+    with the dims of a head together), f16 or bf16, of the same strides. What rope_append stores to must
+    not share memory: neither keys with values nor expanded pages."""
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor):
         if k.dim() != 4 or k.shape != v.shape or k.stride() != v.stride() or k.dtype != v.dtype or k.device != v.device:
@@ -114,7 +115,7 @@ class PagedKV:
 def rope_append(rope: Rope | None, kv: PagedKV, q, k, v, row_off, seq_len, page_table, prefix_len: int = 0, pos=None,
                 out=None, err=None):
     """Rotate q and k and append k and v to the pages (z2b_rope_append); returns the rotated q
-    (`out` when given, which may be q). q may be None (nothing returned), k and v may be None (only
+    (`out` when given, which may be q, or lie apart from q, k and v). q may be None (nothing returned), k and v may be None (only
     q turns); rope None stores unrotated keys. `pos` [rows] int32 replaces the positions prefix_len +
     cache row. A new result is contiguous, and its padding rows are not written."""
     return _rope_append(rope._at if rope is not None else 0, kv._at, kv._idx, q, k, v, row_off, seq_len, page_table, prefix_len,
