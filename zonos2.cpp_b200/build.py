@@ -7,7 +7,8 @@ libz2b_synth.so  host-only synthetic GGUF writer (include/z2b_tools.h).
 _ops.so          the Python binding of include/z2b_ops.h for torch tensors (module z2b._ops, used
                  by z2b.ops); the one part compiled against torch, left out where there is none.
 
-Objects go to zonos2.cpp_b200/_build/ and are rebuilt when a source or header is newer.
+Objects go to zonos2.cpp_b200/_build/ and are rebuilt when a source or header is newer, _ops.so also
+when torch or the interpreter changes.
 """
 from __future__ import annotations
 
@@ -103,18 +104,31 @@ def build_z2b(verbose=False):
     return LIB
 
 
+def _torch_key(torch):
+    """What _ops.so is bound to besides its sources: the torch build and the interpreter."""
+    with open(os.path.join(torch, "version.py")) as f:
+        return sys.implementation.cache_tag + "\n" + torch + "\n" + f.read()
+
+
 def build_ops():
     spec = importlib.util.find_spec("torch")
     if spec is None:
         return None
-    src = os.path.join(CSRC, "py_ops.cpp")
-    if _stale(OPS_LIB, [src, os.path.join(INCLUDE, "z2b_ops.h")]):
-        torch = spec.submodule_search_locations[0]
+    src, stamp = os.path.join(CSRC, "py_ops.cpp"), os.path.join(BUILD, "ops.torch")
+    torch = spec.submodule_search_locations[0]
+    key, had = _torch_key(torch), None
+    if os.path.exists(stamp):
+        with open(stamp) as f:
+            had = f.read()
+    if had != key or _stale(OPS_LIB, [src, os.path.join(INCLUDE, "z2b_ops.h")]):
         libs = os.path.join(torch, "lib")
         _run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-I" + os.path.join(torch, "include"),
               "-I" + os.path.join(torch, "include", "torch", "csrc", "api", "include"), "-I/usr/local/cuda/include",
               "-I" + sysconfig.get_paths()["include"], src, "-o", OPS_LIB, "-L" + libs, "-ltorch_python", "-ltorch",
               "-ltorch_cpu", "-lc10", "-lc10_cuda", "-ltorch_cuda", "-L" + PKG, "-lz2b", "-Wl,-rpath,$ORIGIN"])
+        os.makedirs(BUILD, exist_ok=True)
+        with open(stamp, "w") as f:
+            f.write(key)
     return OPS_LIB
 
 
