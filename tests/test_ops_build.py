@@ -60,3 +60,12 @@ def test_a_build_that_failed_is_tried_again(made, monkeypatch):
     monkeypatch.setattr(B, "_run", good)
     B.build_ops()
     assert len(ran) == 2
+
+
+def test_no_torch_with_cuda_no_binding(made, monkeypatch):
+    """The rest of the library builds without torch, and beside one that has no CUDA."""
+    torch, ran = made
+    os.remove(torch / "lib" / "libtorch_cuda.so")
+    assert B.build_ops() is None
+    monkeypatch.setattr(B.importlib.util, "find_spec", lambda name: None)
+    assert B.build_ops() is None and not ran

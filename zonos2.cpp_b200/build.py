@@ -5,7 +5,7 @@ libz2b.so        the decode-step library: GGUF loader, tile repack, sm_100a kern
                  (include/z2b_dac.h).
 libz2b_synth.so  host-only synthetic GGUF writer (include/z2b_tools.h).
 _ops.so          the Python binding of include/z2b_ops.h for torch tensors (module z2b._ops, used
-                 by z2b.ops); the one part compiled against torch, left out where there is none.
+                 by z2b.ops); the one part compiled against torch, left out where there is none with CUDA.
 
 Objects go to zonos2.cpp_b200/_build/ and are rebuilt when a source or header is newer, _ops.so also
 when torch or the interpreter changes.
@@ -116,6 +116,8 @@ def build_ops():
         return None
     src, stamp = os.path.join(CSRC, "py_ops.cpp"), os.path.join(BUILD, "ops.torch")
     torch = spec.submodule_search_locations[0]
+    if not os.path.exists(os.path.join(torch, "lib", "libtorch_cuda.so")):
+        return None                     # a torch without CUDA has no tensors for it
     key, had = _torch_key(torch), None
     if os.path.exists(stamp):
         with open(stamp) as f:
