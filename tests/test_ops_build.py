@@ -69,3 +69,20 @@ def test_no_torch_with_cuda_no_binding(made, monkeypatch):
     assert B.build_ops() is None
     monkeypatch.setattr(B.importlib.util, "find_spec", lambda name: None)
     assert B.build_ops() is None and not ran
+
+
+def test_a_missing_binding_says_what_to_do(monkeypatch):
+    import importlib
+    import sys
+
+    pytest.importorskip("torch")
+    import z2b
+    import z2b.ops as was
+
+    monkeypatch.setitem(sys.modules, "z2b._ops", None)       # an import of it fails
+    monkeypatch.delattr(z2b, "_ops")
+    monkeypatch.delitem(sys.modules, "z2b.ops")
+    with pytest.raises(ImportError, match="build.py ops"):
+        importlib.import_module("z2b.ops")
+    monkeypatch.undo()
+    assert importlib.import_module("z2b.ops") is was

@@ -21,7 +21,11 @@ import math
 import torch
 from torch.autograd import forward_ad
 
-from . import _ops                      # the compiled binding, built with the library
+try:
+    from . import _ops                  # the compiled binding, built with the library
+except ImportError as e:
+    raise ImportError(f"z2b.ops: its compiled binding _ops.so is missing or was built against another torch ({e}); "
+                      "build it with `python zonos2.cpp_b200/build.py ops`") from e
 from .runtime import Z2BError, lib
 
 TIMEOUT, BAD_INDEX, BAD_PAGE = 1, 2, 4
