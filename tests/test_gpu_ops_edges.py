@@ -295,3 +295,259 @@ def test_tensors_that_share_memory():
     a = ops.prefix_attention(same, q, meta[0], lens, _i32([[0], [1], [2]]))
     b = ops.prefix_attention(ops.PagedKV(*(same.k.contiguous() for _ in range(2))), q, meta[0], lens, _i32([[0], [1], [2]]))
     assert torch.equal(a, b)
+
+
+# ------------------------------------------------------------------------- large calls against 64 bits
+class Paged:
+    """Streams of uneven lengths with pages in random order behind one prefix, on the device: the pages a
+    stream does not need have ids out of range, cache rows that no stream has are not numbers."""
+
+    def __init__(self, counts, lens, page, nkv, hd, dtype, prefix, ahead=0, pad=0, seed=0):
+        g = _gen(seed)
+        need = [-(-n // page) for n in lens]
+        np_, B = -(-prefix // page), len(counts)
+        order = torch.randperm(sum(need) + np_ + 2, generator=g).to(torch.int32)
+        self.table = torch.full((B, max([*need, 1])), -1, dtype=torch.int32)
+        at = np_
+        for b, n in enumerate(need):
+            self.table[b, :n] = order[at: at + n]
+            at += n
+        self.shared, self.prefix, self.page = order[:np_], prefix, page
+        dg = torch.Generator(device=DEV)
+        dg.manual_seed(seed)
+        k, v = (torch.randn((len(order), page, nkv, hd), generator=dg, device=DEV).to(dtype) for _ in range(2))
+        for pages, n in [(self.shared, prefix)] + [(self.table[b, :m], lens[b]) for b, m in enumerate(need)]:
+            if n % page:
+                k[pages[-1], n % page:] = math.nan
+                v[pages[-1], n % page:] = math.nan
+        self.kv, self.lens, self.counts = ops.PagedKV(k, v), list(lens), list(counts)
+        self.off = [ahead]
+        for n in counts:
+            self.off.append(self.off[-1] + n)
+        self.rows = self.off[-1] + pad
+        self.args = (_i32(self.off), _i32(lens), self.table.to(DEV), self.shared.to(DEV), prefix)
+
+    def queries(self, nh, seed=1, by=1.5):
+        g = torch.Generator(device=DEV)
+        g.manual_seed(seed)
+        return (torch.randn((self.rows, nh, self.kv.head_dim), generator=g, device=DEV) * by).to(self.kv.dtype)
+
+    def exact(self, q, scale):
+        """out, lse, sum of p |v|, largest sum of |q k| scale, in 64 bits; rows of no stream are 5."""
+        nkv, hd = self.kv.n_head_kv, self.kv.head_dim
+        G = q.shape[1] // nkv
+        out, lse, spread = (torch.full(s, 5.0, dtype=F64, device=DEV) for s in (q.shape, q.shape[:2], q.shape))
+        most, pk, pv = 0.0, *self._rows(self.shared, self.prefix)
+        for b, n in enumerate(self.counts):
+            if n == 0:
+                continue
+            lo, L = self.off[b], self.lens[b]
+            if self.prefix + L == 0:
+                out[lo: lo + n], spread[lo: lo + n], lse[lo: lo + n] = 0.0, 0.0, -math.inf
+                continue
+            ok, ov = self._rows(self.table[b], L)
+            k, v = torch.cat((pk, ok), 1), torch.cat((pv, ov), 1)             # [nkv][keys][hd]
+            x = q[lo: lo + n].double().reshape(n, nkv, G, hd).permute(1, 0, 2, 3).reshape(nkv, n * G, hd)
+            most = max(most, float((x.abs() @ k.abs().transpose(1, 2)).max()) * abs(scale))
+            s = (x @ k.transpose(1, 2)).reshape(nkv, n, G, -1) * scale
+            sees = torch.arange(k.shape[1], device=DEV)[None] < self.prefix + L - n + 1 + torch.arange(n, device=DEV)[:, None]
+            s = s.masked_fill(~sees[None, :, None], -math.inf)
+            p = torch.softmax(s, -1).nan_to_num(0.0).reshape(nkv, n * G, -1)      # a row that sees no key: zeros
+            back = lambda y: y.reshape(nkv, n, G, -1).permute(1, 0, 2, 3).reshape(n, nkv * G, -1)  # noqa: E731
+            out[lo: lo + n], spread[lo: lo + n] = back(p @ v), back(p @ v.abs())
+            lse[lo: lo + n] = back(torch.logsumexp(s, -1)[..., None])[..., 0]
+        return out, lse, spread, most
+
+    def _rows(self, pages, n):
+        p = pages[: -(-n // self.page)].long().to(DEV)
+        return (x[p].flatten(0, 1)[:n].double().transpose(0, 1) for x in (self.kv.k, self.kv.v))
+
+    def check(self, q, out, lse, scale=None):
+        """Every row. Each probability rounded by half a step of the type (eps / 2) for its product with V, the
+        result by half a step again; scores off by 2 hd 2^-24 of sum |q k| (f32 sums, doubled for the tensor
+        cores' alignment), which moves a probability by that much twice (numerator and sum); 2^-18 for ex2,
+        the joins and the division; a probability below the type's normal range by half its smallest step."""
+        scale = self.kv.head_dim ** -0.5 if scale is None else scale
+        want, wlse, spread, most = self.exact(q, scale)
+        dt = self.kv.dtype
+        half, delta = torch.finfo(dt).eps / 2, 4 * self.kv.head_dim * 2.0 ** -24 * most + 2.0 ** -18
+        tol = (half + delta) * spread + half * want.abs() + torch.finfo(dt).smallest_normal
+        off = (out.double() - want).abs() - tol
+        assert torch.isfinite(out).all() and (off <= 0).all(), float(off.max())
+        empty = wlse == -math.inf
+        assert torch.equal(lse == -math.inf, empty)
+        assert ((lse.double() - wlse).abs()[~empty] <= delta + wlse.abs()[~empty] * 2.0 ** -22).all()
+
+
+def _attend(s, q, scale=None):
+    out, lse, err = torch.full_like(q, 5.0), torch.full(q.shape[:2], 5.0, device=DEV), _word()
+    ops.prefix_attention(s.kv, q, *s.args, scale=scale, out=out, lse=lse, err=err)
+    ops.check(err)
+    return out, lse
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=str)
+@pytest.mark.parametrize("hd", [16, 32, 64, 128])
+@pytest.mark.parametrize("nh,nkv,prefix", [(7, 7, 40), (6, 2, 300), (16, 4, 0)], ids=str)
+def test_join_of_many_rows(hd, dtype, nh, nkv, prefix):
+    """More rows x heads than are joined by blocks, head counts that four do not divide, and a stream so much
+    longer than the others that its heads are spread over many partial results."""
+    B = -(-900 // nh) + 3
+    counts = [1 + (b % 11 == 5) for b in range(B)]
+    lens = [2 + 7 * b % 90 for b in range(B)]
+    lens[B // 2], lens[3] = 20011, 0 if counts[3] == 1 else 1
+    s = Paged(counts, lens, 16, nkv, hd, dtype, prefix, ahead=1, pad=2, seed=hd + nh)
+    q = s.queries(nh)
+    assert s.off[-1] * nh > 888
+    s.check(q, *_attend(s, q))
+
+
+TALL = [  # counts, lens, page, nh, nkv, hd, prefix, ahead, pad
+    ([1] * 64, [5 + 3 * b for b in range(64)], 16, 16, 4, 128, 3001, 0, 0),                # 256 rows a key head
+    ([1] * 65, [1] * 65, 64, 16, 4, 128, 2500, 0, 3),                                      # 260: four in a second segment
+    ([5] * 13, [70] * 13, 16, 6, 2, 64, 13501, 0, 0),
+    ([1] * 33, [40] * 33, 256, 12, 1, 128, 6017, 3, 1),                                    # 396 + rows ahead: 432
+    ([1] * 32, [9] * 32, 8, 1, 1, 64, 65541, 0, 0),                                        # 32 rows, many CTAs a segment
+    ([3, 0, 90, 1], [3, 9, 4000, 2], 48, 4, 1, 128, 5700, 0, 9),
+    ([1] * 150, [300 + b for b in range(150)], 32, 8, 8, 64, 2000, 1, 0),                  # own keys through all SMs
+]
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=str)
+@pytest.mark.parametrize("case", TALL, ids=str)
+def test_tall_prefix_every_row(case, dtype):
+    """Prefixes that the tensor cores take in 256-row tiles: every row, row tile borders among them."""
+    counts, lens, page, nh, nkv, hd, prefix, ahead, pad = case
+    s = Paged(counts, lens, page, nkv, hd, dtype, prefix, ahead, pad, seed=hd)
+    q = s.queries(nh)
+    assert hd >= 64 and s.rows * nh // nkv >= 32 and s.rows * nh * prefix >= 1 << 21
+    s.check(q, *_attend(s, q))
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.11, 0.9], ids=str)
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=str)
+def test_tall_prefix_scales(scale, dtype):
+    """head_dim 128: all keys alike, a negative scale, and one where a few keys take all and the maximum runs ahead."""
+    s = Paged([1] * 40, [30] * 40, 16, 2, 128, dtype, 4100, seed=2)
+    q = s.queries(8)
+    s.check(q, *_attend(s, q, scale), scale)
+
+
+# ------------------------------------------------------------------------- a prefix launch and what runs beside it
+def _layer(x, rope, s, i, wait):
+    """One layer of a decode pass: rotate and append, then attend; `wait` after each where given."""
+    q, k, v = x[i]
+    kv, lens = s.layers[i], s.d_lens
+    q = ops.rope_append(rope, kv, q, k, v, s.args[0], lens, s.args[2], prefix_len=s.prefix)
+    wait()
+    out, lse = ops.prefix_attention(kv, q, s.args[0], lens, *s.args[2:], lse=True)
+    wait()
+    return out, lse, q
+
+
+def _two_layers(hd, nh, nkv, B, prefix, own, dtype):
+    s = Paged([2] * B, [own] * B, 16, nkv, hd, dtype, prefix, seed=8)
+    k, v = (torch.nan_to_num(t, 0.5) for t in (s.kv.k, s.kv.v))
+    s.layers = [ops.PagedKV(k.clone(), v.clone()), ops.PagedKV(v.clone(), k.clone())]
+    s.d_lens = s.args[1].clone()
+    assert s.rows * nh * prefix >= 1 << 21
+    x = [[torch.zeros((s.rows, h, hd), dtype=dtype, device=DEV) for h in (nh, nkv, nkv)] for _ in range(2)]
+    return s, x
+
+
+def _fill(s, x, step):
+    g = torch.Generator(device=DEV)
+    g.manual_seed(step)
+    for t in (t for layer in x for t in layer):
+        t.copy_(torch.randn(t.shape, generator=g, device=DEV))
+    s.d_lens.copy_((s.args[1] - 5 * step).clamp_(min=2))
+
+
+SIZES = [(64, 8, 2, 40, 6600, 30), (128, 16, 4, 33, 4000, 700), (128, 8, 8, 64, 9000, 14)]
+
+
+@pytest.mark.parametrize("hd,nh,nkv,B,prefix,own", SIZES, ids=str)
+def test_tall_prefix_straight_behind_the_append(hd, nh, nkv, B, prefix, own):
+    """Two layers back to back, eagerly, on a side stream, and as two graphs that share a memory pool replayed
+    in turn on changing inputs: the bits of a run that waits after every call."""
+    s, x = _two_layers(hd, nh, nkv, B, prefix, own, BF16)
+    rope, none = ops.Rope(hd, layout="half"), lambda: None
+    run = lambda wait=none: [t for i in range(2) for t in _layer(x, rope, s, i, wait)]  # noqa: E731
+    was = [(kv.k.clone(), kv.v.clone()) for kv in s.layers]
+
+    def reset():
+        for kv, (k, v) in zip(s.layers, was):
+            kv.k.copy_(k)
+            kv.v.copy_(v)
+
+    want = []
+    for step in range(4):
+        reset()
+        _fill(s, x, step)
+        torch.cuda.synchronize()
+        want.append([t.clone() for t in run(torch.cuda.synchronize)])
+    for a, b in zip(want, want[1:]):
+        assert not torch.equal(a[0], b[0])
+    pool, graphs = torch.cuda.graph_pool_handle(), []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, pool=pool):
+            res = run()
+        graphs.append((g, res))
+    side = torch.cuda.Stream()
+    for step in (3, 0, 2, 1, 0, 3):
+        reset()
+        _fill(s, x, step)
+        got = run()
+        assert all(torch.equal(a, b) for a, b in zip(got, want[step]))
+        for g, res in graphs:
+            reset()
+            g.replay()
+            got = [t.clone() for t in res]
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(got, want[step]))
+        reset()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            got = run()
+        torch.cuda.current_stream().wait_stream(side)
+        assert all(torch.equal(a, b) for a, b in zip(got, want[step]))
+
+
+@pytest.mark.parametrize("hd,nh,nkv,B,prefix,own", SIZES, ids=str)
+def test_two_tall_calls_at_once(hd, nh, nkv, B, prefix, own):
+    """Two streams, each with calls of its own back to back."""
+    cases = [Paged([1] * B, [own + 9 * i] * B, 16, nkv, hd, F16, prefix + 100 * i, seed=i) for i in range(2)]
+    qs = [s.queries(nh) for s in cases]
+    want = [_attend(s, q) for s, q in zip(cases, qs)]
+    torch.cuda.synchronize()
+    sides, got = [torch.cuda.Stream() for _ in range(2)], []
+    for _ in range(10):
+        for s, q, w, st in zip(cases, qs, want, sides):
+            with torch.cuda.stream(st):
+                got.append((ops.prefix_attention(s.kv, q, *s.args, lse=True), w))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for g, w in got for a, b in zip(g, w))
+
+
+# ------------------------------------------------------------------------- the distribution of verified frames
+def test_verified_frames_follow_the_target():
+    """Drafts drawn from q and verified: the first frame's two tokens are distributed as p's product, the second's,
+    where there is one, again. 200000 streams a case: a count differs from n p by six sigma at most (2e-9 a cell)."""
+    V, C, B, g = 5, 2, 200000, _gen(12)
+    p1 = torch.softmax(torch.randn((3, C, V), generator=g), -1)
+    q1 = torch.softmax(torch.randn((2, C, V), generator=g), -1)
+    for q in (q1, None):
+        draft = torch.stack([torch.multinomial(q1[f, c].double(), B, True, generator=g) for f in range(2) for c in range(C)], 1)
+        draft = draft.reshape(B, 2, C).to(torch.int32)
+        if q is None:                                        # a certain draft: any token, here always the same
+            draft = torch.tensor([[[1, 3], [0, 2]]], dtype=torch.int32).expand(B, 2, C).contiguous()
+        u, r = torch.rand((B, 2, C), generator=g, dtype=F64), torch.rand((B, 3, C), generator=g, dtype=F64)
+        tok, kept = ops.verify_drafts(p1.to(DEV).expand(B, 3, C, V), None if q is None else q.to(DEV).expand(B, 2, C, V), *_dev(draft, u, r))
+        tok, kept = tok.cpu().long(), kept.cpu()
+        for f in range(3):
+            has = kept >= f
+            n = int(has.sum())
+            cells = torch.bincount(tok[has, f, 0] * V + tok[has, f, 1], minlength=V * V).double()
+            want = (p1[f, 0].double()[:, None] * p1[f, 1].double()).flatten()
+            assert n > 100 and ((cells - n * want).abs() <= 6 * (n * want * (1 - want)).sqrt() + 1).all(), (f, n)
