@@ -148,7 +148,9 @@ typedef struct z2b_prefix_attn_args {
  * stream's own pages up to the row's own; a row that sees none gives zeros and an lse of
  * -infinity. No two rows or heads of out share memory; it may lie across q. Products of 16-bit operands, sums and softmax statistics in f32, the
  * probabilities rounded to the cache's type for their product with V. Cache rows at or
- * behind seq_len and prefix_len may hold anything; those before must be finite. The result
+ * behind seq_len and prefix_len may hold anything; those before and the scores must be finite,
+ * and bf16 values of V below 2^80 (probabilities are held up to 2^15 ahead of their sum, so that
+ * small ones keep their bits). A query that is not a number has a result that is not. The result
  * does not depend on timing: the same call gives the same bits. */
 int z2b_prefix_attention(const z2b_prefix_attn_args* args, void* stream);
 /* Workspace bytes of a call with these sizes and this cache (no other pointer is looked at); 0 for

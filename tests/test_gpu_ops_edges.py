@@ -433,6 +433,18 @@ def test_tall_prefix_scales(scale, dtype):
     s.check(q, *_attend(s, q, scale), scale)
 
 
+def test_tall_values():
+    """bf16 values of up to 2^79 in V: sums over thousands of keys and probabilities held above 1 stay finite."""
+    for counts, prefix in (([1] * 3, 3000), ([1] * 40, 6600)):
+        s = Paged(counts, [40] * len(counts), 16, 2, 64, BF16, prefix, seed=3)
+        q = s.queries(8)
+        out, lse = _attend(s, q)
+        big = torch.tensor(2.0 ** 76, dtype=BF16, device=DEV)
+        s.kv.v.mul_(big)
+        got, glse = _attend(s, q)
+        assert torch.equal(got, out * big) and torch.equal(lse, glse)     # powers of two: the same bits
+
+
 # ------------------------------------------------------------------------- a prefix launch and what runs beside it
 def _layer(x, rope, s, i, wait):
     """One layer of a decode pass: rotate and append, then attend; `wait` after each where given."""

@@ -19,7 +19,7 @@ constexpr int MIN_UNITS = 2;           // line positions per worker at least, be
 constexpr int SEG_COST = 1, TC_SEG_COST = 3;
 // The reference m of a row's probabilities 2^(s - m) is its maximum less P_SHIFT, and stays until
 // the maximum is LAG above it: probabilities lie below 2^15, within f16, sums and O are f32, so
-// nothing overflows, rescaling O becomes rare, and the shift keeps small probabilities of f16
+// nothing overflows (bf16 values of V below 2^80: 2^15 of each of 2^30 keys), rescaling O becomes rare, and the shift keeps small probabilities of f16
 // caches off the bottom of its range (2^-31 of the largest is still there).
 constexpr float P_SHIFT = 7.0f, LAG = 15.0f;
 
