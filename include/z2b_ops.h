@@ -28,10 +28,10 @@
  *
  * Rows: stream b of n_seq owns the packed rows [row_off[b], row_off[b+1]) of the n_rows rows
  * of q (row_off[0] >= 0, ascending, row_off[n_seq] <= n_rows; rows ahead of row_off[0] and behind
- * row_off[n_seq] are padding that no call reads or writes). seq_len[b] counts the cached rows of the stream's
- * own pages, its new rows included: new row i of n is cache row seq_len[b] - n + i, which
- * lives in row (that % page_len) of page page_table[b * table_stride + that / page_len], and
- * its position is prefix_len + that.
+ * row_off[n_seq] are padding, which no call writes or lets into a result). seq_len[b] counts the
+ * cached rows of the stream's own pages, its new rows included: new row i of n is cache row
+ * seq_len[b] - n + i, which lives in row (that % page_len) of page
+ * page_table[b * table_stride + that / page_len], and its position is prefix_len + that.
  */
 #ifndef Z2B_OPS_H
 #define Z2B_OPS_H

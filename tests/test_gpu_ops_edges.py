@@ -563,3 +563,44 @@ def test_verified_frames_follow_the_target():
             cells = torch.bincount(tok[has, f, 0] * V + tok[has, f, 1], minlength=V * V).double()
             want = (p1[f, 0].double()[:, None] * p1[f, 1].double()).flatten()
             assert n > 100 and ((cells - n * want).abs() <= 6 * (n * want * (1 - want)).sqrt() + 1).all(), (f, n)
+
+
+# ------------------------------------------------------------------------- the largest numbers
+@pytest.mark.parametrize("hd,nh,nkv", [(16, 8, 1), (64, 16, 2), (128, 4, 1)], ids=str)
+def test_as_many_streams_as_a_call_takes(hd, nh, nkv):
+    """4096 streams, whose records leave the least room for the copies, behind a short and a tall prefix."""
+    B = 4096
+    for prefix in (20, 300):
+        s = Paged([1 if b % 8 else 0 for b in range(B)], [1 + b % 70 for b in range(B)], 16, nkv, hd, BF16, prefix, seed=hd)
+        q = s.queries(nh)
+        out, lse = _attend(s, q)
+        pick = list(range(0, B, 61)) + [B - 1]               # some of the streams against 64 bits
+        rows = [s.off[b] for b in pick if s.counts[b]]
+        t = Paged([1], [1], 16, nkv, hd, BF16, 0)
+        t.kv, t.prefix, t.shared = s.kv, prefix, s.shared
+        t.table, t.lens, t.counts = s.table[pick], [s.lens[b] for b in pick], [s.counts[b] for b in pick]
+        t.off = [sum(t.counts[:i]) for i in range(len(pick) + 1)]
+        t.check(q[rows], out[rows], lse[rows])
+
+
+def test_offsets_beyond_32_bits():
+    """Pages more than 2^32 elements apart, rows of q as well: appended and read back."""
+    hd, far = 64, (1 << 32) + 64
+    big = [torch.zeros(far + 32 * hd, dtype=F16, device=DEV) for _ in range(2)]
+    kv = ops.PagedKV(*(x.as_strided((2, 16, 2, hd), (far, 2 * hd, hd, 1)) for x in big))
+    g = _gen(30)
+    q, k, v = (torch.randn((2, h, hd), generator=g).to(F16).to(DEV) for h in (4, 2, 2))
+    wide = torch.zeros(far + 4 * hd, dtype=F16, device=DEV)
+    qs = wide.as_strided((2, 4, hd), (far, hd, 1))
+    qs.copy_(q)
+    small = ops.PagedKV(*(torch.zeros((2, 16, 2, hd), dtype=F16, device=DEV) for _ in range(2)))
+    meta = (_i32([0, 1, 2]), _i32([7, 9]), _i32([[0], [1]]))
+    rope = ops.Rope(hd)
+    want = ops.rope_append(rope, small, q, k, v, *meta)
+    assert torch.equal(ops.rope_append(rope, kv, qs, k, v, *meta, out=qs), want)
+    for a, b in ((kv.k, small.k), (kv.v, small.v)):
+        assert torch.equal(a, b)
+    o = ops.prefix_attention(small, want, *meta, _i32([1]), 12)
+    assert torch.equal(ops.prefix_attention(kv, qs, *meta, _i32([1]), 12, out=qs), o)
+    del big, wide, kv, qs
+    torch.cuda.empty_cache()
