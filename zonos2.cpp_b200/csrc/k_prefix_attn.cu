@@ -10,6 +10,17 @@
 //   own:    each stream's rows (its query heads of one key head side by side) over its pages.
 // Bound: the own part by HBM bytes, the prefix by tensor-core rate once the rows are many.
 //
+// Probabilities are rounded to the cache's type for their product with V, since the tensor cores take
+// 16-bit operands; taking them as a sum of two such would double those products. Against 64 bits the
+// result is 1.2 to 1.4 times as far off as with f32 probabilities (bf16 0.0023 of the output's size to
+// 0.0017, f16 0.00026 to 0.00021), the last rounding included. Sums and statistics are f32.
+//
+// Made for decode and draft rows. Prompt rows are right but far from the tensor cores' rate: their own
+// keys come here too, read again from L2 for every row tile. 2048 rows of one stream over themselves, 32
+// heads of 128 dims, take 394 us (87 TFLOP/s; the operations alone 21); 8 x 256 rows behind a prefix of
+// 8192, which k_prefix_tc.cu takes, 370 us (765 TFLOP/s). head_dim 16 and 32 never take that path: 64
+// streams of 16 heads behind a prefix of 8192 take 44 us with either, 26 with 64 dims.
+//
 // Work split: a unit is KU keys of one segment (row tile x key head). All units form one line
 // that is cut into equal contiguous ranges, one per worker, whatever the lengths; a worker
 // leaves one partial result per segment it touches. Partial slots are segment + worker: going
@@ -797,11 +808,13 @@ size_t up(size_t x) { return (x + 255) & ~(size_t)255; }
 // PF_LEAVES, where the second starts beside it (the tensor cores are power-bound and lose less than
 // their share of SMs, HBM would idle). While a CTA there takes one of its units an early CTA takes
 // some OWN_PER_PF; what the early ones do not get through, all SMs share when the prefix is done.
-// None / 36 left, us: 256 streams, 32 heads of 128, prefix 32768, own up to 600: 198 / 177 (212 / 206
-// over hundreds of passes, when the clocks have fallen); 64, 16 heads, 8192, up to 200: 48 / 38; up to
-// 4000: 105 / 93; 64 x 5 rows of 64 dims, 4097, up to 300: 42 / 40. With next to no own keys 64 dims
-// lose (256, 32768, up to 8: 71 / 80; 128 dims: 97 / 94). 16, 24, 32, 40 left, the first of these at 12
-// units: 219 (the early CTAs end last), 214, 182, 181.
+// None / 36 left, us: 256 streams, 32 heads of 128, prefix 32768, own up to 600: 197 / 173 (216 / 202
+// over hundreds of passes, when the clocks have fallen); 64, 16 heads, 8192, up to 200: 47 / 38; up to
+// 4000: 102 / 92; 64 x 5 rows of 64 dims, 4097, up to 300: 41 / 38. With next to no own keys 64 dims
+// lose (256, 16 heads, 32768, up to 8: 70 / 78; 128 dims: 93 / 91): the host does not see the lengths, and
+// the number stays one. 16, 24, 32, 40 left, the first of these at 12 units: 219 (the early CTAs end
+// last), 214, 182, 181 where 36 took 177. Where the early CTAs get through the whole line, the others
+// start behind the prefix all the same, find nothing and end.
 constexpr int PF_LEAVES = 36, OWN_PER_PF = 16;
 
 std::atomic<int> g_polls{-1};           // limit of a wait set by a test, or negative
@@ -821,10 +834,11 @@ HostPlan host_plan(const z2b_prefix_attn_args& a) {
     const long long R = (long long)a.n_rows * h.G;
     const int mt = 8 * h.nb;
     // The prefix on tcgen05 costs a launch and its filling (6 us), on the line a read of its keys per
-    // row tile. Calls of 4 key heads, head_dim 128, line / tcgen05 in us, R rows a key head, prefixes of
-    // 512, 2048, 8192, 32768: R 16: 9 / 15, 11 / 15, 14 / 17, 25 / 32; R 32: 10 / 15, 11 / 16, 16 / 18,
-    // 36 / 32; R 64: 11 / 16, 13 / 17, 22 / 19, 61 / 34; R 256: 20 / 29, 31 / 33, 70 / 38, 218 / 55; and
-    // at head_dim 64: R 64: 9 / 14, 10 / 14, 18 / 16, 41 / 27; R 256: 17 / 23, 23 / 25, 48 / 27, 142 / 40
+    // row tile. Calls of 4 key heads, up to 8 own keys, head_dim 128, line / tcgen05 in us, R rows a key
+    // head, prefixes of 512, 2048, 8192, 32768: R 16: 9 / 14, 11 / 14, 15 / 16, 27 / 29; R 32: 10 / 14,
+    // 11 / 14, 17 / 16, 42 / 30; R 64: 11 / 15, 13 / 15, 25 / 17, 74 / 31; R 256: 17 / 27, 31 / 25, 84 / 36,
+    // 293 / 52; and at head_dim 64: R 32: 8 / 12, 9 / 12, 13 / 14, 26 / 25; R 64: 10 / 12, 10 / 13, 17 / 15,
+    // 46 / 25; R 256: 15 / 22, 23 / 19, 55 / 25, 180 / 38
     h.pf_tc = hd >= 64 && R >= 32 && (double)a.n_rows * a.n_head * a.prefix_len >= 2097152.0;
     const int pf_tiles = a.prefix_len > 0 && !h.pf_tc ? (int)((R + mt - 1) / mt) : 0;
     h.own = PartSet{nullptr, nullptr, mt, unit_keys(hd), CTAS * h.warps, 0, pf_tiles};

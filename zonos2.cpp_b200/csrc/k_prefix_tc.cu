@@ -32,8 +32,9 @@ namespace z2b {
 namespace {
 
 // Three warpgroups: two of softmax, one of TMA (warp 8) and MMA (warp 9). Launched at 168
-// registers a thread (384 x 168 = 64512); the third keeps 80 so that the softmax rows' 128
-// scores fit 208: 256 x 208 + 128 x 80 = 63488.
+// registers a thread (384 x 168 = 64512); the third keeps 80 and the softmax rows, which hold 128
+// scores each, get 208: 256 x 208 + 128 x 80 = 63488. At head_dim 128 that still leaves 52 bytes a thread
+// in local memory (112 read back), 8 at 64.
 constexpr int TC_THREADS = 384;
 
 __device__ __forceinline__ uint32_t idesc_t(bool bf16, int n, bool b_mn) {
