@@ -350,7 +350,7 @@ class Paged:
             x = q[lo: lo + n].double().reshape(n, nkv, G, hd).permute(1, 0, 2, 3).reshape(nkv, n * G, hd)
             most = max(most, float((x.abs() @ k.abs().transpose(1, 2)).max()) * abs(scale))
             s = (x @ k.transpose(1, 2)).reshape(nkv, n, G, -1) * scale
-            sees = torch.arange(k.shape[1], device=DEV)[None] < self.prefix + L - n + 1 + torch.arange(n, device=DEV)[:, None]
+            sees = torch.arange(k.shape[1], device=DEV)[None] < self.prefix + (L - n + 1 + torch.arange(n, device=DEV)[:, None]).clamp(min=0)
             s = s.masked_fill(~sees[None, :, None], -math.inf)
             p = torch.softmax(s, -1).nan_to_num(0.0).reshape(nkv, n * G, -1)      # a row that sees no key: zeros
             back = lambda y: y.reshape(nkv, n, G, -1).permute(1, 0, 2, 3).reshape(n, nkv * G, -1)  # noqa: E731
