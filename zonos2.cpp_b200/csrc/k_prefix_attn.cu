@@ -293,6 +293,7 @@ __global__ void __launch_bounds__(32 * max_warps(HD), 1) prefix_attn_kernel(cons
 
     int it = 0;
     bool dead = false;                                           // a wait ran out
+    const bool quick = p.polls > 0;                              // read here, not on the first wait's way
     Seg g;
     if (u < u1) {
         g = find_seg<MT, KU>(p, ln, u);
@@ -343,7 +344,8 @@ __global__ void __launch_bounds__(32 * max_warps(HD), 1) prefix_attn_kernel(cons
             const int key0 = (u - g.unit0) * KU;
             if (key0 >= g.lim_max) { u = end; break; }           // no row of the tile sees the rest
             const int st = it % NS;
-            if (!dead) dead = __any_sync(0xffffffffu, !mbar_wait(&full[st], (it / NS) & 1, p.err, p.polls));
+            if (!dead)
+                dead = __any_sync(0xffffffffu, !((quick && mbar_try_wait(&full[st], (it / NS) & 1)) || mbar_wait(&full[st], (it / NS) & 1, p.err, p.polls)));
             if (dead) {                                          // this and the range's other segments: not numbers
 #pragma unroll
                 for (int nb_ = 0; nb_ < NB; ++nb_) l[nb_][0] = l[nb_][1] = NAN;
@@ -777,8 +779,8 @@ __global__ void __launch_bounds__(256, 4) prefix_attn_join_few_kernel(const __gr
     if (warp > 0) return;
     for (int w = 1; w < W; ++w) {
         const float top = fmaxf(M, s_acc[w][HD]);
-        if (top == -INFINITY) { L += s_acc[w][HD + 1]; continue; }       // no key seen: a sum of 0, or none
-        const float f = ex2(M - top), fw = ex2(s_acc[w][HD] - top);
+        const float to = top == -INFINITY ? 0.0f : top;          // no key seen
+        const float f = ex2(M - to), fw = ex2(s_acc[w][HD] - to);
         M = top;
         L = L * f + s_acc[w][HD + 1] * fw;
         if (HD >= 32 || lane < HD)

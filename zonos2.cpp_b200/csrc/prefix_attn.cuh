@@ -28,7 +28,6 @@ struct AttnP {
     long long q_row, q_head, table_stride;
     const int *row_off, *seq_len, *table, *prefix_pages;
     uint32_t* err;
-    uint32_t polls;                    // limit of a wait
     int n_rows, n_seq, nkv, G, page_len, n_pages, max_pages, prefix_len;
     uint32_t g_mul;                    // ceil(2^32 / G), for quotients by G of numbers x with x G < 2^32
     int box_rows, box_halves;          // rows of one TMA box (a power of two that divides page_len, at most a
@@ -39,6 +38,7 @@ struct AttnP {
     int early, head_start;             // CTAs that find an SM while that one runs, and line positions each gets through meanwhile
     float* part_o;                     // [slots][rows of a segment][head_dim]
     float2* part_ml;                   // [slots][rows of a segment] (m in log2 units, l)
+    uint32_t polls;                    // limit of a wait
     int* plan;                         // [2][n_seq + 1] unit and segment offsets of the streams, written for the join
 };
 
