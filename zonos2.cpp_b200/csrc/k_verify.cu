@@ -52,6 +52,9 @@ __device__ __forceinline__ double left_at(const T* __restrict__ p, const T* __re
     else return fmax(x, 0.0);
 }
 
+// A number drawn with, in [0, 1]: below, the first token with mass is drawn, else out of range the last.
+__device__ __forceinline__ double unit(double r) { return r < 0.0 ? 0.0 : r < 1.0 ? r : 1.0; }
+
 __device__ __forceinline__ double warp_sum_f64(double v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -65,8 +68,8 @@ template <int WARPS> struct DrawShared {
     int found, last;
 };
 
-// The drawn token of a row of at most 32 WARPS EACH entries, or NO_MASS. r in [0, 1]. Called by
-// the whole CTA; all threads get it.
+// The drawn token of a row of at most 32 WARPS EACH entries, or NO_MASS. Called by the
+// whole CTA; all threads get it.
 template <typename T, bool HAS_Q, bool SUB, int WARPS>
 __device__ int draw_small(const T* p, const T* q, int V, int drafted, double r, DrawShared<WARPS>& sh) {
     const int w = threadIdx.x >> 5, lane = threadIdx.x & 31, each = (V + 32 * WARPS - 1) / (32 * WARPS);
@@ -93,7 +96,7 @@ __device__ int draw_small(const T* p, const T* q, int V, int drafted, double r, 
         total += sh.warp_tot[i];
     }
     if (!(total > 0.0)) return NO_MASS;
-    const double target = r * total;
+    const double target = unit(r) * total;
     before += inc - mine;
     if (mine > 0.0) {
         int last = -1, first = 0x7fffffff;
@@ -114,7 +117,7 @@ __device__ int draw_small(const T* p, const T* q, int V, int drafted, double r, 
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
 
-// The drawn token, r in [0, 1]. Called by every thread of the cluster, all of whose CTAs have
+// The drawn token. Called by every thread of the cluster, all of whose CTAs have
 // started. NO_MASS comes from the cluster's total alone, so that its CTAs agree whether another draw
 // (with its barriers) follows; else the CTA whose range holds the target gets the token and the others
 // ELSEWHERE. That range has mass: the target is at least 0, so a range whose sum takes the running
@@ -156,7 +159,7 @@ __device__ int draw_large(const T* p, const T* q, int V, int drafted, double r, 
         total += cta[i];
     }
     if (!(total > 0.0)) return NO_MASS;
-    const double target = r * total;
+    const double target = unit(r) * total;
     double run = 0.0;
 #pragma unroll
     for (int i = 0; i < MAX_CLUSTER; ++i) {
@@ -277,11 +280,7 @@ __global__ void __launch_bounds__(32 * WARPS) verify_kernel(const __grid_constan
         if (rank == 0 && threadIdx.x == 0) out[end * C] = x;
         return;
     }
-    double r = a.u_draw[((long long)b * (N + 1) + end) * C + c];
-    if (!(r >= 0.0 && r < 1.0)) {                                // below: the first token with mass, else the last
-        if (rank == 0 && threadIdx.x == 0 && a.err) atomicOr(a.err, Z2B_OPS_BAD_INDEX);
-        r = r < 0.0 ? 0.0 : 1.0;
-    }
+    const double r = a.u_draw[((long long)b * (N + 1) + end) * C + c];
     const T* pr = p + end * a.p_frame + c * a.p_book;
     const T* qr = HAS_Q && end < n ? q + end * a.q_frame + c * a.q_book : nullptr;
     int tok = NO_MASS;
@@ -292,6 +291,8 @@ __global__ void __launch_bounds__(32 * WARPS) verify_kernel(const __grid_constan
         if (end < n) tok = draw_large<T, HAS_Q, true, WARPS>(pr, qr, V, x, r, rank, n_cta, 0, sh);
         if (tok == NO_MASS) tok = draw_large<T, HAS_Q, false, WARPS>(pr, nullptr, V, -1, r, rank, n_cta, 1, sh);
     }
+    // looked at last: the rows are not to wait for it
+    if (rank == 0 && threadIdx.x == 0 && a.err && !(r >= 0.0 && r < 1.0)) atomicOr(a.err, Z2B_OPS_BAD_INDEX);
     // a row without any mass has no token (-1); its first CTA says so
     if (threadIdx.x == 0 && (tok >= 0 || (tok == NO_MASS && rank == 0))) out[end * C] = tok;
 }
