@@ -80,14 +80,11 @@ __global__ void __launch_bounds__(32 * WARPS) rope_append_ops_kernel(const __gri
     }
     // a stream whose offsets cannot be is left out whole; offsets that descend may still name a row
     // for a stream whose own are sound
-    if (lo < 0 || hi < lo || hi > total || hi > p.n_rows || (t < lo && b > 0)) {
-        if (lane == 0 && p.err) atomicOr(p.err, Z2B_OPS_BAD_INDEX);
-        return;
-    }
-    if (t < lo || t >= total) return;                                // ahead of the first stream, padding: stays as it is
-    const long long r = (long long)len - (hi - lo) + (t - lo);       // cache row
-    if (t >= hi || r < 0 || (p.k && r >= (long long)p.max_pages * p.page_len)) {
-        if (lane == 0 && p.err) atomicOr(p.err, Z2B_OPS_BAD_INDEX);
+    const bool broken = lo < 0 || hi < lo || hi > total || hi > p.n_rows || (t < lo && b > 0);
+    const long long r = (long long)len - hi + t;                     // cache row
+    if (broken || t < lo || t >= hi || r < 0 || (p.k && r >= (long long)p.max_pages * p.page_len)) {
+        // rows ahead of the first stream and padding stay as they are
+        if ((broken || (t >= lo && t < total)) && lane == 0 && p.err) atomicOr(p.err, Z2B_OPS_BAD_INDEX);
         return;
     }
     const long long at = p.pos ? (long long)p.pos[t] : (long long)p.prefix_len + r;
