@@ -11,7 +11,7 @@
 // CTA, or a cluster of them for large vocabularies, takes one (stream, codebook): every CTA
 // finds the run's end for itself (a handful of gathers). Then
 //   small rows: a thread holds up to EACH consecutive entries; one block scan finds the draw (1026
-//   entries: 3.1 us, where a first pass for the sum and a second for the draw took 4.6);
+//   entries: 3.0 us, where a first pass for the sum and a second for the draw took 4.6);
 //   large rows: the row is split over the cluster, each warp summing one contiguous share with
 //   lanes side by side; the totals are exchanged through distributed shared memory, and the one
 //   CTA whose range holds the target scans the one warp's share that does.
