@@ -122,3 +122,21 @@ def test_attention_refuses_results_that_share_memory():
     # the keys may be the values there, and pages may repeat: they are only read
     a = _attn(_view(page_stride=0, **view), device=NO_DEVICE, workspace_bytes=1 << 40)
     assert _call("z2b_prefix_attention", a)[0] != ARG
+
+
+def test_append_takes_rows_that_run_backwards():
+    """Negative strides of q, q_out, k and v name the same boxes from their other end."""
+    import random
+    rng = random.Random(6)
+    seen = {True: 0, False: 0}
+    for _ in range(3000):
+        pick = lambda: (rng.randrange(200, 360), rng.choice((-24, -8, 8, 16, 24)), rng.choice((-12, -4, 4, 8, 12)))  # noqa: E731
+        q, o, k, v = pick(), pick(), pick(), pick()
+        o = q if rng.random() < 0.2 else o
+        rc, msg, shared = _append_boxes(q, o, k, v, 1000, 1024, (48, 8, 4))
+        seen[shared] += 1
+        assert (rc == ARG) == shared, (q, o, k, v, msg)
+    assert min(seen.values()) > 300
+    for row, head, ok in ((-256, 64, True), (-256, -64, True), (-64, 64, False), (-96, -64, False)):
+        a = _attn(_view(), device=NO_DEVICE, n_rows=3, n_head=2, o_row=row, o_head=head, workspace_bytes=1 << 40)
+        assert (_call("z2b_prefix_attention", a)[0] == ARG) == (not ok)

@@ -68,22 +68,28 @@ bool reaches(const Var* v, int n, long long delta, int* steps) {
 
 struct Box {
     const void* p;
-    int n = 0;
-    long long stride[4], len[4], last = 0;       // last: offset of the last element
-    bool real = true;                            // false: it ends beyond any address, there is nothing to compare
-    Box(const void* p_, std::initializer_list<std::pair<long long, long long>> dims) : p(p_) {
-        __int128 end = 0;
+    int n = 0, size;
+    bool back[4];                                // a dim that runs backwards: taken from its other end
+    long long stride[4], len[4], first = 0, last = 0;       // elements from p to the lowest one, from that to the highest
+    bool real;                                   // false: it spans more than addresses do, there is nothing to compare
+    // `size` bytes an element, aligned to it
+    Box(const void* p_, int size_, std::initializer_list<std::pair<long long, long long>> dims) : p(p_), size(size_) {
+        __int128 low = 0, span = 0;
         for (const auto& d : dims) {
             if (d.second <= 1) continue;         // a dim of one has no stride
-            stride[n] = d.first;
+            const __int128 far = (__int128)d.first * (d.second - 1);
+            back[n] = far < 0;
+            if (far < 0) low += far;
+            span += far < 0 ? -far : far;
+            stride[n] = far < 0 ? -d.first : d.first;
             len[n++] = d.second;
-            end += (__int128)d.first * (d.second - 1);
         }
-        real = end >= 0 && end < 1ll << 56;
-        if (real) last = (long long)end;
+        real = span < 1ll << 56;
+        if (real) { first = (long long)low; last = (long long)span; }
     }
     bool same_place(const Box& o) const {
-        return p == o.p && n == o.n && std::equal(stride, stride + n, o.stride) && std::equal(len, len + n, o.len);
+        return p == o.p && n == o.n && std::equal(stride, stride + n, o.stride) && std::equal(back, back + n, o.back) &&
+               std::equal(len, len + n, o.len);
     }
 };
 bool steeper(const Var& a, const Var& b) { return a.stride > b.stride; }
@@ -92,7 +98,7 @@ bool steeper(const Var& a, const Var& b) { return a.stride > b.stride; }
 bool shares_itself(const Box& b) {
     Var v[4];
     for (int i = 0; i < b.n; ++i) {
-        if (b.stride[i] <= 0) return true;
+        if (b.stride[i] == 0) return true;
         v[i] = Var{b.stride[i], 1 - b.len[i], b.len[i] - 1};
     }
     if (!b.real) return false;
@@ -111,15 +117,15 @@ bool shares_itself(const Box& b) {
     return false;
 }
 
-// Some element of one is an element of the other; both of `size` bytes an element, aligned to it.
-bool share(const Box& a, const Box& b, int size) {
-    const long long d = (long long)((uintptr_t)b.p - (uintptr_t)a.p) / size;
+// Some element of one is an element of the other, of the same size.
+bool share(const Box& a, const Box& b) {
+    const long long d = (long long)((uintptr_t)b.p - (uintptr_t)a.p) / a.size + b.first - a.first;
     if (!a.real || !b.real || d > a.last || -d > b.last) return false;
     Var v[8];
     int n = 0;
-    for (int i = 0; i < a.n; ++i) if (a.stride[i] > 0) v[n++] = Var{a.stride[i], 0, a.len[i] - 1};
+    for (int i = 0; i < a.n; ++i) if (a.stride[i]) v[n++] = Var{a.stride[i], 0, a.len[i] - 1};
     for (int i = 0; i < b.n; ++i) {
-        if (b.stride[i] <= 0) continue;          // an input's dim without a stride stays where it is
+        if (!b.stride[i]) continue;              // an input's dim without a stride stays where it is
         int j = 0;
         while (j < n && v[j].stride != b.stride[i]) ++j;
         if (j == n) v[n++] = Var{b.stride[i], 0, 0};
@@ -207,7 +213,7 @@ int z2b_rope_append(const z2b_rope_append_args* args, void* stream) {
     if (a.n_seq > OPS_MAX_SEQ) return unsupported("rope_append: more than 4096 streams");
     if (a.n_rows > (1 << 30) || a.n_head > (1 << 20) || a.kv->n_head_kv > (1 << 20))    // row and head numbers are 32-bit
         return unsupported("rope_append: too many rows or heads for one call");
-    const unsigned e = type_size(a.type);
+    const int e = (int)type_size(a.type);
     if (!aligned(a.q, e) || !aligned(a.q_out, e) || !aligned(a.k, e) || !aligned(a.v, e) || !aligned(a.pos, 4))
         return bad("rope_append: misaligned array");
     if (a.n_rows == 0 || a.n_seq == 0 || (a.n_head == 0 && !a.k)) return Z2B_OK;
@@ -215,19 +221,19 @@ int z2b_rope_append(const z2b_rope_append_args* args, void* stream) {
     if (*m) return bad(m);
     // rows are turned and stored at the same time, in any order
     const z2b_paged_kv& c = *a.kv;
-    const Box out(a.n_head ? a.q_out : nullptr, {{a.o_row, a.n_rows}, {a.o_head, a.n_head}, {1, c.head_dim}});
+    const Box out(a.n_head ? a.q_out : nullptr, e, {{a.o_row, a.n_rows}, {a.o_head, a.n_head}, {1, c.head_dim}});
     if (out.p) {
-        const Box q(a.q, {{a.q_row, a.n_rows}, {a.q_head, a.n_head}, {1, c.head_dim}});
+        const Box q(a.q, e, {{a.q_row, a.n_rows}, {a.q_head, a.n_head}, {1, c.head_dim}});
         if (shares_itself(out)) return bad("rope_append: rows or heads of q_out share memory");
-        if (!out.same_place(q) && share(out, q, e)) return bad("rope_append: q_out lies across q");
+        if (!out.same_place(q) && share(out, q)) return bad("rope_append: q_out lies across q");
     }
     if (a.k) {
-        const Box k(a.k, {{a.k_row, a.n_rows}, {a.k_head, c.n_head_kv}, {1, c.head_dim}});
-        const Box v(a.v, {{a.v_row, a.n_rows}, {a.v_head, c.n_head_kv}, {1, c.head_dim}});
-        if (out.p && (share(out, k, e) || share(out, v, e))) return bad("rope_append: q_out lies across k or v");
-        const Box kc(c.k, {{c.page_stride, c.n_pages}, {c.row_stride, c.page_len}, {c.head_stride, c.n_head_kv}, {1, c.head_dim}});
-        const Box vc(c.v, {{c.page_stride, c.n_pages}, {c.row_stride, c.page_len}, {c.head_stride, c.n_head_kv}, {1, c.head_dim}});
-        if (shares_itself(kc) || share(kc, vc, 2)) return bad("rope_append: pages, rows, heads or keys and values of the cache share memory");
+        const Box k(a.k, e, {{a.k_row, a.n_rows}, {a.k_head, c.n_head_kv}, {1, c.head_dim}});
+        const Box v(a.v, e, {{a.v_row, a.n_rows}, {a.v_head, c.n_head_kv}, {1, c.head_dim}});
+        if (out.p && (share(out, k) || share(out, v))) return bad("rope_append: q_out lies across k or v");
+        const Box kc(c.k, 2, {{c.page_stride, c.n_pages}, {c.row_stride, c.page_len}, {c.head_stride, c.n_head_kv}, {1, c.head_dim}});
+        const Box vc(c.v, 2, {{c.page_stride, c.n_pages}, {c.row_stride, c.page_len}, {c.head_stride, c.n_head_kv}, {1, c.head_dim}});
+        if (shares_itself(kc) || share(kc, vc)) return bad("rope_append: pages, rows, heads or keys and values of the cache share memory");
     }
     DeviceGuard g(a.device);
     if (g.rc != cudaSuccess) return launched(g.rc, "rope_append: device: ");
@@ -284,7 +290,7 @@ int z2b_prefix_attention(const z2b_prefix_attn_args* args, void* stream) {
     if (a.prefix_len > 0 && !a.prefix_pages) return bad("prefix_attention: null prefix_pages");
     if (!a.workspace || !aligned(a.workspace, 16)) return bad("prefix_attention: the workspace must be 16-byte aligned");
     if (a.workspace_bytes < prefix_attention_bytes(a)) return bad("prefix_attention: the workspace is too small");
-    if (shares_itself(Box(a.out, {{a.o_row, a.n_rows}, {a.o_head, a.n_head}, {1, c.head_dim}})))
+    if (shares_itself(Box(a.out, 2, {{a.o_row, a.n_rows}, {a.o_head, a.n_head}, {1, c.head_dim}})))
         return bad("prefix_attention: rows or heads of out share memory");
     DeviceGuard g(a.device);
     if (g.rc != cudaSuccess) return launched(g.rc, "prefix_attention: device: ");
