@@ -140,3 +140,7 @@ def test_append_takes_rows_that_run_backwards():
     for row, head, ok in ((-256, 64, True), (-256, -64, True), (-64, 64, False), (-96, -64, False)):
         a = _attn(_view(), device=NO_DEVICE, n_rows=3, n_head=2, o_row=row, o_head=head, workspace_bytes=1 << 40)
         assert (_call("z2b_prefix_attention", a)[0] == ARG) == (not ok)
+
+
+def test_a_context_that_is_not_read_may_be_anything():
+    assert ops.Rope(64, orig_ctx=-1).table.step[1] == ops.Rope(64).table.step[1]

@@ -9,9 +9,9 @@ tensor of one element on the device that the kernels OR ``BAD_INDEX``, ``BAD_PAG
 
 Rows are packed over the streams: stream b owns rows [row_off[b], row_off[b + 1]) of q
 [rows][heads][head_dim], rows ahead of row_off[0] and from row_off[-1] on are padding and stay as they
-are, seq_len[b] counts the stream's cached rows with the new ones, and page_table[b] lists its pages. There is no
-backward pass and no forward-mode gradient: tensors that want one or carry a tangent are refused, and
-autograd does not see what is written in place (the pages, `out`, `lse`).
+are, seq_len[b] counts the stream's cached rows with the new ones, and page_table[b] lists its pages.
+There is no backward pass and no forward-mode gradient: tensors that want one or carry a tangent are
+refused, and autograd does not see what is written in place (the pages, `out`, `lse`).
 """
 from __future__ import annotations
 
@@ -73,8 +73,8 @@ class Rope:
                  factor: float = 1.0, orig_ctx: int = 0):
         if layout not in _LAYOUT or scaling not in _SCALING:
             _refuse("rope: layout is 'interleaved' or 'half', scaling 'none', 'linear', 'ntk' or 'by_parts'")
-        if not all(0 <= int(x) < 2 ** 31 for x in (rot_dim, orig_ctx)):      # ctypes would wrap them
-            _refuse("rope: rot_dim and orig_ctx are numbers from 0 to 2^31 - 1")
+        if not all(-2 ** 31 <= int(x) < 2 ** 31 for x in (rot_dim, orig_ctx)):      # ctypes would wrap them
+            _refuse("rope: rot_dim and orig_ctx are 32-bit numbers")
         self.table = RopeTable()
         self._at = ctypes.addressof(self.table)
         f = lib().z2b_rope_init
@@ -119,9 +119,9 @@ class PagedKV:
 def rope_append(rope: Rope | None, kv: PagedKV, q, k, v, row_off, seq_len, page_table, prefix_len: int = 0, pos=None,
                 out=None, err=None):
     """Rotate q and k and append k and v to the pages (z2b_rope_append); returns the rotated q
-    (`out` when given, which may be q, or lie apart from q, k and v). q may be None (nothing returned), k and v may be None (only
-    q turns); rope None stores unrotated keys. `pos` [rows] int32 replaces the positions prefix_len +
-    cache row. A new result is contiguous, and its padding rows are not written."""
+    (`out` when given, which may be q, or lie apart from q, k and v). q may be None (nothing returned), k
+    and v may be None (only q turns); rope None stores unrotated keys. `pos` [rows] int32 replaces the
+    positions prefix_len + cache row. A new result is contiguous, and its padding rows are not written."""
     return _rope_append(rope._at if rope is not None else 0, kv._at, kv._idx, q, k, v, row_off, seq_len, page_table, prefix_len,
                         pos, out, err)
 
@@ -141,7 +141,7 @@ def verify_drafts(p, q, draft, u_accept, u_draw, n_draft=None, err=None):
     """Keep or replace drafted frames (z2b_verify_drafts). p [streams][drafts + 1][codebooks][vocab]:
     the target's probabilities; q [streams][drafts][codebooks][vocab]: the draft's, or None when it put
     all on the drafted token; draft int32 and u_accept float64 [streams][drafts][codebooks]; u_draw
-    float64 [streams][drafts + 1][codebooks]; n_draft [streams] int32. Returns (tokens int32
+    float64 [streams][drafts + 1][codebooks], both in [0, 1); n_draft [streams] int32. Returns (tokens int32
     [streams][drafts + 1][codebooks], accepted frames int32 [streams]); tokens behind the frame after
     the accepted ones are -1."""
     return _verify_drafts(p, q, draft, u_accept, u_draw, n_draft, err)
